@@ -294,8 +294,9 @@ def _plain_inputs(s):
     add, need, back = (t - c).clamp(min=0), (want - have).clamp(min=0), (have - want).clamp(min=0)
     free = s.num_free.long().clamp(0, s.free.numel())
     top = free + back.sum()
-    granted = (add.cumsum(0) <= s.tokens) & ((need == 0) | (need.cumsum(0) <= top))
-    add, need = add * granted, need * granted
+    fits = add.cumsum(0) <= s.tokens
+    granted = fits & ((need == 0) | (need.cumsum(0) <= top))  # the others stay as they are
+    add, need = add * fits, need * granted
     lens = torch.where((t < c) | granted, t, c)
     zero = torch.zeros(1, dtype=torch.long, device=dev)
     cu_q, cu_k = torch.cat([zero, add.cumsum(0)]), torch.cat([zero, lens.cumsum(0)])
@@ -322,7 +323,7 @@ def _plain_inputs(s):
     place = c[row] + token - cu_q[row]
     block = tables[row, (place // bs).clamp(0, width - 1)].long()
     slot = block * bs + place % bs
-    slots = torch.where(real & (block >= 0) & (slot < s.slots), slot, -1)
+    slots = torch.where(real & granted[row] & (block >= 0) & (slot < s.slots), slot, -1)
     positions = place if s.mask is None else c[row] + (_popcount(s.mask) - 1).clamp(min=0)
     positions = torch.where(real, positions, 0)
     return (tables, s.free, positions, slots.int(), cu_q.int(), cu_k.int(), (cu_q[1:] - 1).clamp(min=0).int(), lens.int(), left.int())
