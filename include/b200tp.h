@@ -364,6 +364,34 @@ int b2_advance_decode(const int64_t* tokens, int64_t* input_ids, int64_t* positi
                       int32_t* slot_mapping, const int32_t* block_tables, int64_t bt_stride, int bt_width,
                       int block_size, int64_t num_slots, int n, void* stream);
 
+/* ---- a step's inputs from the requests' lengths, computed on the device: what
+ *      ModelRunner.prepare_prefill / prepare_decode build on the host
+ *      (nanovllm/engine/model_runner.py:129-188), with the blocks that
+ *      BlockManager hands out and takes back (nanovllm/engine/block_manager.py) --
+ * Row i of block_tables (int32 [n, bt_width], row stride bt_stride) belongs to a request with cached_lens[i] tokens in the
+ * cache that is to have seq_lens[i].  A longer one gets the blocks it lacks from the stack free_blocks (int32 [free_capacity], the
+ * *num_free lowest are free, taken from the top) and its new tokens get places; a shorter one gives blocks back and gets none.
+ * What is given back is on top of the stack, in the order of the rows, when the granted rows take from it, in theirs.
+ * Outputs:
+ *   positions [max_tokens] int64, slot_mapping [max_tokens] int32: of the new tokens, row after row; 0 and -1 behind them
+ *   cu_seqlens_q [n + 1]: new tokens before each row; cu_seqlens_k [n + 1]: the same of context_lens
+ *   last_token_index [n]: cu_seqlens_q[i + 1] - 1, never below 0
+ *   context_lens [n]: seq_lens[i], or cached_lens[i] of a row that was not served;  *num_free_out: blocks that are free now
+ * block_tables and free_blocks are updated in place: entries past a row's blocks, and places of the stack above its top, keep what they
+ * held.  No output may overlap an input.  The other inputs are not changed, so that the same call again gives the same results.
+ * tree_mask (may be NULL): int64 [>= max_tokens, mask_words] with row stride mask_stride, the new tokens' ancestors as for b2_tree_attention;
+ * a token's position is then cached_lens[i] + its visible nodes - 1 (its depth), not below cached_lens[i]; its slot stays in the tokens' order.
+ * A row is not served when more than max_tokens are asked for by it and those before it - it then has no tokens - or when it needs
+ * blocks and more than there are are asked for by it and those before it - its tokens then keep their places with slot -1 -; its
+ * length and blocks stay.  A token whose table entry is negative or whose slot would be >= num_slots gets slot -1.  A row with a length
+ * that is negative or more than bt_width * block_size counts as a row without tokens.  A block may belong to one row only.
+ * n <= 8192 and n * bt_width * block_size < 2^31 (B2_ERR_SHAPE otherwise). */
+int b2_batch_inputs(int32_t* block_tables, int64_t bt_stride, int bt_width, const int32_t* cached_lens, const int32_t* seq_lens, int n,
+                    int32_t* free_blocks, int free_capacity, const int32_t* num_free, int block_size, int64_t num_slots, int max_tokens,
+                    const int64_t* tree_mask, int64_t mask_stride, int mask_words, int64_t* positions, int32_t* slot_mapping,
+                    int32_t* cu_seqlens_q, int32_t* cu_seqlens_k, int32_t* last_token_index, int32_t* context_lens, int32_t* num_free_out,
+                    void* stream);
+
 /* ---- elementwise neighbours of the path (the reference generates these with
  *      torch.compile -> Triton) ----------------------------------------------
  * SiluAndMul.forward (nanovllm/layers/activation.py:8-11):
@@ -402,7 +430,7 @@ int b2_rope(const void* q, int64_t ldq, const void* k, int64_t ldk, int M, int n
  *   out = softmax(scale q K^T) V over the sequence's first context_lens tokens,
  * fp32 scores and sums, probabilities rounded to bf16 for the second product.  Lengths and tables
  * are read on the device, so a captured call serves any later batch of the same size; they are read while earlier
- * b2_* kernels of the stream may still be running, so they must not be results of one, b2_advance_decode excepted.
+ * b2_* kernels of the stream may still be running, so they must not be results of one, b2_advance_decode and b2_batch_inputs excepted.
  * Calls of one context must be stream-ordered: they share its workspace for partial results.  scale: of either sign, or zero.
  * b2_paged_attention_supported says (1 / 0) whether the shape is served: head_dim 128, blocks of a
  * multiple of 64 tokens, at most 1024 sequences, one or two query heads per KV head, or up to eight where n_seqs * nkv >= 128. */
@@ -451,6 +479,56 @@ int b2_prefill_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const voi
                          const int32_t* cu_k, int n_seqs, int max_q, int tokens, int nq, int nkv, int head_dim, float scale,
                          void* out, void* stream);
 int b2_prefill_attention_supported(int nq, int nkv, int head_dim, int block_size);
+
+/* ---- attention of a tree of drafted tokens per sequence over the paged cache (the verification step of speculative decoding;
+ *      no counterpart in the reference, whose decode step has one query token per sequence, nanovllm/layers/attention.py:70-74) --
+ * q [tokens, nq, head_dim] bf16 (row stride q_stride): sequence b's nodes are rows cu_q[b] .. cu_q[b+1].  Their keys and values are in the
+ * cache already: context_lens[b] counts them, node k of t is at place context_lens[b] - t + k, and all places before the tree are seen by
+ * every node.  tree_mask int64 [tokens, mask_words] (row stride mask_stride): bit k % 64 of word k / 64 of a row says that the
+ * node sees node k of its sequence, itself included; bits past the tree are ignored, nodes past 64 * mask_words are not seen.
+ *   out = softmax(scale q K^T over what the node sees) V, [tokens, nq, head_dim] contiguous, fp32 scores and sums
+ * What a node does not see may hold anything.  A node that sees nothing, rows of a sequence whose context is shorter than its tree
+ * (0: a padded sequence) and rows behind the last sequence are zero.  max_q: the most nodes of a sequence.  scale: of either sign, or zero.
+ * b2_tree_attention_supported says (1 / 0) whether the shape is served: head_dim 64 or 128, up to 128 query heads per KV head, blocks of
+ * a multiple of 16 tokens.  b2_tree_attention_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant; calls
+ * that may run at the same time need one each), or -1 where the shape is not served. */
+int b2_tree_attention_supported(int nq, int nkv, int head_dim, int block_size);
+int64_t b2_tree_attention_workspace(b2_ctx* ctx, int n_seqs, int max_q, int nq, int nkv, int head_dim, int block_size, int bt_width);
+int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int num_blocks, int block_size,
+                      const int32_t* block_tables, int64_t bt_stride, int bt_width, const int32_t* cu_q, const int32_t* context_lens,
+                      const int64_t* tree_mask, int64_t mask_stride, int mask_words, int n_seqs, int max_q, int tokens, int nq, int nkv,
+                      int head_dim, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- rules on logits, between b2_lm_head and the sampler (no counterpart in the reference, whose sampler takes the logits as they
+ *      are, nanovllm/layers/sampler.py:7-12) ------------------------------------------
+ * For row i of logits [rows, vocab] (bf16, or fp32 where fp32 is 1), its request s and token v, in 32 bits and in this order:
+ *   seen in history or among the drafted tokens of the row's path:  x = x > 0 ? x / repetition_penalty[s] : x * repetition_penalty[s]
+ *   count > 0:  x = x - frequency_penalty[s] * count - presence_penalty[s]     (count: in the output part of history and the path)
+ *   x = x + the bias of v;   not allowed: x = -inf
+ * then rounded to the logits' type; logits that no rule touches are copied bit for bit.  out may be logits itself, with the same stride.
+ * Every rule may be left out (NULL).  Request s's rows are cu_seqlens[s] .. cu_seqlens[s+1], rows behind the last request are copied; with
+ * cu_seqlens NULL row i is request i and n_seqs = rows. */
+typedef struct b2_logit_rules {
+  int n_seqs;
+  const int32_t* cu_seqlens;
+  const int64_t* history;  /* [n_seqs, history_width]: the first history_lens[s] tokens of request s, of which prompt_lens[s] (NULL: none) are its prompt */
+  int64_t history_stride;
+  int history_width;
+  const int32_t *history_lens, *prompt_lens;
+  const float *repetition_penalty, *presence_penalty, *frequency_penalty; /* [n_seqs] */
+  const int64_t* bias_ids; /* [n_seqs, n_bias]: token ids and their biases; of equal ids the last counts */
+  int64_t bias_stride;
+  int n_bias;
+  const float* bias_values;
+  int64_t bias_value_stride;
+  const int32_t* allowed_mask; /* [rows, (vocab + 31) / 32]: bit v % 32 of word v / 32 says that token v is allowed */
+  int64_t allowed_stride;
+  const int64_t* draft_tokens; /* [rows]: the drafted token of each row's node; with cu_seqlens and tree_mask */
+  const int64_t* tree_mask;    /* [rows, mask_words], as for b2_tree_attention: the nodes a row sees are its path */
+  int64_t mask_stride;
+  int mask_words;
+} b2_logit_rules; /* token ids outside the vocabulary are ignored */
+int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, int fp32, int rows, int vocab, const b2_logit_rules* rules, void* stream);
 
 /* Greedy pick: out[i] = argmax_j logits[i, j] (first index on ties), int64.
  * The reference's Sampler (nanovllm/layers/sampler.py:7-12) at temperature -> 0. */

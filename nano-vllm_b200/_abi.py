@@ -55,6 +55,15 @@ class TilePlan(C.Structure):
                                        "out_off", "bar_off", "smem", "width")]
 
 
+class LogitRules(C.Structure):
+    """b2_logit_rules: the rules that b2_adjust_logits applies."""
+    _fields_ = [("n_seqs", C.c_int), ("cu_seqlens", C.c_void_p), ("history", C.c_void_p), ("history_stride", C.c_int64), ("history_width", C.c_int),
+                ("history_lens", C.c_void_p), ("prompt_lens", C.c_void_p), ("repetition_penalty", C.c_void_p), ("presence_penalty", C.c_void_p),
+                ("frequency_penalty", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_stride", C.c_int64), ("n_bias", C.c_int), ("bias_values", C.c_void_p),
+                ("bias_value_stride", C.c_int64), ("allowed_mask", C.c_void_p), ("allowed_stride", C.c_int64), ("draft_tokens", C.c_void_p),
+                ("tree_mask", C.c_void_p), ("mask_stride", C.c_int64), ("mask_words", C.c_int)]
+
+
 _p, _i, _i64, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
 
 SIGNATURES = {
@@ -92,8 +101,13 @@ SIGNATURES = {
     "b2_prefill_attention_supported": [_i, _i, _i, _i],
     "b2_decode_stack_workspace": [_p, _i, _i, _i, _i, _i, _i, _i, _i],
     "b2_decode_stack": [_p, _p, _i, _p, _i, _i, _i, _i, _i, _f, _f, _f, _p, _p, _i, _p, _p, _p, _p, _i64, _i, _i, _i, _p, _p, _i64, _p],
+    "b2_tree_attention": [_p, _p, _i64, _p, _p, _i, _i, _p, _i64, _i, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _i, _f, _p, _p, _i64, _p],
+    "b2_tree_attention_supported": [_i, _i, _i, _i],
+    "b2_tree_attention_workspace": [_p, _i, _i, _i, _i, _i, _i, _i],
+    "b2_adjust_logits": [_p, _i64, _p, _i64, _i, _i, _i, C.POINTER(LogitRules), _p],
     "b2_argmax": [_p, _i64, _i, _i, _p, _p],
     "b2_broadcast_tokens": [_p, _p, _i, _p],
+    "b2_batch_inputs": [_p, _i64, _i, _p, _p, _i, _p, _i, _p, _i, _i64, _i, _p, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _p],
     "b2_advance_decode": [_p, _p, _p, _p, _p, _p, _i64, _i, _i, _i64, _i, _p],
     # the planner as data: no CUDA call, usable without a GPU
     "b2_plan_gemm": [_i, _i, _i, _i, _i, C.POINTER(_i), C.POINTER(GemmPlan)],
@@ -115,7 +129,7 @@ for _name, _args in SIGNATURES.items():
     _fn.restype = _i
 lib.b2_last_error.restype = C.c_char_p
 lib.b2_last_error.argtypes = []
-lib.b2_launch_count.restype = lib.b2_decode_stack_workspace.restype = _i64
+lib.b2_launch_count.restype = lib.b2_decode_stack_workspace.restype = lib.b2_tree_attention_workspace.restype = _i64
 lib.b2_launch_count.argtypes = []
 
 EXPORTED = list(SIGNATURES) + ["b2_last_error", "b2_launch_count"]

@@ -478,6 +478,210 @@ PyObject* decode_stack(Args a) {
   return wrap(out);
 }
 
+// ---- a verification step of drafted tokens ---------------------------------------------------
+// a matrix that is read row by row: [rows, at least cols], columns contiguous
+void row_matrix(const at::Tensor& t, at::ScalarType type, int64_t rows, int64_t cols, const char* what) {
+  if (t.scalar_type() != type) raise(PyExc_TypeError, "%s: expected %s, got %s", what, c10::toString(type), c10::toString(t.scalar_type()));
+  if (t.dim() != 2 || t.size(0) != rows || t.size(1) < cols)
+    raise(PyExc_ValueError, "%s: expected %lld rows of %lld or more, got %lld elements in %lld dimensions", what, (long long)rows, (long long)cols, (long long)t.numel(), (long long)t.dim());
+  if (t.size(1) > 1 && t.stride(1) != 1) raise(PyExc_AssertionError, "%s: columns must be contiguous", what);
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+void vector_of(const at::Tensor& t, at::ScalarType type, int64_t n, const char* what) {
+  if (t.scalar_type() != type) raise(PyExc_TypeError, "%s: expected %s, got %s", what, c10::toString(type), c10::toString(t.scalar_type()));
+  if (t.dim() != 1 || t.size(0) != n) raise(PyExc_ValueError, "%s: expected %lld elements, got %lld in %lld dimensions", what, (long long)n, (long long)t.numel(), (long long)t.dim());
+  if (!t.is_contiguous()) raise(PyExc_AssertionError, "%s must be contiguous", what);
+}
+void beside(const at::Tensor& t, const at::Tensor& x, const char* what) {
+  if (t.defined() && t.device() != x.device()) raise(PyExc_TypeError, "%s is on %s, the other tensors on %s", what, t.device().str().c_str(), x.device().str().c_str());
+}
+void forward_only(std::initializer_list<const at::Tensor*> inputs, const char* what) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : inputs)
+    if (t->defined() && t->requires_grad()) raise(PyExc_ValueError, "%s has no backward pass: call it under torch.no_grad()", what);
+}
+// the bytes between a tensor's first and last element
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return reinterpret_cast<uintptr_t>(t.const_data_ptr()) + (last + 1) * t.element_size();
+  };
+  return a.numel() > 0 && b.numel() > 0 && reinterpret_cast<uintptr_t>(a.const_data_ptr()) < end(b) && reinterpret_cast<uintptr_t>(b.const_data_ptr()) < end(a);
+}
+
+// batch_inputs(block_tables, cached_lens, seq_lens, free_blocks, num_free, block_size, num_slots, max_tokens, tree_mask):
+// (positions, slot_mapping, cu_seqlens_q, cu_seqlens_k, last_token_index, context_lens, num_free)
+PyObject* batch_inputs(Args a) {
+  const at::Tensor &tables = tensor(a[0], "block_tables"), &cached = tensor(a[1], "cached_lens"), &wanted = tensor(a[2], "seq_lens"), &free = tensor(a[3], "free_blocks"),
+                   &num_free = tensor(a[4], "num_free");
+  const int64_t bs = integer(a[5]), num_slots = integer(a[6]), max_tokens = integer(a[7]);
+  const at::Tensor mask = optional_tensor(a[8], "tree_mask");
+  if (tables.dim() != 2) raise(PyExc_ValueError, "block_tables: expected 2 dimensions, got %lld", (long long)tables.dim());
+  const int64_t n = tables.size(0), width = tables.size(1);
+  row_matrix(tables, at::kInt, n, n > 0 ? 1 : 0, "block_tables");
+  if (n > 1 && tables.stride(0) < width) raise(PyExc_AssertionError, "block_tables: rows must not overlap");
+  vector_of(cached, at::kInt, n, "cached_lens");
+  vector_of(wanted, at::kInt, n, "seq_lens");
+  vector_of(free, at::kInt, free.numel(), "free_blocks");
+  vector_of(num_free, at::kInt, 1, "num_free");
+  constexpr int64_t limit = (int64_t(1) << 31) - 1;
+  if (bs < 1 || bs > limit || num_slots < 1 || num_slots > limit || max_tokens < 0 || max_tokens > 1 << 30)
+    raise(PyExc_ValueError, "batch_inputs: block_size %lld, num_slots %lld, max_tokens %lld", (long long)bs, (long long)num_slots, (long long)max_tokens);
+  if (n > 8192 || width > limit / bs / std::max<int64_t>(n, 1) || n * width + free.numel() > limit)
+    raise(PyExc_ValueError, "batch_inputs: %lld rows of %lld blocks of %lld tokens: at most 8192 rows and 2^31 - 1 tokens", (long long)n, (long long)width, (long long)bs);
+  if (mask.defined()) {
+    if (mask.dim() != 2 || mask.size(0) < max_tokens || mask.size(1) < 1) raise(PyExc_ValueError, "tree_mask: expected a row for each of %lld tokens", (long long)max_tokens);
+    row_matrix(mask, at::kLong, mask.size(0), 1, "tree_mask");
+  }
+  const std::pair<const at::Tensor*, const char*> named[] = {{&tables, "block_tables"}, {&cached, "cached_lens"}, {&wanted, "seq_lens"}, {&free, "free_blocks"}, {&num_free, "num_free"}};
+  for (int i : {0, 3})
+    for (int k = 0; k < 5; ++k)
+      if (k != i && overlap(*named[i].first, *named[k].first)) raise(PyExc_ValueError, "%s, which is written, overlaps %s", named[i].second, named[k].second);
+  on_current_gpu(tables, "block_tables");
+  for (const auto& t : named) beside(*t.first, tables, t.second);
+  beside(mask, tables, "tree_mask");
+  auto empty = [&](int64_t size, at::ScalarType type) { return at::detail::empty_cuda({size}, type, tables.device(), std::nullopt); };
+  const at::Tensor out[7] = {empty(max_tokens, at::kLong), empty(max_tokens, at::kInt), empty(n + 1, at::kInt), empty(n + 1, at::kInt), empty(n, at::kInt), empty(n, at::kInt), empty(1, at::kInt)};
+  auto ints = [&](int i) { return out[i].mutable_data_ptr<int32_t>(); };
+  launch("b2_batch_inputs", b2_batch_inputs, tables.mutable_data_ptr<int32_t>(), row_stride(tables), width, cached.const_data_ptr<int32_t>(), wanted.const_data_ptr<int32_t>(), n,
+         free.mutable_data_ptr<int32_t>(), free.numel(), num_free.const_data_ptr<int32_t>(), bs, num_slots, max_tokens, mask.defined() ? mask.const_data_ptr<int64_t>() : nullptr,
+         mask.defined() ? row_stride(mask) : 0, mask.defined() ? mask.size(1) : 0, out[0].mutable_data_ptr<int64_t>(), ints(1), ints(2), ints(3), ints(4), ints(5), ints(6), stream());
+  PyObject* p = PyTuple_New(7);
+  if (p == nullptr) throw Raised{};
+  for (int i = 0; i < 7; ++i) PyTuple_SET_ITEM(p, i, wrap(out[i]));
+  return p;
+}
+
+// tree_attention(ctx, q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, tree_mask, max_q, scale)
+PyObject* tree_attention(Args a) {
+  const at::Tensor &q = tensor(a[1], "q"), &kc = tensor(a[2], "k_cache"), &vc = tensor(a[3], "v_cache"), &cu_q = tensor(a[4], "cu_seqlens_q"), &lens = tensor(a[5], "context_lens"),
+                   &tables = tensor(a[6], "block_tables"), &mask = tensor(a[7], "tree_mask");
+  const int64_t max_q = integer(a[8]);
+  if (q.dim() != 3 || kc.dim() != 4) raise(PyExc_ValueError, "tree_attention: q of 3 and caches of 4 dimensions, got %lld and %lld", (long long)q.dim(), (long long)kc.dim());
+  const int64_t n = q.size(0), nq = q.size(1), hd = q.size(2), nkv = kc.size(2), bs = kc.size(1), n_seqs = lens.numel();
+  if (q.scalar_type() != at::kBFloat16) raise(PyExc_TypeError, "q: expected bf16, got %s", c10::toString(q.scalar_type()));
+  values_like_keys(kc, vc, hd);
+  if (nq > 8192 || bs > 1 << 20 || !b2_tree_attention_supported(nq, nkv, hd, bs))
+    raise(PyExc_ValueError, "tree_attention: %lld query and %lld KV heads of %lld, blocks of %lld tokens: head dimension 64 or 128, at most 128 query heads per KV head, blocks of a multiple of 16",
+          (long long)nq, (long long)nkv, (long long)hd, (long long)bs);
+  if (!row_layout(q, nq, hd)) raise(PyExc_AssertionError, "q: heads must lie side by side, in rows on 16-byte boundaries");
+  if (!kc.is_contiguous() || !vc.is_contiguous() || !on_16_bytes(kc) || !on_16_bytes(vc)) raise(PyExc_AssertionError, "k_cache and v_cache must be contiguous, on 16-byte boundaries");
+  constexpr int64_t limit = (int64_t(1) << 31) - 1;
+  if (kc.size(0) < 1 || kc.size(0) > limit / bs || tables.dim() != 2 || tables.size(1) > limit / bs || n > 1 << 24 || n_seqs > 65535)
+    raise(PyExc_ValueError, "tree_attention: %lld blocks, %lld tokens, %lld sequences", (long long)kc.size(0), (long long)n, (long long)n_seqs);
+  vector_of(lens, at::kInt, n_seqs, "context_lens");
+  vector_of(cu_q, at::kInt, n_seqs + 1, "cu_seqlens_q");
+  row_matrix(tables, at::kInt, n_seqs, n_seqs > 0 ? 1 : 0, "block_tables");
+  row_matrix(mask, at::kLong, n, n > 0 ? 1 : 0, "tree_mask");
+  if (max_q < 0 || (n > 0 && n_seqs > 0 && max_q < 1)) raise(PyExc_ValueError, "tree_attention: max_seqlen_q %lld", (long long)max_q);
+  forward_only({&q, &kc, &vc}, "tree_attention");
+  on_current_gpu(q, "q");
+  beside(kc, q, "k_cache");
+  beside(vc, q, "v_cache");
+  beside(cu_q, q, "cu_seqlens_q");
+  beside(lens, q, "context_lens");
+  beside(tables, q, "block_tables");
+  beside(mask, q, "tree_mask");
+  const at::Tensor out = at::detail::empty_cuda({n, nq, hd}, at::kBFloat16, q.device(), std::nullopt);
+  if (n == 0) return wrap(out);
+  b2_ctx* const ctx = context(a[0]);
+  const int64_t bytes = b2_tree_attention_workspace(ctx, n_seqs, max_q, nq, nkv, hd, bs, tables.size(1));
+  if (bytes < 0) check(B2_ERR_UNSUPPORTED, "b2_tree_attention_workspace");
+  const at::Tensor ws = at::detail::empty_cuda({bytes}, at::kByte, q.device(), std::nullopt);
+  launch("b2_tree_attention", b2_tree_attention, ctx, q.data_ptr(), n > 1 ? q.stride(0) : nq * hd, kc.data_ptr(), vc.data_ptr(), kc.size(0), bs, tables.const_data_ptr<int32_t>(),
+         std::max(row_stride(tables), tables.size(1)), tables.size(1), cu_q.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(), mask.const_data_ptr<int64_t>(), row_stride(mask),
+         mask.size(1), n_seqs, max_q, n, nq, nkv, hd, number(a[9]), out.data_ptr(), ws.data_ptr(), bytes, stream());
+  return wrap(out);
+}
+
+// adjust_logits(logits, history, history_lens, prompt_lens, repetition, presence, frequency, bias_ids, bias_values, allowed_mask, cu_seqlens,
+//               draft_tokens, tree_mask, out)
+PyObject* adjust_logits(Args a) {
+  at::Tensor x = tensor(a[0], "logits");
+  const char* const names[] = {"logits", "history", "history_lens", "prompt_lens", "repetition_penalty", "presence_penalty", "frequency_penalty",
+                               "bias_ids", "bias_values", "allowed_mask", "cu_seqlens", "draft_tokens", "tree_mask", "out"};
+  at::Tensor t[14];
+  for (int i = 1; i < 14; ++i) t[i] = optional_tensor(a[i], names[i]);
+  if (x.dim() != 2) raise(PyExc_ValueError, "logits: expected [rows, vocabulary], got %lld dimensions", (long long)x.dim());
+  if (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat) raise(PyExc_TypeError, "logits: expected bf16 or fp32, got %s", c10::toString(x.scalar_type()));
+  const int64_t rows = x.size(0), vocab = x.size(1);
+  if (rows > 1 << 30 || vocab > 1 << 30) raise(PyExc_ValueError, "logits: %lld rows of %lld", (long long)rows, (long long)vocab);
+  if (t[10].defined()) {
+    vector_of(t[10], at::kInt, t[10].numel(), names[10]);
+    if (t[10].numel() < 1) raise(PyExc_ValueError, "cu_seqlens: at least one element");
+  }
+  const int64_t n = t[10].defined() ? t[10].numel() - 1 : rows;
+  b2_logit_rules r{};
+  r.n_seqs = n;
+  r.cu_seqlens = cptr<int32_t>(t[10]);
+  if (t[1].defined() != t[2].defined() || (t[3].defined() && !t[1].defined())) raise(PyExc_ValueError, "history, its history_lens and prompt_lens belong together");
+  for (int i = 4; i < 7; ++i)
+    if (t[i].defined()) {
+      if (!t[1].defined() && !t[11].defined()) raise(PyExc_ValueError, "%s: penalties need a history or drafted tokens", names[i]);
+      vector_of(t[i], at::kFloat, n, names[i]);
+    }
+  if (t[1].defined()) {
+    row_matrix(t[1], at::kLong, n, 0, names[1]);
+    if (t[1].size(1) > 1 << 30) raise(PyExc_ValueError, "history: rows of %lld", (long long)t[1].size(1));
+    vector_of(t[2], at::kInt, n, names[2]);
+    if (t[3].defined()) vector_of(t[3], at::kInt, n, names[3]);
+    r.history = cptr<int64_t>(t[1]);
+    r.history_stride = row_stride(t[1]);
+    r.history_width = t[1].size(1);
+    r.history_lens = cptr<int32_t>(t[2]);
+    r.prompt_lens = cptr<int32_t>(t[3]);
+  }
+  r.repetition_penalty = cptr<float>(t[4]);
+  r.presence_penalty = cptr<float>(t[5]);
+  r.frequency_penalty = cptr<float>(t[6]);
+  if (t[7].defined() != t[8].defined()) raise(PyExc_ValueError, "bias_ids and bias_values belong together");
+  if (t[7].defined()) {
+    row_matrix(t[7], at::kLong, n, 0, names[7]);
+    row_matrix(t[8], at::kFloat, n, 0, names[8]);
+    if (t[7].size(1) != t[8].size(1) || t[7].size(1) > 1 << 30) raise(PyExc_ValueError, "bias_ids: %lld a request, bias_values %lld", (long long)t[7].size(1), (long long)t[8].size(1));
+    r.bias_ids = cptr<int64_t>(t[7]);
+    r.bias_stride = row_stride(t[7]);
+    r.n_bias = t[7].size(1);
+    r.bias_values = cptr<float>(t[8]);
+    r.bias_value_stride = row_stride(t[8]);
+  }
+  if (t[9].defined()) {
+    row_matrix(t[9], at::kInt, rows, (vocab + 31) / 32, names[9]);
+    r.allowed_mask = cptr<int32_t>(t[9]);
+    r.allowed_stride = row_stride(t[9]);
+  }
+  if (t[11].defined() != t[12].defined() || (t[11].defined() && !t[10].defined())) raise(PyExc_ValueError, "draft_tokens, tree_mask and cu_seqlens belong together");
+  if (t[11].defined()) {
+    vector_of(t[11], at::kLong, rows, names[11]);
+    row_matrix(t[12], at::kLong, rows, rows > 0 ? 1 : 0, names[12]);
+    if (t[12].size(1) > 1 << 20) raise(PyExc_ValueError, "tree_mask: rows of %lld words", (long long)t[12].size(1));
+    r.draft_tokens = cptr<int64_t>(t[11]);
+    r.tree_mask = cptr<int64_t>(t[12]);
+    r.mask_stride = row_stride(t[12]);
+    r.mask_words = t[12].size(1);
+  }
+  auto in_rows = [&](const at::Tensor& m) { return (vocab <= 1 || m.stride(1) == 1) && (rows <= 1 || m.stride(0) >= vocab); };
+  at::Tensor out = t[13];
+  if (out.defined()) {
+    if (out.scalar_type() != x.scalar_type()) raise(PyExc_TypeError, "out: expected %s, got %s", c10::toString(x.scalar_type()), c10::toString(out.scalar_type()));
+    if (out.sizes() != x.sizes()) raise(PyExc_ValueError, "out and logits differ in shape");
+    if (!in_rows(out)) raise(PyExc_AssertionError, "out: rows must be contiguous and must not overlap");
+    const bool itself = out.const_data_ptr() == x.const_data_ptr() && (rows <= 1 || out.stride(0) == x.stride(0)) && in_rows(x);
+    if (!itself && overlap(out, x)) raise(PyExc_ValueError, "out overlaps the logits without being them");
+    for (int i = 1; i < 13; ++i)
+      if (t[i].defined() && overlap(out, t[i])) raise(PyExc_ValueError, "out overlaps %s", names[i]);
+  }
+  forward_only({&x, &t[4], &t[5], &t[6], &t[8], &t[13]}, "adjust_logits");
+  on_current_gpu(x, "logits");
+  for (int i = 1; i < 14; ++i) beside(t[i], x, names[i]);
+  if (!in_rows(x)) x = x.contiguous();
+  if (!out.defined()) out = at::detail::empty_cuda({rows, vocab}, x.scalar_type(), x.device(), std::nullopt);
+  if (rows > 0 && vocab > 0)
+    launch("b2_adjust_logits", b2_adjust_logits, x.const_data_ptr(), row_stride(x), out.data_ptr(), row_stride(out), int(x.scalar_type() == at::kFloat), rows, vocab, &r, stream());
+  return wrap(out);
+}
+
 PyObject* init(Args a) {
   Py_INCREF(a[0]);
   Py_XDECREF(g_check);
@@ -504,7 +708,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {B2_ENTRY(init, 1), B2_ENTRY(gemm, 4), B2_ENTRY(gemm_silu_mul, 3), B2_ENTRY(qkv_fused, 15), B2_ENTRY(rowpar_fused, 7),
                          B2_ENTRY(rmsnorm, 3), B2_ENTRY(add_rmsnorm, 4), B2_ENTRY(silu_and_mul, 1), B2_ENTRY(store_kvcache, 5),
                          B2_ENTRY(qk_norm_rope_store, 12), B2_ENTRY(rope, 5), B2_ENTRY(embed, 5), B2_ENTRY(paged_attention, 7), B2_ENTRY(prefill_attention, 9),
-                         B2_ENTRY(decode_stack, 16), {nullptr, nullptr, 0, nullptr}};
+                         B2_ENTRY(decode_stack, 16), B2_ENTRY(batch_inputs, 9), B2_ENTRY(tree_attention, 10), B2_ENTRY(adjust_logits, 14), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_b2torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -4,6 +4,7 @@ The calls of a decoder layer do that in native code (csrc/b2_torch.cpp)."""
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -251,3 +252,53 @@ def advance_decode(tokens, input_ids, positions, context_lens, slot_mapping, blo
     _abi.check(_lib.b2_advance_decode(tokens.data_ptr(), input_ids.data_ptr(), positions.data_ptr(), context_lens.data_ptr(),
                                       slot_mapping.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
                                       block_size, num_slots, n, _stream()), "b2_advance_decode")
+
+
+class BatchInputs(NamedTuple):
+    """What a step of the model takes from the requests' lengths (see batch_inputs)."""
+    positions: torch.Tensor         # int64 [max_tokens]; 0 behind the last token
+    slot_mapping: torch.Tensor      # int32 [max_tokens]; -1 behind the last token
+    cu_seqlens_q: torch.Tensor      # int32 [n + 1]
+    cu_seqlens_k: torch.Tensor      # int32 [n + 1]
+    last_token_index: torch.Tensor  # int32 [n]
+    context_lens: torch.Tensor      # int32 [n]
+    num_free: torch.Tensor          # int32 [1]
+
+
+def batch_inputs(block_tables: torch.Tensor, cached_lens: torch.Tensor, seq_lens: torch.Tensor, free_blocks: torch.Tensor, num_free: torch.Tensor, block_size: int,
+                 num_slots: int, max_tokens: int, tree_mask: torch.Tensor | None = None) -> BatchInputs:
+    """The inputs of a step of n requests, built on the GPU: request i has cached_lens[i] tokens in the cache and is to have seq_lens[i].
+    Requests that grow take blocks from the stack free_blocks[:num_free], requests that shrink (to 0: finished ones) give theirs back;
+    block_tables [n, width] and free_blocks are updated in place, the new stack's height is the result's num_free.  max_tokens: room for the
+    step's new tokens (a captured call serves any batch that fits).  tree_mask int64 [max_tokens or more, words]: the new tokens are trees of drafted tokens,
+    whose positions follow their depth.  A request for which there are no blocks or no room is not served: its context_lens
+    stays cached_lens[i].  The rules in full are at b2_batch_inputs."""
+    return BatchInputs(*_native.batch_inputs(block_tables, cached_lens, seq_lens, free_blocks, num_free, block_size, num_slots, max_tokens, tree_mask))
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_seqlens_q: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor,
+                   tree_mask: torch.Tensor, max_seqlen_q: int, scale: float) -> torch.Tensor:
+    """Attention of a tree of drafted tokens per sequence, q [tokens, nq, head_dim], over the paged cache, which holds the trees' keys and
+    values already: the last tokens of each context, in the nodes' order.  Every node sees what is before the tree, and of the tree the nodes
+    whose bit is set in its row of tree_mask (int64 [tokens, words], bit k % 64 of word k / 64 for node k, itself included).  What a node
+    does not see may hold anything; a node that sees nothing and tokens behind the last sequence come back as zeros.  Shapes that the kernel
+    does not serve (head_dim other than 64 and 128, blocks that are no multiple of 16 tokens) raise.  Forward only."""
+    return _native.tree_attention(get_runtime().handle, q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, tree_mask, max_seqlen_q, scale)
+
+
+def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, history_lens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                  repetition_penalty: torch.Tensor | None = None, presence_penalty: torch.Tensor | None = None, frequency_penalty: torch.Tensor | None = None,
+                  bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None, allowed_mask: torch.Tensor | None = None,
+                  cu_seqlens: torch.Tensor | None = None, draft_tokens: torch.Tensor | None = None, tree_mask: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The logits [rows, vocab] (bf16 or fp32) of n requests under their rules, for the sampler or argmax; out may be logits itself.
+
+    history int64 [n, width]: the first history_lens[s] tokens of request s, of which the first prompt_lens[s] are its prompt.
+    repetition_penalty fp32 [n] divides positive and multiplies other logits of tokens that occur in it; frequency_penalty times the count in the
+    output part, and presence_penalty once, are taken off.  bias_ids int64 / bias_values fp32 [n, k] are added (of equal ids the last counts; ids outside the
+    vocabulary are ignored).  allowed_mask int32 [rows, (vocab + 31) / 32]: tokens whose bit is not set get -inf.
+
+    Row i belongs to request i, or with cu_seqlens int32 [n + 1] request s has rows cu_seqlens[s] .. cu_seqlens[s + 1] (rows behind the last are
+    copied); with draft_tokens int64 [rows] and tree_mask (as for tree_attention) the drafted tokens that a row's node sees count as its output."""
+    return _native.adjust_logits(logits, history, history_lens, prompt_lens, repetition_penalty, presence_penalty, frequency_penalty, bias_ids, bias_values, allowed_mask,
+                                 cu_seqlens, draft_tokens, tree_mask, out)
