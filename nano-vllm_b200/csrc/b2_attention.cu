@@ -759,48 +759,6 @@ struct PrefillArgs {
   B2Status* status;
 };
 
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a_tmem, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a_tmem), "l"(desc_b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
-      "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// tcgen05.wait::ld, before which nothing reads the 64 columns
-__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[2][32]) {
-  b2::tc_wait_ld();
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      asm volatile("" : "+r"(r[h][i]), "+r"(r[h][i + 1]), "+r"(r[h][i + 2]), "+r"(r[h][i + 3]), "+r"(r[h][i + 4]), "+r"(r[h][i + 5]), "+r"(r[h][i + 6]), "+r"(r[h][i + 7]));
-}
-// two products and sums in one instruction, each rounded as fmaf rounds it
-__device__ __forceinline__ uint64_t pair_of(float x, float y) {
-  uint64_t p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
-  return p;
-}
-__device__ __forceinline__ void fma_pair(float& x, float& y, uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d));
-}
-// V as the second operand, [tokens][dimensions] with the dimensions contiguous: MN-major, 128-byte swizzle.  8 tokens are 1024
-// bytes apart (stride offset), the two halves of 64 dimensions PF_KV / 2 (leading offset).
-__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t addr) {
-  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>((PF_KV / 2) >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
-         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
-}
-
 template <bool PAIRS>
 __global__ void __launch_bounds__(PF_THREADS, 1)
 prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PrefillArgs a) {
@@ -897,7 +855,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     const int h = warp - 1;
     const uint32_t idesc_s = b2::umma_idesc_bf16(PF_KEYS) | a.negate;
     constexpr uint32_t idesc_o = b2::umma_idesc_bf16(128) | (1u << 16);  // second operand MN-major
-    const uint64_t desc_q = b2::umma_smem_desc(s_q + h * PF_Q), desc_k = b2::umma_smem_desc(s_k), desc_v = umma_smem_desc_mn(s_v);  // (addresses in 16 bytes)
+    const uint64_t desc_q = b2::umma_smem_desc(s_q + h * PF_Q), desc_k = b2::umma_smem_desc(s_k), desc_v = b2::umma_smem_desc_mn(s_v, PF_KV / 2);  // (addresses in 16 bytes)
     auto wait = [&](uint32_t bar, uint32_t phase, int code) {
       const bool ok = all_wait(bar, phase, code);
       b2::tc_fence_after();
@@ -927,7 +885,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         const uint64_t dv = desc_v + st * (PF_KV >> 4);
 #pragma unroll
         for (int k = 0; k < PF_KEYS / 16; ++k)  // 16 tokens: 8 columns of P, 2048 bytes of V
-          umma_bf16_ts(tmem + 256 + h * 128, tmem + buf * PF_KEYS + k * 8, dv + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+          b2::umma_bf16_ts(tmem + 256 + h * 128, tmem + buf * PF_KEYS + k * 8, dv + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
         b2::umma_commit(o_done + h * 8);
         b2::umma_commit(v_empty + st * 8);
         if (j == n - 1) b2::umma_commit(o_final + h * 8);
@@ -942,7 +900,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     const int pos = shift + t0 + row;  // the last key this row sees
     float m = -INFINITY;               // the row's maximum, in units of scores
     float l[4] = {};                   // its sum, of columns 2 i and 2 i + 1 of every eight
-    const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
+    const uint64_t scale2 = b2::pair_of(a.scale_log2, a.scale_log2);
     bool ok = true;
     for (int j = 0; ok && j < n; ++j) {
       const int buf = h * 2 + (j & 1);
@@ -955,7 +913,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         b2::tc_fence_after();
         b2::tmem_ld_32x32(at, r[0]);
         b2::tmem_ld_32x32(at + 32, r[1]);
-        tc_wait_ld(r);
+        b2::tc_wait_ld(r);
         const int last = min(pos, kv_len - 1) - block_of(i) * PF_KEYS;  // keys 0 .. last of the block count
         if (__any_sync(0xffffffffu, last < PF_KEYS - 1)) {
 #pragma unroll
@@ -983,7 +941,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
       __syncwarp();
       if (lane == 0) b2::mbar_arrive(f_full + (buf * 4 + q) * 8);
       const float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
-      const uint64_t ref2 = pair_of(-ref, -ref);
+      const uint64_t ref2 = b2::pair_of(-ref, -ref);
 #pragma unroll
       for (int i = 0; i < 4; ++i) l[i] *= f;
 #pragma unroll
@@ -992,15 +950,15 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           float x, y;
-          fma_pair(x, y, pair_of(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), scale2, ref2);
+          b2::fma_pair(x, y, b2::pair_of(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), scale2, ref2);
           x = b2::ex2(x);
           y = b2::ex2(y);
           l[(e >> 1) & 3] = l[(e >> 1) & 3] + x + y;
           p[e >> 1] = b2::pack_bf16(x, y);
         }
-        tmem_st_32x16(t_s + c * 16, p);  // (this row has read its columns)
+        b2::tmem_st_32x16(t_s + c * 16, p);  // (this row has read its columns)
       }
-      tc_wait_st();
+      b2::tc_wait_st();
       b2::tc_fence_before();
       __syncwarp();
       if (lane == 0) b2::mbar_arrive(p_full + buf * 8);
@@ -1017,7 +975,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         uint32_t r[2][32];
         b2::tmem_ld_32x32(t_o + c * 64, r[0]);
         b2::tmem_ld_32x32(t_o + c * 64 + 32, r[1]);
-        tc_wait_ld(r);
+        b2::tc_wait_ld(r);
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
           uint32_t w[4];
@@ -1069,13 +1027,13 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
             uint32_t r[2][32];
             b2::tmem_ld_32x32(t_o + c * 64, r[0]);
             b2::tmem_ld_32x32(t_o + c * 64 + 32, r[1]);
-            tc_wait_ld(r);
+            b2::tc_wait_ld(r);
 #pragma unroll
             for (int e = 0; e < 64; ++e) r[e >> 5][e & 31] = __float_as_uint(__uint_as_float(r[e >> 5][e & 31]) * f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_st_32x16(t_o + c * 64 + i * 16, &r[i >> 1][(i & 1) * 16]);
+            for (int i = 0; i < 4; ++i) b2::tmem_st_32x16(t_o + c * 64 + i * 16, &r[i >> 1][(i & 1) * 16]);
           }
-          tc_wait_st();
+          b2::tc_wait_st();
           b2::tc_fence_before();
         }
         __syncwarp();
@@ -1094,10 +1052,6 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
   }
   if (warp == 1) b2::tmem_dealloc(tmem, 512);
 }
-
-// Softmax scale * log2(e) for kernels that mask and compare scores before they scale them: its size - masked scores are -inf, and -inf times
-// zero is none -, with the query negated in a negative one's place, which changes no product but for its sign.
-float scale_size(float scale) { return std::max(fabsf(scale * 1.4426950408889634f), FLT_MIN); }
 
 constexpr size_t ATT_SMEM_LIMIT = 113 * 1024;  // two CTAs per SM (228 KB, 1 KB of it reserved per CTA)
 constexpr size_t attention_smem(int n_seqs, int group) {
@@ -1172,7 +1126,7 @@ int b2_paged_attention_decode(b2_ctx* ctx, const void* q, int64_t q_stride, cons
   if (a.group > ATT_MAX_GROUP) {
     const bool few = items <= 2 * ctx->num_sms;
     a.flip = scale < 0.f ? 0x80008000u : 0u;
-    a.scale_log2 = scale_size(scale);
+    a.scale_log2 = b2::scale_size(scale);
     a.stages = items <= ctx->num_sms ? WD_MAX_STAGES : few ? 6 : items <= 3 * ctx->num_sms ? 4 : 3;
     const auto kernel = few ? paged_decode_wide_kernel<true> : paged_decode_wide_kernel<false>;
     B2_CUDA(b2_launch(kernel, dim3(items), dim3(ATT_THREADS), wide_smem(a.stages), static_cast<cudaStream_t>(stream), maps[0], maps[1], maps[2], maps[3], a));
@@ -1216,7 +1170,7 @@ int b2_prefill_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const voi
   a.nq = nq;
   a.out = static_cast<uint16_t*>(out);
   a.negate = scale < 0.f ? b2::kUmmaNegateA : 0u;
-  a.scale_log2 = scale_size(scale);
+  a.scale_log2 = b2::scale_size(scale);
   a.status = ctx->status_dev;
   a.group = nq / nkv;
   const auto kernel = block_tables != nullptr && a.group > 2 ? prefill_attention_kernel<true> : prefill_attention_kernel<false>;

@@ -7,6 +7,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
 #include "../../include/b200tp.h"
 
 // ---------------------------------------------------------------------------
@@ -217,6 +221,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
+// the same of a 3-D map (x: elements, y: heads, z: rows)
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;"
+      ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
+
 // ---- tcgen05 / tensor memory -------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_result, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_result), "r"(ncols) : "memory");
@@ -360,6 +373,48 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int n) {
          | (1u << 10)                               // B format: BF16
          | (static_cast<uint32_t>(n >> 3) << 17)    // N / 8
          | (static_cast<uint32_t>(128 >> 4) << 24); // M / 16
+}
+
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a_tmem, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+      "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// tcgen05.wait::ld, before which nothing reads the 64 columns
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[2][32]) {
+  tc_wait_ld();
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+      asm volatile("" : "+r"(r[h][i]), "+r"(r[h][i + 1]), "+r"(r[h][i + 2]), "+r"(r[h][i + 3]), "+r"(r[h][i + 4]), "+r"(r[h][i + 5]), "+r"(r[h][i + 6]), "+r"(r[h][i + 7]));
+}
+// two products and sums in one instruction, each rounded as fmaf rounds it
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ void fma_pair(float& x, float& y, uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d));
+}
+// A second operand [tokens][dimensions] with the dimensions contiguous (V): MN-major, 128-byte swizzle.  8 tokens are 1024
+// bytes apart (stride offset), the halves of 64 dimensions half_bytes (leading offset; unused where there is one half).
+__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t addr, uint32_t half_bytes) {
+  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(half_bytes >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 
 // added to a descriptor: the first operand is negated
@@ -539,6 +594,14 @@ void count_launch();
 bool pdl_enabled();  // false when the environment has B2_PDL=0
 int encode_tmap_2d(CUtensorMap* out, const void* base, uint64_t inner, uint64_t rows, uint64_t ld_elems,
                    uint32_t box_inner, uint32_t box_rows);
+// heads of `inner` elements side by side in rows
+int encode_tmap_3d(CUtensorMap* out, const void* base, uint64_t inner, uint64_t heads, uint64_t rows, uint64_t ld_elems,
+                   uint32_t box_inner, uint32_t box_heads, uint32_t box_rows);
+
+// Softmax scale * log2(e) for kernels that mask and compare scores before they scale them: its size - masked scores are -inf, and -inf times
+// zero is none -, with the query negated in a negative one's place, which changes no product but for its sign.
+inline float scale_size(float scale) { return std::max(fabsf(scale * 1.4426950408889634f), FLT_MIN); }
+
 
 // What a GEMM's store epilogue does with the accumulator (b2_gemm, b2_gemm_silu_mul, b2_qkv_fused).
 struct StoreEpilogue {

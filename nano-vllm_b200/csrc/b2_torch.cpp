@@ -568,7 +568,7 @@ PyObject* tree_attention(Args a) {
   if (!row_layout(q, nq, hd)) raise(PyExc_AssertionError, "q: heads must lie side by side, in rows on 16-byte boundaries");
   if (!kc.is_contiguous() || !vc.is_contiguous() || !on_16_bytes(kc) || !on_16_bytes(vc)) raise(PyExc_AssertionError, "k_cache and v_cache must be contiguous, on 16-byte boundaries");
   constexpr int64_t limit = (int64_t(1) << 31) - 1;
-  if (kc.size(0) < 1 || kc.size(0) > limit / bs || tables.dim() != 2 || tables.size(1) > limit / bs || n > 1 << 24 || n_seqs > 65535)
+  if (kc.size(0) < 1 || kc.size(0) > limit / bs || tables.dim() != 2 || tables.size(1) > limit / bs || n > 1 << 24 || n_seqs > 1024)
     raise(PyExc_ValueError, "tree_attention: %lld blocks, %lld tokens, %lld sequences", (long long)kc.size(0), (long long)n, (long long)n_seqs);
   vector_of(lens, at::kInt, n_seqs, "context_lens");
   vector_of(cu_q, at::kInt, n_seqs + 1, "cu_seqlens_q");

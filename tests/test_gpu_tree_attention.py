@@ -35,6 +35,13 @@ def ops(pkg, rt):
     return ops
 
 
+@pytest.fixture(autouse=True)
+def no_wait_has_run_out(rt):
+    yield
+    torch.cuda.synchronize()
+    rt.check_status()
+
+
 class Case:
     """Sequences with prefixes[i] tokens before a tree of counts[i] nodes, in a cache whose other places hold NaN."""
 
