@@ -31,6 +31,7 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int TR_ROWS = 128, TR_KEYS = 64, TR_THREADS = 192, TR_CTAS_PER_SM = 2, TR_COLUMNS = 256;
 constexpr int TR_MAX_SEQS = 1024;
+constexpr float TR_GROWTH = 8.f;
 constexpr uint64_t TR_LIMIT_NS = 1000000000ull;
 template <int HD>
 struct Tree {
@@ -243,18 +244,27 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         for (int i = 0; i < HALVES; ++i) b2::tma_load_3d(s_q + i * T::Q_HALF, &tmQ, q_full, i * 64, walk.head * a.group, s.q0 + n0, b2::kEvictNormal);
       }
       __syncwarp();
-      auto load = [&](int j, int no, const CUtensorMap* map, uint32_t full, uint32_t empty, uint32_t dst) {
-        const int st = no % STAGES, tok = j * TR_KEYS, boxes = (min(TR_KEYS, s.len - tok) + a.box - 1) / a.box;
+      // Rows of the cache of 32 boxes at a time, one per lane, and those of the next 32 before they are needed: an entry of the table takes half a
+      // microsecond to arrive.  Tile j of the segment's first is in boxes j * per_tile ...; K runs ahead of V, which keeps its own.
+      const int per_tile = TR_KEYS / a.box, boxes_end = (s.len + a.box - 1) / a.box;
+      auto rows_of = [&](int group) {
+        const int box = walk.t0 * per_tile + group * 32 + lane, p = box * a.box, blk = p / a.block_size;
+        if (box >= boxes_end) return 0;
+        return min(max(0, __ldg(table + blk)), a.num_blocks - 1) * a.block_size + p - blk * a.block_size;  // inside the cache whatever the table holds
+      };
+      int k_rows = rows_of(0), k_next = rows_of(1), v_rows = k_rows, v_next = k_next, k_group = 0, v_group = 0;
+      auto load = [&](int j, int no, const CUtensorMap* map, uint32_t full, uint32_t empty, uint32_t dst, int& rows, int& next, int& group) {
+        const int st = no % STAGES, boxes = (min(TR_KEYS, s.len - (walk.t0 + j) * TR_KEYS) + a.box - 1) / a.box, first = j * per_tile;
+        if (first >> 5 != group) {
+          rows = next;
+          group = first >> 5;
+          next = rows_of(group + 1);
+        }
         if (!all_wait(empty + st * 8, ((no / STAGES) & 1) ^ 1, B2_WAIT_SMEM_EMPTY)) return false;
         const uint32_t bar = full + st * 8;
-        int row = 0;
-        if (lane < boxes) {
-          const int p = tok + lane * a.box, blk = p / a.block_size;
-          row = min(max(0, __ldg(table + blk)), a.num_blocks - 1) * a.block_size + p - blk * a.block_size;  // inside the cache whatever the table holds
-        }
         if (b2::elect_one()) b2::mbar_arrive_expect_tx(bar, boxes * a.box * 128 * HALVES);
         for (int i = 0; i < boxes; ++i) {
-          const int r = __shfl_sync(0xffffffffu, row, i);
+          const int r = __shfl_sync(0xffffffffu, rows, (first + i) & 31);
           if (b2::elect_one())
             for (int h = 0; h < HALVES; ++h)
               b2::tma_load_2d(dst + st * T::TILE + h * T::HALF + i * a.box * 128, map, bar, walk.head * HD + h * 64, r, Y > 1 ? b2::kEvictNormal : b2::kEvictFirst);
@@ -262,13 +272,15 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         __syncwarp();
         return true;
       };
+      auto load_k = [&](int j) { return load(j, c + j, &tmK, k_full, k_empty, s_k, k_rows, k_next, k_group); };
+      auto load_v = [&](int j) { return load(j, c + j, &tmV, v_full, v_empty, s_v, v_rows, v_next, v_group); };
       // in the order of use: K of two tiles, then V of a tile and K of the one after the next
       const int n = walk.t1 - walk.t0;
-      ok = load(walk.t0, c, &tmK, k_full, k_empty, s_k);
-      if (n > 1) ok = ok && load(walk.t0 + 1, c + 1, &tmK, k_full, k_empty, s_k);
+      ok = load_k(0);
+      if (n > 1) ok = ok && load_k(1);
       for (int j = 0; ok && j < n; ++j) {
-        ok = load(walk.t0 + j, c + j, &tmV, v_full, v_empty, s_v);
-        if (j + 2 < n) ok = ok && load(walk.t0 + j + 2, c + j + 2, &tmK, k_full, k_empty, s_k);
+        ok = load_v(j);
+        if (j + 2 < n) ok = ok && load_k(j + 2);
       }
       c += n;
       ++seg;
@@ -391,9 +403,13 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           for (int e = 0; e < 64; e += 4)
 #pragma unroll
             for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(r[e >> 5][(e & 31) + k]));
+          // The reference m moves when a row of the warp is TR_GROWTH past it (or has seen its first key): O then has to be rescaled, which takes as long
+          // as half a tile.  Until then probabilities are up to 2^TR_GROWTH, which costs no bits: they are rounded relative to themselves, and l is the sum
+          // of what they are rounded to, so that a key that outweighs the others keeps its weight of exactly one.
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          const float f = top > m ? b2::ex2((m - top) * a.scale_log2) : 1.f;
-          m = top;
+          const bool grown = __any_sync(0xffffffffu, (top - m) * a.scale_log2 > TR_GROWTH);
+          const float f = grown && top > m ? b2::ex2((m - top) * a.scale_log2) : 1.f;
+          if (grown) m = top;
           const float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
           const uint64_t ref2 = b2::pair_of(-ref, -ref);
 #pragma unroll
@@ -405,14 +421,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             for (int e = 0; e < 32; e += 2) {
               float u, w;
               b2::fma_pair(u, w, b2::pair_of(__uint_as_float(r[h][e]), __uint_as_float(r[h][e + 1])), scale2, ref2);
-              u = b2::ex2(u);
-              w = b2::ex2(w);
-              l[(e >> 1) & 3] = l[(e >> 1) & 3] + u + w;
-              p[e >> 1] = b2::pack_bf16(u, w);
+              p[e >> 1] = b2::pack_bf16(b2::ex2(u), b2::ex2(w));
+              l[(e >> 1) & 3] += b2::bf16_lo(p[e >> 1]) + b2::bf16_hi(p[e >> 1]);
             }
             b2::tmem_st_32x16(t_s + h * 16, p);  // (this row has read its columns)
           }
-          if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+          if (j > 0 && grown) {
             ok = all_wait(o_done + ((i - 1) & 1) * 8, ((i - 1) >> 1) & 1, B2_WAIT_TMEM_FULL);
             if (!ok) break;
             b2::tc_fence_after();

@@ -1,7 +1,8 @@
 """ops.tree_attention on a B200 against its definition in 64 bits on the same bf16 inputs.
 
-Tolerance, per element: the probabilities are rounded to bf16 for the second product, each by at most 2^-8 of itself, which moves the
-result by at most 2^-8 A with A = sum p |v|; the result's own rounding adds 2^-8 (|o| + that).  What is done in 32 bits: a score is a sum of
+Tolerance, per element: the probabilities are rounded to bf16 for the second product, each by at most 2^-8 of itself, and their sum is that of
+the rounded ones: sum p (1 + e) v / sum p (1 + e) is off by sum p e (v - o), at most 2^-8 (A + |o|) with A = sum p |v|; the result's own rounding
+adds 2^-8 (|o| + that).  What is done in 32 bits: a score is a sum of
 head_dim <= 128 products, each partial sum off by 2^-24 of sum |q k|, which here is below 500 * scale * ... : with scores whose terms add up to
 S = scale * sum |q k| the error is below 128 * 2^-24 S = 2^-17 S; exp2's argument and result add 2^-22 (1 + |score|), the sums over n keys
 at most n * 2^-24 for n partial sums one after the other (tiles of 64 and parts: below 2^-13 at 32768 keys if all errors had one sign).  S stays below 64 for the
@@ -94,7 +95,7 @@ def compare(got, want, size, what=""):
     assert torch.equal(torch.isnan(got), nan), f"{what}: NaN in {torch.isnan(got).sum().item()} places, expected {nan.sum().item()}"
     assert torch.equal(got[inf], want[inf]), f"{what}: infinities differ"
     fine = ~(nan | inf)
-    err, bound = (got - want).abs()[fine], ((HALF + FP32) * size + HALF * (want.abs() + (HALF + FP32) * size))[fine]
+    err, bound = (got - want).abs()[fine], ((1 + HALF) * (HALF * (size + want.abs()) + FP32 * size) + HALF * want.abs())[fine]
     if err.numel():
         worst = (err - bound).argmax()
         assert (err <= bound).all(), f"{what}: off by {err[worst].item():.3e}, bound {bound[worst].item():.3e}; {(err > bound).sum().item()} of {err.numel()} elements"
