@@ -195,14 +195,15 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   const uint32_t tmem = b2::uniform(s_tmem);
   const int x = blockIdx.x, y = blockIdx.y, total = first_tile[a.n_seqs] * a.nkv;
 
-  // ---- rows without anything to see: of sequences with a context shorter than their tree, and behind the last sequence ----
-  {
+  // ---- rows without anything to see: of sequences with a context shorter than their tree, and behind the last sequence (by the warps of the
+  // rows, while the first tiles are on their way) ----
+  auto clear_rows = [&]() {
     const int row = a.nq * HD / 8, cta = y * X + x, ctas = X * Y;
     auto clear = [&](int from, int to) {
       from = max(from, 0);
       uint4* out = reinterpret_cast<uint4*>(a.out) + static_cast<int64_t>(from) * row;
       const int64_t n = static_cast<int64_t>(min(to, a.tokens) - from) * row;
-      for (int64_t i = threadIdx.x; i < n; i += TR_THREADS) out[i] = make_uint4(0, 0, 0, 0);
+      for (int64_t i = threadIdx.x; i < n; i += TR_ROWS) out[i] = make_uint4(0, 0, 0, 0);
     };
     for (int b = cta; b < a.n_seqs; b += ctas) {
       const Sequence s = sequence(a, b);
@@ -210,7 +211,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     }
     const int behind = a.n_seqs > 0 ? max(0, __ldg(a.cu_q + a.n_seqs)) : 0;
     for (int t = behind + cta; t < a.tokens; t += ctas) clear(t, t + 1);
-  }
+  };
 
   // ---- this CTA's range ----
   const int per = (total + X - 1) / X;
@@ -229,6 +230,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   int c = 0, seg = 0;  // tiles and segments so far
 
   if (begin >= end) {
+    if (warp < 4) clear_rows();
     if (threadIdx.x == 0) a.joins[y * X + x] = make_int4(0, 0, 0, 0);
   } else if (warp == 4) {
     // ---------------- TMA (the whole warp walks and one thread issues, here and in the next warp) ----------------
@@ -344,6 +346,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     const uint64_t scale2 = b2::pair_of(a.scale_log2, a.scale_log2);
     bool ok = true;
     int4 join = make_int4(0, 0, 0, 0);
+    clear_rows();
     while (ok && walk.next(a, s)) {
       const int n0 = first_node(), nodes = min(a.npt, s.nodes - n0), prefix = s.len - s.nodes;
       if (nodes <= 0) continue;
@@ -355,10 +358,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       const bool idle = warp * 32 >= nodes * a.group;  // none of the warp's rows exists
       for (int j = 0; j < n; ++j) {
         const int i = c + j, buf = i & 1, place = (walk.t0 + j) * TR_KEYS, off = place - prefix, there = s.len - place;
+        const bool special = off > -TR_KEYS || there < TR_KEYS;
+        uint64_t sees = off > -TR_KEYS ? visible(mask, a.words, off) : ~0ull;  // (on its way while the scores are)
+        if (there < TR_KEYS) sees &= (1ull << there) - 1;
         ok = all_wait(s_full + buf * 8, (i >> 1) & 1, B2_WAIT_TMEM_FULL);
         if (!ok) break;
         b2::tc_fence_after();
-        const bool special = off > -TR_KEYS || there < TR_KEYS;
         if (special) {
           // Rows of V past the context's end count as zero, and so do infinities and NaN in the tree's: a row that does not see them
           // has a probability of zero there, and zero times them is NaN.
@@ -391,8 +396,6 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           b2::tmem_ld_32x32(t_s + 32, r[1]);
           b2::tc_wait_ld(r);
           if (special) {
-            uint64_t sees = off > -TR_KEYS ? visible(mask, a.words, off) : ~0ull;
-            if (there < TR_KEYS) sees &= (1ull << there) - 1;
             const uint32_t half[2] = {static_cast<uint32_t>(sees), static_cast<uint32_t>(sees >> 32)};
 #pragma unroll
             for (int e = 0; e < 64; ++e)
@@ -517,22 +520,24 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 }
 
 // Joins the parts of the items that several ranges share: O = sum w O_k / sum w l_k with w = exp2(m_k - max m), the parts in the order of
-// their keys.  A block takes 32 rows and 16 dimensions of an item, its warps every eighth part each.
-constexpr int TC_WARPS = 8, TC_ROWS = 32, TC_DIMS = 16;
+// their keys.  Few parts: a block takes 32 rows and 64 dimensions of an item, every thread all parts of its elements.  Many: 32 rows and 16 dimensions,
+// its warps every eighth part each, which then meet in shared memory.  (64 sequences of 4096 tokens, 128 rows, 2 to 3 parts an item: 60 us where the
+// warps always shared the parts, of which most had none.)
+constexpr int TC_WARPS = 8, TC_ROWS = 32, TC_FEW = 16;
 template <int HD>
 __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const TreeArgs a, int X, int Y) {
   using T = Tree<HD>;
   __shared__ int s_units[TC_WARPS * 32 + 1], s_sum[TC_WARPS];
   __shared__ float s_m[TC_WARPS][TC_ROWS], s_l[TC_WARPS][TC_ROWS];
-  __shared__ float4 s_o[TC_WARPS][TC_DIMS / 4][TC_ROWS];
+  __shared__ float4 s_o[TC_WARPS][4][TC_ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = X * Y;
   b2::pdl_launch_dependents();
   b2::pdl_wait();
-  // units of all items, prefix-summed in chunks of a block's threads (there is one chunk, or a few)
+  // units of all items, prefix-summed in chunks of a block's threads (there are one or two)
   int before = 0;
   for (int i0 = 0; i0 < n; i0 += TC_WARPS * 32) {
     const int4 mine = i0 + tid < n ? a.joins[i0 + tid] : make_int4(0, 0, 0, 0);
-    const int units = mine.x > 0 ? (mine.z * a.group + TC_ROWS - 1) / TC_ROWS * (HD / TC_DIMS) : 0;
+    const int units = mine.x > 0 ? (mine.z * a.group + TC_ROWS - 1) / TC_ROWS * (HD / (mine.x <= TC_FEW ? 64 : 16)) : 0;
     int incl = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -548,7 +553,7 @@ __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const TreeA
     if (tid == TC_WARPS * 32 - 1) s_units[TC_WARPS * 32] = at + incl;
     __syncthreads();
     const int all = s_units[TC_WARPS * 32];
-    int u = blockIdx.x - before % gridDim.x;
+    int u = static_cast<int>(blockIdx.x) - before % static_cast<int>(gridDim.x);
     if (u < 0) u += gridDim.x;
     for (; u < all; u += gridDim.x) {
       int lo = 0, hi = TC_WARPS * 32 - 1;  // the last entry that begins at or before u
@@ -557,52 +562,72 @@ __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const TreeA
         if (s_units[mid] <= u) lo = mid;
         else hi = mid - 1;
       }
-      const int4 join = a.joins[i0 + lo];
-      const int part = u - s_units[lo], row = part / (HD / TC_DIMS) * TC_ROWS + lane, dims = part % (HD / TC_DIMS) * TC_DIMS, e = i0 + lo;
-      const bool exists = row < join.z * a.group;
+      const int e = i0 + lo, part = u - s_units[lo];
+      const int4 join = a.joins[e];
+      const int parts = join.x;
       // the item begins in range e (its slot [1]) and goes on in the ranges after it (their slots [0])
       auto slot = [&](int k) { return a.parts + (k == 0 ? static_cast<int64_t>(Y) * X + e : static_cast<int64_t>(e) + k) * T::SLOT; };
-      float mx = -INFINITY, sum = 0.f;
-      float4 acc[TC_DIMS / 4];
-#pragma unroll
-      for (int d = 0; d < TC_DIMS / 4; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (exists) {
-        for (int k = warp; k < join.x; k += TC_WARPS) mx = fmaxf(mx, slot(k)[HD * TR_ROWS + row]);
-#pragma unroll 2
-        for (int k = warp; k < join.x; k += TC_WARPS) {
+      auto store = [&](int row, int dim, const float4& o, float l) {
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const int token = join.y + row / a.group, head = join.w * a.group + row % a.group;
+        *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(token) * a.nq + head) * HD + dim) = make_uint2(b2::pack_bf16(o.x * inv, o.y * inv), b2::pack_bf16(o.z * inv, o.w * inv));
+      };
+      auto add = [](float4& acc, float f, const float4& o) { acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w; };
+      // 0 for a part that saw nothing where another one did; 1 where none did, or for an infinity
+      auto weight = [&](float m, float top) { return m == top ? 1.f : b2::ex2((m - top) * a.scale_log2); };
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (parts <= TC_FEW) {
+        const int row = part / (HD / 64) * TC_ROWS + lane, quad = part % (HD / 64) * 16 + warp;
+        if (row >= join.z * a.group) continue;
+        float top = -INFINITY, l = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < parts; ++k) top = fmaxf(top, slot(k)[HD * TR_ROWS + row]);
+        float4 o0 = zero, o1 = zero;
+#pragma unroll 4
+        for (int k = 0; k < parts; ++k) {
           const float* p = slot(k);
-          const float m = p[HD * TR_ROWS + row], f = m == mx ? 1.f : b2::ex2((m - mx) * a.scale_log2);
+          const float f = weight(p[HD * TR_ROWS + row], top);
+          l += f * p[(HD + 1) * TR_ROWS + row];
+          add(o0, f, *reinterpret_cast<const float4*>(p + (quad * TR_ROWS + row) * 4));
+          add(o1, f, *reinterpret_cast<const float4*>(p + ((quad + 8) * TR_ROWS + row) * 4));
+        }
+        store(row, quad * 4, o0, l);
+        store(row, (quad + 8) * 4, o1, l);
+        continue;
+      }
+      const int row = part / (HD / 16) * TC_ROWS + lane, quad = part % (HD / 16) * 4;
+      const bool exists = row < join.z * a.group;
+      float mx = -INFINITY, sum = 0.f;
+      float4 acc[4] = {zero, zero, zero, zero};
+      if (exists) {
+        for (int k = warp; k < parts; k += TC_WARPS) mx = fmaxf(mx, slot(k)[HD * TR_ROWS + row]);
+#pragma unroll 2
+        for (int k = warp; k < parts; k += TC_WARPS) {
+          const float* p = slot(k);
+          const float f = weight(p[HD * TR_ROWS + row], mx);
           sum += f * p[(HD + 1) * TR_ROWS + row];
 #pragma unroll
-          for (int d = 0; d < TC_DIMS / 4; ++d) {
-            const float4 o = *reinterpret_cast<const float4*>(p + ((dims / 4 + d) * TR_ROWS + row) * 4);
-            acc[d].x += f * o.x; acc[d].y += f * o.y; acc[d].z += f * o.z; acc[d].w += f * o.w;
-          }
+          for (int d = 0; d < 4; ++d) add(acc[d], f, *reinterpret_cast<const float4*>(p + ((quad + d) * TR_ROWS + row) * 4));
         }
       }
       __syncthreads();
       s_m[warp][lane] = mx;
       s_l[warp][lane] = sum;
 #pragma unroll
-      for (int d = 0; d < TC_DIMS / 4; ++d) s_o[warp][d][lane] = acc[d];
+      for (int d = 0; d < 4; ++d) s_o[warp][d][lane] = acc[d];
       __syncthreads();
-      if (warp < TC_DIMS / 4 && exists) {
+      if (warp < 4 && exists) {
         float top = -INFINITY, l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 o = zero;
 #pragma unroll
         for (int w = 0; w < TC_WARPS; ++w) top = fmaxf(top, s_m[w][lane]);
 #pragma unroll
         for (int w = 0; w < TC_WARPS; ++w) {
-          if (w >= join.x) break;
-          const float m = s_m[w][lane], f = m == top ? 1.f : b2::ex2((m - top) * a.scale_log2);
-          const float4 v = s_o[w][warp][lane];
+          const float f = weight(s_m[w][lane], top);
           l += f * s_l[w][lane];
-          o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+          add(o, f, s_o[w][warp][lane]);
         }
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        const int token = join.y + row / a.group, head = join.w * a.group + row % a.group;
-        *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(token) * a.nq + head) * HD + dims + warp * 4) =
-            make_uint2(b2::pack_bf16(o.x * inv, o.y * inv), b2::pack_bf16(o.z * inv, o.w * inv));
+        store(row, (quad + warp) * 4, o, l);
       }
     }
     before += all;
