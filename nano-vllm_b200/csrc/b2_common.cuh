@@ -391,6 +391,12 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r)
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // tcgen05.wait::ld, before which nothing reads the 64 columns
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[32]) {
+  tc_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
 __device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[2][32]) {
   tc_wait_ld();
 #pragma unroll
@@ -410,6 +416,17 @@ __device__ __forceinline__ void fma_pair(float& x, float& y, uint64_t a, uint64_
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d));
 }
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ void halves_of(uint64_t p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
 // A second operand [tokens][dimensions] with the dimensions contiguous (V): MN-major, 128-byte swizzle.  8 tokens are 1024
 // bytes apart (stride offset), the halves of 64 dimensions half_bytes (leading offset; unused where there is one half).
 __device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t addr, uint32_t half_bytes) {

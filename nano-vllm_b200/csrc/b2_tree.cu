@@ -28,9 +28,11 @@ namespace {
 //   warp 4       TMA: Q of the segment, then K and V tiles
 //   warp 5       tcgen05.mma: S = Q K^T (128 x 64, two buffers, so that the next tile's scores are there before this one's are done
 //                with), O += P V with P read from tensor memory
+// (Two threads per row, 32 keys each, which tell each other their maxima: 83 us instead of 73 for one context of 32768 tokens, tree of 64, 64 / 8 heads.)
 // ---------------------------------------------------------------------------
-constexpr int TR_ROWS = 128, TR_KEYS = 64, TR_THREADS = 192, TR_CTAS_PER_SM = 2, TR_COLUMNS = 256;
+constexpr int TR_ROWS = 128, TR_KEYS = 64, TR_THREADS = TR_ROWS + 64, TR_CTAS_PER_SM = 2, TR_COLUMNS = 256;
 constexpr int TR_MAX_SEQS = 1024;
+constexpr int TR_ITEM_UNITS = 2;
 constexpr float TR_GROWTH = 8.f;
 constexpr uint64_t TR_LIMIT_NS = 1000000000ull;
 template <int HD>
@@ -44,7 +46,7 @@ struct Tree {
   static constexpr size_t smem(int n_seqs) { return 1024 + Q + 2 * STAGES * TILE + (n_seqs + 1) * sizeof(int); }
   static constexpr int SLOT = TR_ROWS * (HD + 2);           // floats of a part: O as [HD / 4][row][4], then the maxima and the sums
 };
-static_assert(2 * (Tree<128>::smem(TR_MAX_SEQS) + 2048) <= 228 * 1024, "two CTAs per SM (2048: static, reserved)");
+static_assert(2 * (Tree<128>::smem(TR_MAX_SEQS) + 2048) <= 228 * 1024, "two CTAs per SM (2 KB: static, reserved)");
 
 struct TreeArgs {
   const uint16_t* v;
@@ -74,33 +76,36 @@ __device__ __forceinline__ Sequence sequence(const TreeArgs& a, int b) {
 }
 __device__ __forceinline__ int tiles_of(int len) { return (len + TR_KEYS - 1) / TR_KEYS; }
 
-// A range [pos, end) of the batch's tiles as segments that lie inside one item.  A sequence with more nodes than gridDim.y tiles of rows hold is
-// walked several times (pass).
+// A range [pos, end) of the batch's units as segments that lie inside one item.  An item has a unit for each of its tiles and, before those,
+// TR_ITEM_UNITS for its beginning and its end (loading Q, the tree's masks, storing O).  A sequence with more nodes than gridDim.y tiles of rows hold
+// is walked several times (pass).  A segment may hold no tiles (t0 >= t1).
 struct TreeWalk {
-  const int* first_tile;  // [n_seqs + 1] tiles per KV head before each sequence
+  const int* first_unit_of;  // [n_seqs + 1] units per KV head before each sequence
   int nkv, pos, end, b, head, pass, tiles, t0, t1;
-  __device__ __forceinline__ TreeWalk(const int* ft, int n_seqs, int heads, int begin, int stop) : first_tile(ft), nkv(heads), pos(begin), end(stop), b(0) {
+  __device__ __forceinline__ TreeWalk(const int* fu, int n_seqs, int heads, int begin, int stop) : first_unit_of(fu), nkv(heads), pos(begin), end(stop), b(0) {
     int hi = n_seqs - 1;
     while (b < hi) {
       const int mid = (b + hi + 1) >> 1;
-      if (first_tile[mid] * nkv <= pos) b = mid;
+      if (first_unit_of[mid] * nkv <= pos) b = mid;
       else hi = mid - 1;
     }
   }
   __device__ __forceinline__ bool next(const TreeArgs& a, Sequence& s) {
     if (pos >= end) return false;
-    while (first_tile[b + 1] * nkv <= pos) ++b;
+    while (first_unit_of[b + 1] * nkv <= pos) ++b;
     s = sequence(a, b);
     tiles = tiles_of(s.len);
-    const int in_seq = pos - first_tile[b] * nkv, item = in_seq / tiles;
+    const int units = tiles + TR_ITEM_UNITS, in_seq = pos - first_unit_of[b] * nkv, item = in_seq / units;
     pass = item / nkv;
     head = item - pass * nkv;
-    t0 = in_seq - item * tiles;
-    t1 = min(tiles, t0 + end - pos);
-    pos += t1 - t0;
+    const int u0 = in_seq - item * units, u1 = min(units, u0 + end - pos);
+    pos += u1 - u0;
+    t0 = max(0, u0 - TR_ITEM_UNITS);
+    t1 = u1 - TR_ITEM_UNITS;
     return true;
   }
-  __device__ __forceinline__ int item_begin() const { return pos - t1; }
+  // the unit of the item's first tile, after a segment that holds some
+  __device__ __forceinline__ int first_unit() const { return pos - t1; }
 };
 
 // Bits 64 tile .. of what row `words` of the mask sees, for a tile that begins `off` places after the tree does (before it: negative)
@@ -141,7 +146,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t s_q = b2::smem_u32(smem), s_k = s_q + T::Q, s_v = s_k + STAGES * T::TILE;
-  int* first_tile = reinterpret_cast<int*>(smem + T::Q + 2 * STAGES * T::TILE);
+  int* first_unit = reinterpret_cast<int*>(smem + T::Q + 2 * STAGES * T::TILE);
   __shared__ __align__(8) uint64_t s_bars[2 + 4 * STAGES + 6];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_unbounded[2];
@@ -153,7 +158,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     b2::tma_prefetch_desc(&tmQ);
     b2::tma_prefetch_desc(&tmK);
     b2::tma_prefetch_desc(&tmV);
-    for (int i = 0; i < 2 + 4 * STAGES + 6; ++i) b2::mbar_init(q_full + i * 8, q_full + i * 8 == p_full || q_full + i * 8 == p_full + 8 ? 4 : 1);
+    for (int i = 0; i < 2 + 4 * STAGES + 6; ++i) b2::mbar_init(q_full + i * 8, q_full + i * 8 == p_full || q_full + i * 8 == p_full + 8 ? TR_ROWS / 32 : 1);
     s_abort = 0;
     s_unbounded[0] = s_unbounded[1] = -1;
     b2::mbar_fence_init();
@@ -165,7 +170,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   b2::pdl_launch_dependents();
   b2::pdl_wait();
 
-  // ---- tiles per sequence, prefix-summed by one warp ----
+  // ---- units per sequence, prefix-summed by one warp ----
   const int X = gridDim.x, Y = gridDim.y, rows_y = Y * a.npt;
   if (warp == 0) {
     const int per = (a.n_seqs + 31) / 32, s0 = lane * per;
@@ -174,8 +179,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     for (int i = 0; i < per; ++i)
       if (s0 + i < a.n_seqs) {
         const Sequence s = sequence(a, s0 + i);
-        const int all = s.len > 0 ? tiles_of(s.len) * ((s.nodes + rows_y - 1) / rows_y) : 0;
-        first_tile[s0 + i + 1] = all;
+        const int all = s.len > 0 ? (tiles_of(s.len) + TR_ITEM_UNITS) * ((s.nodes + rows_y - 1) / rows_y) : 0;
+        first_unit[s0 + i + 1] = all;
         mine += all;
       }
     int incl = mine;
@@ -185,15 +190,15 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       if (lane >= o) incl += up;
     }
     int at = incl - mine;
-    if (lane == 0) first_tile[0] = 0;
+    if (lane == 0) first_unit[0] = 0;
     for (int i = 0; i < per; ++i)
-      if (s0 + i < a.n_seqs) first_tile[s0 + i + 1] = at += first_tile[s0 + i + 1];
+      if (s0 + i < a.n_seqs) first_unit[s0 + i + 1] = at += first_unit[s0 + i + 1];
   }
   b2::tc_fence_before();
   __syncthreads();
   b2::tc_fence_after();
   const uint32_t tmem = b2::uniform(s_tmem);
-  const int x = blockIdx.x, y = blockIdx.y, total = first_tile[a.n_seqs] * a.nkv;
+  const int x = blockIdx.x, y = blockIdx.y, total = first_unit[a.n_seqs] * a.nkv;
 
   // ---- rows without anything to see: of sequences with a context shorter than their tree, and behind the last sequence (by the warps of the
   // rows, while the first tiles are on their way) ----
@@ -215,12 +220,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 
   // ---- this CTA's range ----
   const int per = (total + X - 1) / X;
-  const int ctas = min(X, per <= 8 ? (total + max(1, per) - 1) / max(1, per) : X);
+  const int ctas = min(X, per <= TR_ITEM_UNITS + 6 ? (total + max(1, per) - 1) / max(1, per) : X);
   const int base = ctas > 0 ? total / ctas : 0, rem = ctas > 0 ? total % ctas : 0;
   auto begin_of = [&](int i) { return i * base + min(i, rem); };
   auto cta_of = [&](int t) { const int big = rem * (base + 1); return t < big ? t / (base + 1) : rem + (t - big) / base; };
   const int begin = x < ctas ? begin_of(x) : 0, end = x < ctas ? begin_of(x + 1) : 0;
-  TreeWalk walk(first_tile, a.n_seqs, a.nkv, begin, end);
+  TreeWalk walk(first_unit, a.n_seqs, a.nkv, begin, end);
   Sequence s;
   auto all_wait = [&](uint32_t bar, uint32_t phase, int code) {
     return __all_sync(0xffffffffu, b2::mbar_wait(bar, phase, abort_flag, TR_LIMIT_NS, code)) != 0;
@@ -237,7 +242,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     bool ok = true;
     while (ok && walk.next(a, s)) {
       const int n0 = first_node();
-      if (n0 >= s.nodes) continue;
+      if (n0 >= s.nodes || walk.t0 >= walk.t1) continue;
       const int32_t* table = a.tables + static_cast<int64_t>(walk.b) * a.bt_stride;
       ok = all_wait(q_empty, (seg & 1) ^ 1, B2_WAIT_SMEM_EMPTY);
       if (!ok) break;
@@ -317,7 +322,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     };
     bool ok = true;
     while (ok && walk.next(a, s)) {
-      if (first_node() >= s.nodes) continue;
+      if (first_node() >= s.nodes || walk.t0 >= walk.t1) continue;
       const int n = walk.t1 - walk.t0;
       ok = wait(q_full, seg & 1, B2_WAIT_SMEM_FULL) && scores(c, n == 1);
       if (n > 1) ok = ok && scores(c + 1, n == 2);
@@ -349,12 +354,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     clear_rows();
     while (ok && walk.next(a, s)) {
       const int n0 = first_node(), nodes = min(a.npt, s.nodes - n0), prefix = s.len - s.nodes;
-      if (nodes <= 0) continue;
+      if (nodes <= 0 || walk.t0 >= walk.t1) continue;
       const int n = walk.t1 - walk.t0;
       const int token = s.q0 + n0 + min(my_node, nodes - 1);  // (rows behind the last node go along with it)
       const int64_t* mask = a.mask + static_cast<int64_t>(token) * a.mask_stride;
       float m = -INFINITY;  // the row's maximum, in units of scores
-      float l[4] = {};      // its sum, of columns 2 i and 2 i + 1 of every eight
+      uint64_t l[2] = {};   // its sum, in two pairs
       const bool idle = warp * 32 >= nodes * a.group;  // none of the warp's rows exists
       for (int j = 0; j < n; ++j) {
         const int i = c + j, buf = i & 1, place = (walk.t0 + j) * TR_KEYS, off = place - prefix, there = s.len - place;
@@ -407,16 +412,17 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 #pragma unroll
             for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(r[e >> 5][(e & 31) + k]));
           // The reference m moves when a row of the warp is TR_GROWTH past it (or has seen its first key): O then has to be rescaled, which takes as long
-          // as half a tile.  Until then probabilities are up to 2^TR_GROWTH, which costs no bits: they are rounded relative to themselves, and l is the sum
-          // of what they are rounded to, so that a key that outweighs the others keeps its weight of exactly one.
+          // as half a tile.  Until then probabilities are up to 2^TR_GROWTH, which costs no bits: they are rounded relative to themselves.
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           const bool grown = __any_sync(0xffffffffu, (top - m) * a.scale_log2 > TR_GROWTH);
           const float f = grown && top > m ? b2::ex2((m - top) * a.scale_log2) : 1.f;
           if (grown) m = top;
           const float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
           const uint64_t ref2 = b2::pair_of(-ref, -ref);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) l[k] *= f;
+          if (grown) {
+            l[0] = b2::mul_pair(l[0], b2::pair_of(f, f));
+            l[1] = b2::mul_pair(l[1], b2::pair_of(f, f));
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t p[16];
@@ -424,8 +430,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             for (int e = 0; e < 32; e += 2) {
               float u, w;
               b2::fma_pair(u, w, b2::pair_of(__uint_as_float(r[h][e]), __uint_as_float(r[h][e + 1])), scale2, ref2);
-              p[e >> 1] = b2::pack_bf16(b2::ex2(u), b2::ex2(w));
-              l[(e >> 1) & 3] += b2::bf16_lo(p[e >> 1]) + b2::bf16_hi(p[e >> 1]);
+              u = b2::ex2(u);
+              w = b2::ex2(w);
+              l[(e >> 1) & 1] = b2::add_pair(l[(e >> 1) & 1], b2::pair_of(u, w));
+              p[e >> 1] = b2::pack_bf16(u, w);
             }
             b2::tmem_st_32x16(t_s + h * 16, p);  // (this row has read its columns)
           }
@@ -457,7 +465,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       b2::tc_fence_after();
       const bool whole = walk.t0 == 0 && walk.t1 == walk.tiles;
       if (!idle) {
-        const float sum = (l[0] + l[2]) + (l[1] + l[3]), inv = sum != 0.f ? 1.f / sum : 0.f;  // (nothing seen: zeros)
+        float sums[2];
+        b2::halves_of(b2::add_pair(l[0], l[1]), sums[0], sums[1]);
+        const float sum = sums[0] + sums[1], inv = sum != 0.f ? 1.f / sum : 0.f;  // (nothing seen: zeros)
         const bool exists = my_node < nodes;
         const bool add = *reinterpret_cast<volatile int*>(&s_unbounded[seg & 1]) == seg;
         const int32_t* table = a.tables + static_cast<int64_t>(walk.b) * a.bt_stride;
@@ -499,7 +509,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         }
       }
       if (walk.t0 == 0 && walk.t1 < walk.tiles) {
-        const int first = walk.item_begin();
+        const int first = walk.first_unit();
         join = make_int4(cta_of(first + walk.tiles - 1) - cta_of(first) + 1, s.q0 + n0, nodes, walk.head);
       }
       ++seg;
@@ -523,13 +533,15 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 // their keys.  Few parts: a block takes 32 rows and 64 dimensions of an item, every thread all parts of its elements.  Many: 32 rows and 16 dimensions,
 // its warps every eighth part each, which then meet in shared memory.  (64 sequences of 4096 tokens, 128 rows, 2 to 3 parts an item: 60 us where the
 // warps always shared the parts, of which most had none.)
-constexpr int TC_WARPS = 8, TC_ROWS = 32, TC_FEW = 16;
+constexpr int TC_WARPS = 8, TC_ROWS = 32, TC_FEW = 16, TC_CTAS_PER_SM = 4;
 template <int HD>
-__global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const TreeArgs a, int X, int Y) {
+__global__ void __launch_bounds__(TC_WARPS * 32, TC_CTAS_PER_SM) tree_combine_kernel(const TreeArgs a, int X, int Y) {
   using T = Tree<HD>;
   __shared__ int s_units[TC_WARPS * 32 + 1], s_sum[TC_WARPS];
   __shared__ float s_m[TC_WARPS][TC_ROWS], s_l[TC_WARPS][TC_ROWS];
   __shared__ float4 s_o[TC_WARPS][4][TC_ROWS];
+  __shared__ int4 s_join[TC_WARPS * 32];
+  __shared__ __align__(16) uint16_t s_out[TC_ROWS][64 + 8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = X * Y;
   b2::pdl_launch_dependents();
   b2::pdl_wait();
@@ -550,6 +562,7 @@ __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const TreeA
     int at = 0;
     for (int w = 0; w < warp; ++w) at += s_sum[w];
     s_units[tid] = at + incl - units;
+    s_join[tid] = mine;
     if (tid == TC_WARPS * 32 - 1) s_units[TC_WARPS * 32] = at + incl;
     __syncthreads();
     const int all = s_units[TC_WARPS * 32];
@@ -563,7 +576,7 @@ __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const TreeA
         else hi = mid - 1;
       }
       const int e = i0 + lo, part = u - s_units[lo];
-      const int4 join = a.joins[e];
+      const int4 join = s_join[lo];
       const int parts = join.x;
       // the item begins in range e (its slot [1]) and goes on in the ranges after it (their slots [0])
       auto slot = [&](int k) { return a.parts + (k == 0 ? static_cast<int64_t>(Y) * X + e : static_cast<int64_t>(e) + k) * T::SLOT; };
@@ -578,21 +591,50 @@ __global__ void __launch_bounds__(TC_WARPS * 32) tree_combine_kernel(const TreeA
       const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
       if (parts <= TC_FEW) {
         const int row = part / (HD / 64) * TC_ROWS + lane, quad = part % (HD / 64) * 16 + warp;
-        if (row >= join.z * a.group) continue;
+        const int rows = join.z * a.group;
         float top = -INFINITY, l = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < parts; ++k) top = fmaxf(top, slot(k)[HD * TR_ROWS + row]);
         float4 o0 = zero, o1 = zero;
-#pragma unroll 4
-        for (int k = 0; k < parts; ++k) {
-          const float* p = slot(k);
-          const float f = weight(p[HD * TR_ROWS + row], top);
-          l += f * p[(HD + 1) * TR_ROWS + row];
-          add(o0, f, *reinterpret_cast<const float4*>(p + (quad * TR_ROWS + row) * 4));
-          add(o1, f, *reinterpret_cast<const float4*>(p + ((quad + 8) * TR_ROWS + row) * 4));
+        for (int k0 = 0; row < rows && k0 < parts; k0 += 4) {  // four parts at a time, all of them on their way at once
+          float m[4], sums[4];
+          float4 u[4], w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            m[k] = -INFINITY;
+            sums[k] = 0.f;
+            u[k] = w[k] = zero;
+            if (k0 + k < parts) {
+              const float* p = slot(k0 + k);
+              m[k] = p[HD * TR_ROWS + row];
+              sums[k] = p[(HD + 1) * TR_ROWS + row];
+              u[k] = *reinterpret_cast<const float4*>(p + (quad * TR_ROWS + row) * 4);
+              w[k] = *reinterpret_cast<const float4*>(p + ((quad + 8) * TR_ROWS + row) * 4);
+            }
+          }
+          const float before = top;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = fmaxf(top, m[k]);
+          const float g = weight(before, top);
+          l *= g;
+          o0.x *= g; o0.y *= g; o0.z *= g; o0.w *= g;
+          o1.x *= g; o1.y *= g; o1.z *= g; o1.w *= g;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float f = weight(m[k], top);
+            l += f * sums[k];
+            add(o0, f, u[k]);
+            add(o1, f, w[k]);
+          }
         }
-        store(row, quad * 4, o0, l);
-        store(row, (quad + 8) * 4, o1, l);
+        // through shared memory, so that the stores are of whole pieces of rows
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        __syncthreads();  // (the unit before has left)
+        *reinterpret_cast<uint2*>(&s_out[lane][warp * 4]) = make_uint2(b2::pack_bf16(o0.x * inv, o0.y * inv), b2::pack_bf16(o0.z * inv, o0.w * inv));
+        *reinterpret_cast<uint2*>(&s_out[lane][warp * 4 + 32]) = make_uint2(b2::pack_bf16(o1.x * inv, o1.y * inv), b2::pack_bf16(o1.z * inv, o1.w * inv));
+        __syncthreads();
+        const int r = row - lane + (tid >> 3);
+        if (r < rows)
+          *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(join.y + r / a.group) * a.nq + join.w * a.group + r % a.group) * HD + part % (HD / 64) * 64 + (tid & 7) * 8) =
+              *reinterpret_cast<const uint4*>(&s_out[tid >> 3][(tid & 7) * 8]);
         continue;
       }
       const int row = part / (HD / 16) * TC_ROWS + lane, quad = part % (HD / 16) * 4;
@@ -643,7 +685,7 @@ TreePlan plan_tree(const b2_ctx* ctx, int n_seqs, int max_q, int group, int nkv,
   TreePlan p;
   p.npt = TR_ROWS / group;
   p.y = std::max(1, std::min((max_q + p.npt - 1) / p.npt, 8));
-  const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(n_seqs) * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS) * ((max_q + p.npt * p.y - 1) / (p.npt * p.y)));
+  const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(n_seqs) * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS + TR_ITEM_UNITS) * ((max_q + p.npt * p.y - 1) / (p.npt * p.y)));
   p.x = static_cast<int>(std::min<int64_t>(most, std::max(1, ctx->num_sms * TR_CTAS_PER_SM / p.y)));
   p.slot_bytes = static_cast<int64_t>(head_dim == 128 ? Tree<128>::SLOT : Tree<64>::SLOT) * sizeof(float);
   p.bytes = static_cast<int64_t>(p.x) * p.y * (2 * p.slot_bytes + sizeof(int4));
@@ -695,7 +737,7 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
   const TreePlan p = plan_tree(ctx, n_seqs, max_q, nq / nkv, nkv, head_dim, max_len);
   // (tiles are counted in 32 bits: those of all sequences and heads, a pass for every gridDim.y tiles of rows)
   const int64_t passes = (static_cast<int64_t>(tokens) + p.npt * p.y - 1) / (p.npt * p.y) + n_seqs;
-  if (static_cast<int64_t>(num_blocks) * block_size >= 1ll << 31 || max_len >= 1ll << 31 || passes * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS) >= 1ll << 31)
+  if (static_cast<int64_t>(num_blocks) * block_size >= 1ll << 31 || max_len >= 1ll << 31 || passes * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS + TR_ITEM_UNITS) >= 1ll << 31)
     return b2::set_error(B2_ERR_SHAPE, "%lld slots, tables of %lld tokens", static_cast<long long>(num_blocks) * block_size, static_cast<long long>(max_len));
   if (workspace_bytes < p.bytes) return B2_ERR_ARG;
   const int rc = configure_once();
@@ -734,7 +776,7 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
   const size_t smem = head_dim == 128 ? Tree<128>::smem(n_seqs) : Tree<64>::smem(n_seqs);
   B2_CUDA(b2_launch(head_dim == 128 ? tree_attention_kernel<128> : tree_attention_kernel<64>, dim3(p.x, p.y), dim3(TR_THREADS), smem, on, tmQ, tmK, tmV, a));
-  B2_CUDA(b2_launch(head_dim == 128 ? tree_combine_kernel<128> : tree_combine_kernel<64>, dim3(2 * ctx->num_sms), dim3(TC_WARPS * 32), 0, on, a, p.x, p.y));
+  B2_CUDA(b2_launch(head_dim == 128 ? tree_combine_kernel<128> : tree_combine_kernel<64>, dim3(TC_CTAS_PER_SM * ctx->num_sms), dim3(TC_WARPS * 32), 0, on, a, p.x, p.y));
   return B2_OK;
 }
 
