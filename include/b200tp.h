@@ -491,7 +491,7 @@ int b2_prefill_attention_supported(int nq, int nkv, int head_dim, int block_size
  * (0: a padded sequence) and rows behind the last sequence are zero.  max_q: the most nodes of a sequence.  scale: of either sign, or zero.
  * b2_tree_attention_supported says (1 / 0) whether the shape is served: head_dim 64 or 128, up to 128 query heads per KV head, blocks of
  * a multiple of 16 tokens.  b2_tree_attention_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant; calls
- * that may run at the same time need one each), or -1 where the shape is not served. */
+ * that may run at the same time need one each), or -1 where the shape is not served; at most 1024 sequences. */
 int b2_tree_attention_supported(int nq, int nkv, int head_dim, int block_size);
 int64_t b2_tree_attention_workspace(b2_ctx* ctx, int n_seqs, int max_q, int nq, int nkv, int head_dim, int block_size, int bt_width);
 int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int num_blocks, int block_size,
@@ -527,7 +527,7 @@ typedef struct b2_logit_rules {
   const int64_t* tree_mask;    /* [rows, mask_words], as for b2_tree_attention: the nodes a row sees are its path */
   int64_t mask_stride;
   int mask_words;
-} b2_logit_rules; /* token ids outside the vocabulary are ignored */
+} b2_logit_rules; /* token ids outside the vocabulary are ignored; n_bias <= 4095, history_width + 64 mask_words < 2^19 (B2_ERR_SHAPE otherwise) */
 int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, int fp32, int rows, int vocab, const b2_logit_rules* rules, void* stream);
 
 /* Greedy pick: out[i] = argmax_j logits[i, j] (first index on ties), int64.

@@ -7,8 +7,6 @@
 namespace {
 
 // ---------------------------------------------------------------------------
-// adjust_logits_kernel
-//
 // For a row of logits that belongs to request s, token v, with `count` its occurrences in the request's output (and on the row's path of
 // drafted tokens) and `seen` whether it occurs there or in the prompt, in 32 bits and in this order:
 //   x = seen ? (x > 0 ? x / repetition : x * repetition) : x
@@ -17,21 +15,34 @@ namespace {
 //   x = allowed ? x : -inf
 // and one rounding to the logits' type.  Logits that no rule touches are copied bit for bit.
 //
-// Bound: HBM, logits in and out once.  A CTA takes a slice of the vocabulary for one row, or for several rows of a batch of trees: it
-// counts the request's history into shared memory (all of it is read, the tokens of the slice count), marks the touched tokens in a
-// bitmap and walks the slice in 16-byte vectors, of which only those with a marked or forbidden token are unpacked.  No counts
-// live in memory between calls: the state of a request is the list of its tokens.
+// Bound: HBM, logits in and out once.  Two kernels:
+//
+// mask_logits_kernel moves all logits, 16-byte vectors with the forbidden tokens masked a word at a time.  It is left out where out is the
+// logits and there is no mask.
+//
+// rules_kernel stores the few that history, biases and paths touch, over what the first one stored.  A CTA takes every P-th token of
+// one request: it counts the history into a word of shared memory for each of its tokens (all of it is read, its own tokens count; text repeats low
+// ids, and they are spread over the P CTAs), and whoever finds a word at zero lists its token.  The list is worked through a token to a thread, for four
+// of the request's rows - a tree's nodes - at a time.  A token on a row's path of drafted tokens is marked: it is not the list's, but the thread's of the
+// path's first node that has it.  All that needs no logits stored is done while the first kernel is still at work.  No counts live in memory between calls:
+// the state of a request is the list of its tokens.  Counting works on whole numbers and every store is one thread's, so that the order changes nothing.
+//
+// (One kernel, a CTA for a slice of the vocabulary that counts, changes the touched logits in shared memory and masks them on their way out: 23 us for
+// 64 rows of 151936 with all rules, 91 for 512 rows of trees.  Its loads were in flight for a fraction of its time.)
 // ---------------------------------------------------------------------------
-constexpr int AL_THREADS = 512;
-constexpr int AL_SLICE = 8192;                       // tokens of the vocabulary per CTA
-constexpr int AL_WORDS = AL_SLICE / 32 + 1;          // bitmaps, with a word past the end for reads across words
-constexpr uint32_t AL_PROMPT = 0x80000000u;          // in a count: the token occurs in the prompt
+constexpr int ML_THREADS = 256, ML_CTAS_PER_SM = 4, ML_UNROLL = 4;
+constexpr int RL_THREADS = 512, RL_TOKENS = 16384;  // of one CTA, at most
+constexpr int RL_ROWS = 4;
+// a token's word: how often it occurs in the output, the last place of its id in the request's list of biases (from 1), whether the prompt has it
+constexpr int AL_COUNT_BITS = 19, AL_BIAS_BITS = 12;
+constexpr uint32_t AL_COUNT = (1u << AL_COUNT_BITS) - 1, AL_PROMPT = 0x80000000u;
+static_assert(AL_COUNT_BITS + AL_BIAS_BITS == 31, "a word");
 
 struct LogitArgs {
   const void* logits;
   void* out;
   int64_t ld, ld_out;
-  int rows, vocab, n_seqs, rows_per_cta;
+  int rows, vocab, n_seqs;
   const int32_t* cu;  // null: row i is request i
   const int64_t* history;
   int64_t history_stride;
@@ -48,169 +59,255 @@ struct LogitArgs {
   const int64_t *drafts, *tree_mask;
   int64_t mask_stride;
   int words;
+  // rules_kernel: 2^part_bits CTAs share a request's tokens, as many times `splits` for parts of its rows; after the first kernel
+  int part_bits, splits, second;
 };
 
 template <class T>
 struct Logit;
 template <>
 struct Logit<uint16_t> {
-  static constexpr uint16_t kMinusInf = 0xff80;
+  static constexpr uint32_t kMinusInf = 0xff80ff80u;  // as many as a word holds
   static __device__ __forceinline__ float widen(uint16_t x) { return __uint_as_float(static_cast<uint32_t>(x) << 16); }
   static __device__ __forceinline__ uint16_t narrow(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
+  // ones in the halves whose bit is set: the bits as the signs of two bytes, which a permutation spreads
+  static __device__ __forceinline__ uint32_t keep(uint32_t bits) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(r) : "r"((bits & 3) * 0x4080u));
+    return r;
+  }
 };
 template <>
 struct Logit<uint32_t> {
   static constexpr uint32_t kMinusInf = 0xff800000u;
   static __device__ __forceinline__ float widen(uint32_t x) { return __uint_as_float(x); }
   static __device__ __forceinline__ uint32_t narrow(float x) { return __float_as_uint(x); }
+  static __device__ __forceinline__ uint32_t keep(uint32_t bits) { return 0u - (bits & 1); }
 };
 
-// n <= 8 bits of a bitmap from bit i on
-__device__ __forceinline__ uint32_t bits_at(const uint32_t* map, int i, int n) {
-  return __funnelshift_r(map[i >> 5], map[(i >> 5) + 1], i & 31) & ((1u << n) - 1);
-}
-
 template <class T>
-__global__ void __launch_bounds__(AL_THREADS) adjust_logits_kernel(const LogitArgs a) {
-  extern __shared__ uint32_t s_counts[];  // [AL_SLICE], then the same of places in the request's list of biases, from 1
-  uint32_t* const s_bias = s_counts + AL_SLICE;
-  __shared__ uint32_t s_touched[AL_WORDS], s_allowed[AL_WORDS];
-  constexpr int V = 16 / sizeof(T), PER = AL_SLICE / (V * AL_THREADS);
-  const int tid = threadIdx.x, v0 = blockIdx.x * AL_SLICE, len = min(AL_SLICE, a.vocab - v0);
-  b2::pdl_launch_dependents();
+__global__ void __launch_bounds__(ML_THREADS, ML_CTAS_PER_SM) mask_logits_kernel(const LogitArgs a) {
+  constexpr int V = 16 / sizeof(T), CHUNK = 32 * V, PAIR = 4 / sizeof(T);
   b2::pdl_wait();
-
-  int seq = -1, node0 = 0, nodes = 0;
-  float repetition = 1.f, presence = 0.f, frequency = 0.f;
-  const int row0 = blockIdx.y * a.rows_per_cta, row1 = min(a.rows, row0 + a.rows_per_cta);
-  for (int row = row0; row < row1; ++row) {
-    const T* in = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.ld + v0;
-    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.ld_out + v0;
-    // 16-byte vectors where both rows allow them, the elements before and behind one by one
+  b2::pdl_launch_dependents();  // (only now: the next kernel reads the inputs ahead of its own wait)
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (ML_THREADS / 32);
+  const int ruled = a.cu != nullptr ? __ldg(a.cu + a.n_seqs) : a.rows;  // rows behind the last request are copied
+  const int chunks = (a.vocab + CHUNK - 1) / CHUNK, per_row = (chunks + ML_UNROLL - 1) / ML_UNROLL;
+  // a warp takes ML_UNROLL chunks of a row at a time: 32 vectors where the chunk is whole and both rows have their 16-byte boundaries in common,
+  // but for the elements before the first boundary and behind the last, which go one by one, as all do otherwise
+  int64_t unit = blockIdx.x * (ML_THREADS / 32) + (threadIdx.x >> 5);
+  int row = static_cast<int>(unit / per_row), at = static_cast<int>(unit - static_cast<int64_t>(row) * per_row);
+  const int step_rows = warps / per_row, step_at = warps - step_rows * per_row;
+  while (row < a.rows) {
+    const T* const in = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.ld;
+    T* const out = static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.ld_out;
+    const uint8_t* const bits = reinterpret_cast<const uint8_t*>(a.allowed + static_cast<int64_t>(row) * a.allowed_stride);
+    const bool masked = a.allowed != nullptr && row < ruled;
     const bool same = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    const int head = same ? min(len, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / static_cast<int>(sizeof(T))) : len;
-    const int vectors = (len - head) / V;
-    uint4 x[PER];
+    const int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / static_cast<int>(sizeof(T));
+    auto element = [&](int t) { out[t] = !masked || ((__ldg(bits + (t >> 3)) >> (t & 7)) & 1) ? in[t] : static_cast<T>(Logit<T>::kMinusInf); };
+    auto word = [&](uint32_t w, uint32_t b) {
+      const uint32_t keep = Logit<T>::keep(b);
+      return (w & keep) | (Logit<T>::kMinusInf & ~keep);
+    };
+    const int t0 = at * ML_UNROLL * CHUNK;
+    if (same && t0 + ML_UNROLL * CHUNK <= a.vocab) {
+      uint4 x[ML_UNROLL];
+      uint32_t yes[ML_UNROLL];
+      const bool vector = head == 0 || lane < 31;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (i * AL_THREADS + tid < vectors) x[i] = *reinterpret_cast<const uint4*>(in + head + (i * AL_THREADS + tid) * V);
-
-    // ---- the row's request ----
-    int s = row;
-    if (a.cu != nullptr) {
-      int lo = 0, hi = a.n_seqs;  // the first request whose rows end behind this one
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(a.cu + mid + 1) > row) hi = mid;
-        else lo = mid + 1;
-      }
-      s = lo;
-    }
-    const bool ruled = s < a.n_seqs;  // rows behind the last request are copied
-    __syncthreads();                  // (the row before is done with the shared arrays)
-    if (ruled && s != seq) {
-      for (int i = tid; i < AL_SLICE; i += AL_THREADS) {
-        s_counts[i] = 0;
-        if (a.n_bias > 0) s_bias[i] = 0;
-      }
-      for (int i = tid; i < AL_WORDS; i += AL_THREADS) s_touched[i] = 0;
-      __syncthreads();
-      if (a.history != nullptr) {
-        const int64_t* text = a.history + static_cast<int64_t>(s) * a.history_stride;
-        const int n = max(0, min(__ldg(a.history_lens + s), a.history_width)), prompt = a.prompt_lens != nullptr ? __ldg(a.prompt_lens + s) : 0;
-        for (int i = tid; i < n; i += AL_THREADS) {
-          const int64_t e = __ldg(reinterpret_cast<const long long*>(text) + i) - v0;
-          if (e < 0 || e >= len) continue;
-          if (i < prompt) atomicOr(s_counts + e, AL_PROMPT);
-          else atomicAdd(s_counts + e, 1u);
-          atomicOr(s_touched + (e >> 5), 1u << (e & 31));
+      for (int i = 0; i < ML_UNROLL; ++i) {
+        const int t = t0 + i * CHUNK + head + lane * V;
+        if (vector) {
+          x[i] = *reinterpret_cast<const uint4*>(in + t);
+          if (masked) {
+            yes[i] = __ldg(bits + (t >> 3)) >> (t & 7);
+            if ((t & 7) + V > 8) yes[i] |= static_cast<uint32_t>(__ldg(bits + (t >> 3) + 1)) << (8 - (t & 7));
+          }
         }
       }
-      for (int i = tid; i < a.n_bias; i += AL_THREADS) {
-        const int64_t e = __ldg(reinterpret_cast<const long long*>(a.bias_ids) + s * a.bias_stride + i) - v0;
-        if (e < 0 || e >= len) continue;
-        atomicMax(s_bias + e, static_cast<uint32_t>(i + 1));
-        atomicOr(s_touched + (e >> 5), 1u << (e & 31));
-      }
-      seq = s;
-      repetition = a.repetition != nullptr ? __ldg(a.repetition + s) : 1.f;
-      presence = a.presence != nullptr ? __ldg(a.presence + s) : 0.f;
-      frequency = a.frequency != nullptr ? __ldg(a.frequency + s) : 0.f;
-      if (a.cu != nullptr) {
-        node0 = max(0, __ldg(a.cu + s));
-        nodes = min(min(a.rows, __ldg(a.cu + s + 1)) - node0, 64 * a.words);
-      }
-    }
-    // the drafted tokens that this row's node sees, as output; afterwards they are taken out again
-    auto path = [&](int sign) {
-      if (!ruled || a.drafts == nullptr) return;
-      for (int k = tid; k < nodes; k += AL_THREADS) {
-        if (!((__ldg(reinterpret_cast<const unsigned long long*>(a.tree_mask + static_cast<int64_t>(row) * a.mask_stride + (k >> 6))) >> (k & 63)) & 1)) continue;
-        const int64_t e = __ldg(reinterpret_cast<const long long*>(a.drafts) + node0 + k) - v0;
-        if (e < 0 || e >= len) continue;
-        atomicAdd(s_counts + e, static_cast<uint32_t>(sign));
-        if (sign > 0) atomicOr(s_touched + (e >> 5), 1u << (e & 31));  // (a mark that stays costs the next row a look at a count of zero)
-      }
-    };
-    path(1);
-    if (a.allowed != nullptr)
-      for (int i = tid; i < (len + 31) / 32; i += AL_THREADS) s_allowed[i] = __ldg(a.allowed + static_cast<int64_t>(row) * a.allowed_stride + v0 / 32 + i);
-    __syncthreads();
-
-    // ---- the slice ----
-    auto rule = [&](T raw, int e) -> T {
-      if (a.allowed != nullptr && !((s_allowed[e >> 5] >> (e & 31)) & 1)) return Logit<T>::kMinusInf;
-      if (!((s_touched[e >> 5] >> (e & 31)) & 1)) return raw;
-      const uint32_t c = s_counts[e], count = c & ~AL_PROMPT;
-      float x = Logit<T>::widen(raw);
-      if (c != 0 && a.repetition != nullptr) x = x > 0.f ? __fdiv_rn(x, repetition) : x * repetition;
-      if (count != 0) {
-        x = __fsub_rn(x, __fmul_rn(frequency, static_cast<float>(count)));
-        x = __fsub_rn(x, presence);
-      }
-      if (a.n_bias > 0) {
-        const uint32_t i = s_bias[e];
-        if (i != 0) x += __ldg(a.bias_values + s * a.bias_value_stride + i - 1);
-      }
-      return Logit<T>::narrow(x);
-    };
-    auto element = [&](int e) { out[e] = ruled ? rule(in[e], e) : in[e]; };
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int k = i * AL_THREADS + tid;
-      if (k >= vectors) break;
-      const int e0 = head + k * V;
-      constexpr uint32_t all = (1u << V) - 1;
-      uint32_t special = ruled ? bits_at(s_touched, e0, V) : 0u;
-      if (ruled && a.allowed != nullptr) special |= bits_at(s_allowed, e0, V) ^ all;
-      if (special != 0) {
-        T* const raw = reinterpret_cast<T*>(&x[i]);
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if ((special >> e) & 1) raw[e] = rule(raw[e], e0 + e);
+      for (int i = 0; i < ML_UNROLL; ++i) {
+        const int t = t0 + i * CHUNK;
+        if (masked) x[i] = make_uint4(word(x[i].x, yes[i]), word(x[i].y, yes[i] >> PAIR), word(x[i].z, yes[i] >> 2 * PAIR), word(x[i].w, yes[i] >> 3 * PAIR));
+        if (vector) *reinterpret_cast<uint4*>(out + t + head + lane * V) = x[i];
+        if (head > 0 && lane < V) element(lane < head ? t + lane : t + CHUNK - V + lane);
       }
-      *reinterpret_cast<uint4*>(out + e0) = x[i];
+    } else {
+#pragma unroll 4
+      for (int t = t0 + lane; t < min(t0 + ML_UNROLL * CHUNK, a.vocab); t += 32) element(t);
     }
-    for (int e = tid; e < head; e += AL_THREADS) element(e);
-    for (int e = head + vectors * V + tid; e < len; e += AL_THREADS) element(e);
-    if (row + 1 < row1 && ruled && a.drafts != nullptr) {
-      __syncthreads();
-      path(-1);
+    row += step_rows;
+    at += step_at;
+    if (at >= per_row) {
+      at -= per_row;
+      ++row;
     }
   }
 }
 
-size_t adjust_smem(int n_bias) { return static_cast<size_t>(n_bias > 0 ? 2 : 1) * AL_SLICE * sizeof(uint32_t); }
+// shared memory: words of the tokens, the marks of RL_ROWS rows, the list
+__host__ __device__ constexpr int rules_tokens(int vocab, int part_bits) { return ((vocab - 1) >> part_bits) + 1; }
+constexpr size_t rules_smem(int tokens) { return static_cast<size_t>((tokens + 3) / 4 * 4) * 4 + static_cast<size_t>(RL_ROWS) * ((tokens + 31) / 32) * 4 + static_cast<size_t>(tokens) * 2; }
 
-int configure_once() {
-  static std::atomic<bool> done[64];
+template <class T>
+__global__ void __launch_bounds__(RL_THREADS) rules_kernel(const LogitArgs a) {
+  extern __shared__ __align__(16) uint32_t s_words[];
+  __shared__ int s_listed;
+  const int tokens = rules_tokens(a.vocab, a.part_bits), padded = (tokens + 3) / 4 * 4, mark_words = (tokens + 31) / 32;
+  uint32_t* const s_marks = s_words + padded;
+  uint16_t* const s_list = reinterpret_cast<uint16_t*>(s_marks + RL_ROWS * mark_words);
+  const int tid = threadIdx.x;
+  const uint32_t part = blockIdx.x & ((1u << a.part_bits) - 1);
+  const int s = static_cast<int>((blockIdx.x >> a.part_bits) / a.splits), split = static_cast<int>((blockIdx.x >> a.part_bits) - s * a.splits);
+  b2::pdl_launch_dependents();
+  if (!a.second) b2::pdl_wait();
+
+  for (int i = tid; i < padded / 4; i += RL_THREADS) reinterpret_cast<uint4*>(s_words)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < RL_ROWS * mark_words; i += RL_THREADS) s_marks[i] = 0;
+  if (tid == 0) s_listed = 0;
+  // the request's rows, and this CTA's
+  const int node0 = a.cu != nullptr ? max(0, __ldg(a.cu + s)) : s, end = a.cu != nullptr ? min(a.rows, __ldg(a.cu + s + 1)) : s + 1;
+  const int per = (max(0, end - node0) + a.splits - 1) / a.splits, row0 = node0 + split * per, row1 = min(end, row0 + per);
+  const int nodes = a.drafts != nullptr ? min(end - node0, 64 * a.words) : 0;
+  if (row0 >= row1) {
+    if (a.second) b2::pdl_wait();  // (this kernel must not be over before the first one is: what follows waits for this one)
+    return;
+  }
+  // a token's place among this CTA's, or -1, and back
+  auto place_of = [&](int lo, int hi) {
+    return hi == 0 && static_cast<uint32_t>(lo) < static_cast<uint32_t>(a.vocab) && (lo & ((1u << a.part_bits) - 1)) == part ? lo >> a.part_bits : -1;
+  };
+  auto token_at = [&](int e) { return (e << a.part_bits) + static_cast<int>(part); };
+  auto id = [&](const int64_t* ids, int64_t i) {
+    const int2 t = __ldg(reinterpret_cast<const int2*>(ids) + i);
+    return place_of(t.x, t.y);
+  };
+  // adds a token to the list whose word was zero
+  auto list = [&](uint32_t before, int e) {
+    if (before == 0) s_list[atomicAdd(&s_listed, 1)] = static_cast<uint16_t>(e);
+  };
+  const int64_t* const text = a.history + static_cast<int64_t>(s) * a.history_stride;
+  const int n = a.history != nullptr ? max(0, min(__ldg(a.history_lens + s), a.history_width)) : 0, prompt = a.prompt_lens != nullptr ? __ldg(a.prompt_lens + s) : 0;
+  const float repetition = a.repetition != nullptr ? __ldg(a.repetition + s) : 1.f, presence = a.presence != nullptr ? __ldg(a.presence + s) : 0.f,
+              frequency = a.frequency != nullptr ? __ldg(a.frequency + s) : 0.f;
+  __syncthreads();
+  if (a.n_bias > 0) {
+    for (int i = tid; i < a.n_bias; i += RL_THREADS) {
+      const int e = id(a.bias_ids, s * a.bias_stride + i);
+      if (e >= 0) list(atomicMax(s_words + e, static_cast<uint32_t>(i + 1) << AL_COUNT_BITS), e);
+    }
+    __syncthreads();  // (places first: counts and prompt bits are added to words that hold them)
+  }
+  auto count = [&](int e, int i) {
+    if (e >= 0) list(i < prompt ? atomicOr(s_words + e, AL_PROMPT) : atomicAdd(s_words + e, 1u), e);
+  };
+  // two tokens a load, eight loads on their way at once; the first where it is not on a 16-byte boundary, and an odd last one
+  const int skip = n > 0 && (reinterpret_cast<uintptr_t>(text) & 15) != 0 ? 1 : 0, pairs = (n - skip) >> 1;
+  const int4* const two = reinterpret_cast<const int4*>(text + skip);
+  for (int p0 = tid; p0 < pairs; p0 += 8 * RL_THREADS) {
+    int4 t[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = p0 + k * RL_THREADS < pairs ? __ldg(two + p0 + k * RL_THREADS) : make_int4(-1, -1, -1, -1);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = skip + 2 * (p0 + k * RL_THREADS);
+      count(place_of(t[k].x, t[k].y), i);
+      count(place_of(t[k].z, t[k].w), i + 1);
+    }
+  }
+  if (skip && tid == 0) count(id(text, 0), 0);
+  if (((n - skip) & 1) && tid == 32) count(id(text, n - 1), n - 1);
+  __syncthreads();
+  const int listed = s_listed;
+  if (a.second) b2::pdl_wait();
+
+  // Where out is the logits, a logit that is read here is what it was, or masked, as it then is in the end.
+  auto in_row = [&](int row) { return static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.ld; };
+  auto out_row = [&](int row) { return static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.ld_out; };
+  auto permitted = [&](int row, int t) { return a.allowed == nullptr || ((__ldg(a.allowed + static_cast<int64_t>(row) * a.allowed_stride + (t >> 5)) >> (t & 31)) & 1); };
+  auto bias_of = [&](uint32_t w) {
+    const uint32_t place = (w & ~AL_PROMPT) >> AL_COUNT_BITS;
+    return place != 0 ? __ldg(a.bias_values + s * a.bias_value_stride + place - 1) : 0.f;
+  };
+  auto value = [&](T raw, bool yes, uint32_t w, uint32_t more, float bias) {
+    const uint32_t count = (w & AL_COUNT) + more;
+    float y = Logit<T>::widen(raw);
+    if ((count != 0 || (w & AL_PROMPT)) && a.repetition != nullptr) y = y > 0.f ? __fdiv_rn(y, repetition) : y * repetition;
+    if (count != 0) {
+      y = __fsub_rn(y, __fmul_rn(frequency, static_cast<float>(count)));
+      y = __fsub_rn(y, presence);
+    }
+    if ((w & ~AL_PROMPT) >> AL_COUNT_BITS) y += bias;
+    return yes ? Logit<T>::narrow(y) : static_cast<T>(Logit<T>::kMinusInf);
+  };
+  auto path = [&](int row) { return reinterpret_cast<const unsigned long long*>(a.tree_mask + static_cast<int64_t>(row) * a.mask_stride); };
+  auto on_path = [&](int row, int k) { return (__ldg(path(row) + (k >> 6)) >> (k & 63)) & 1 ? id(a.drafts, node0 + k) : -1; };
+  for (int r0 = row0; r0 < row1; r0 += RL_ROWS) {
+    const int here = min(RL_ROWS, row1 - r0);
+    if (nodes > 0) {
+      for (int i = tid; i < here * nodes; i += RL_THREADS) {
+        const int e = on_path(r0 + i / nodes, i % nodes);
+        if (e >= 0) atomicOr(s_marks + i / nodes * mark_words + (e >> 5), 1u << (e & 31));
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < listed; i += RL_THREADS) {
+      const int e = s_list[i], t = token_at(e);
+      const uint32_t w = s_words[e];
+      T raw[RL_ROWS];
+      bool yes[RL_ROWS];
+#pragma unroll
+      for (int r = 0; r < RL_ROWS; ++r)
+        if (r < here) {
+          raw[r] = in_row(r0 + r)[t];
+          yes[r] = permitted(r0 + r, t);
+        }
+      const float bias = bias_of(w);
+#pragma unroll
+      for (int r = 0; r < RL_ROWS; ++r)
+        if (r < here && !((s_marks[r * mark_words + (e >> 5)] >> (e & 31)) & 1)) out_row(r0 + r)[t] = value(raw[r], yes[r], w, 0, bias);
+    }
+    if (nodes > 0) {
+      for (int i = tid; i < here * nodes; i += RL_THREADS) {
+        const int row = r0 + i / nodes, k = i % nodes, e = on_path(row, k);
+        if (e < 0) continue;
+        uint32_t times = 0;
+        bool first = true;
+        for (int j0 = 0; j0 < nodes; j0 += 64)
+          for (uint64_t bits = __ldg(path(row) + (j0 >> 6)); bits != 0; bits &= bits - 1) {
+            const int j = j0 + __ffsll(bits) - 1;
+            if (j >= nodes) break;
+            if (id(a.drafts, node0 + j) != e) continue;
+            ++times;
+            first = first && j >= k;
+          }
+        if (!first) continue;
+        const int t = token_at(e);
+        const uint32_t w = s_words[e];
+        out_row(row)[t] = value(in_row(row)[t], permitted(row, t), w, times, bias_of(w));
+      }
+      if (r0 + RL_ROWS < row1) {
+        __syncthreads();
+        for (int i = tid; i < RL_ROWS * mark_words; i += RL_THREADS) s_marks[i] = 0;
+        __syncthreads();
+      }
+    }
+  }
+}
+
+// sms: the device's
+int configure_once(int* sms) {
+  static std::atomic<int> done[64];
   int dev = 0;
   B2_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return b2::set_error(B2_ERR_UNSUPPORTED, "device ordinal %d not supported", dev);
-  if (!done[dev].load(std::memory_order_acquire)) {
-    B2_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, adjust_smem(1)));
-    B2_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<uint32_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, adjust_smem(1)));
-    done[dev].store(true, std::memory_order_release);
+  *sms = done[dev].load(std::memory_order_acquire);
+  if (*sms == 0) {
+    B2_CUDA(cudaFuncSetAttribute(rules_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, rules_smem(RL_TOKENS)));
+    B2_CUDA(cudaFuncSetAttribute(rules_kernel<uint32_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, rules_smem(RL_TOKENS)));
+    B2_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    done[dev].store(*sms, std::memory_order_release);
   }
   return B2_OK;
 }
@@ -226,8 +323,11 @@ extern "C" int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64
   if (r->history != nullptr && (r->history_width < 0 || r->history_lens == nullptr)) return B2_ERR_ARG;
   if (r->n_bias < 0 || (r->n_bias > 0 && (!r->bias_ids || !r->bias_values))) return B2_ERR_ARG;
   if (r->allowed_mask != nullptr && r->allowed_stride < (vocab + 31) / 32) return B2_ERR_ARG;
-  if (r->draft_tokens != nullptr && (!r->tree_mask || !r->cu_seqlens || r->mask_words <= 0 || r->mask_stride < r->mask_words || r->mask_words > 1 << 20)) return B2_ERR_ARG;
-  const int rc = configure_once();
+  if (r->draft_tokens != nullptr && (!r->tree_mask || !r->cu_seqlens || r->mask_words <= 0 || r->mask_stride < r->mask_words || r->mask_words > 1 << 12)) return B2_ERR_ARG;
+  if (r->n_bias >= 1 << AL_BIAS_BITS || (r->history != nullptr ? r->history_width : 0) + 64ll * (r->draft_tokens != nullptr ? r->mask_words : 0) > AL_COUNT)
+    return b2::set_error(B2_ERR_SHAPE, "at most %d biases, and %d tokens of history and path", (1 << AL_BIAS_BITS) - 1, AL_COUNT);
+  int sms = 0;
+  const int rc = configure_once(&sms);
   if (rc != B2_OK) return rc;
   LogitArgs a{};
   a.logits = logits;
@@ -257,12 +357,22 @@ extern "C" int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64
   a.tree_mask = r->tree_mask;
   a.mask_stride = r->mask_stride;
   a.words = r->mask_words;
-  // rows of one request share the counts of its history: as many to a CTA as leave four CTAs for every SM
-  const int slices = (vocab + AL_SLICE - 1) / AL_SLICE;
-  a.rows_per_cta = r->cu_seqlens == nullptr ? 1 : std::max(1, static_cast<int>(static_cast<int64_t>(rows) * slices / (4 * 148)));
-  a.rows_per_cta = std::max(a.rows_per_cta, (rows + 65534) / 65535);
-  const dim3 grid(slices, (rows + a.rows_per_cta - 1) / a.rows_per_cta);
-  const auto kernel = fp32 ? adjust_logits_kernel<uint32_t> : adjust_logits_kernel<uint16_t>;
-  B2_CUDA(b2_launch(kernel, grid, dim3(AL_THREADS), adjust_smem(r->n_bias), static_cast<cudaStream_t>(stream), a));
+  const cudaStream_t on = static_cast<cudaStream_t>(stream);
+  if (logits != out || a.allowed != nullptr) {
+    const int64_t chunks = (static_cast<int64_t>(vocab) + (fp32 ? 128 : 256) * ML_UNROLL - 1) / ((fp32 ? 128 : 256) * ML_UNROLL);
+    const int64_t blocks = (chunks * rows + ML_THREADS / 32 - 1) / (ML_THREADS / 32);
+    const auto kernel = fp32 ? mask_logits_kernel<uint32_t> : mask_logits_kernel<uint16_t>;
+    B2_CUDA(b2_launch(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(blocks, static_cast<int64_t>(sms) * ML_CTAS_PER_SM))), dim3(ML_THREADS), 0, on, a));
+    a.second = 1;
+  }
+  if ((a.history != nullptr || a.n_bias > 0 || a.drafts != nullptr) && a.n_seqs > 0) {
+    while (rules_tokens(vocab, a.part_bits) > RL_TOKENS) ++a.part_bits;
+    // a request's rows in so many parts that there are two CTAs for every SM, but no fewer than RL_ROWS of them to a CTA
+    const int64_t items = static_cast<int64_t>(a.n_seqs) << a.part_bits;
+    a.splits = a.cu == nullptr ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((2 * sms + items - 1) / items, (rows / a.n_seqs + RL_ROWS - 1) / RL_ROWS)));
+    if (items * a.splits >= 1ll << 31) return b2::set_error(B2_ERR_SHAPE, "%d requests over %d tokens", a.n_seqs, vocab);
+    const auto kernel = fp32 ? rules_kernel<uint32_t> : rules_kernel<uint16_t>;
+    B2_CUDA(b2_launch(kernel, dim3(static_cast<unsigned>(items * a.splits)), dim3(RL_THREADS), rules_smem(rules_tokens(vocab, a.part_bits)), on, a));
+  }
   return B2_OK;
 }

@@ -623,7 +623,6 @@ PyObject* adjust_logits(Args a) {
     }
   if (t[1].defined()) {
     row_matrix(t[1], at::kLong, n, 0, names[1]);
-    if (t[1].size(1) > 1 << 30) raise(PyExc_ValueError, "history: rows of %lld", (long long)t[1].size(1));
     vector_of(t[2], at::kInt, n, names[2]);
     if (t[3].defined()) vector_of(t[3], at::kInt, n, names[3]);
     r.history = cptr<int64_t>(t[1]);
@@ -632,6 +631,8 @@ PyObject* adjust_logits(Args a) {
     r.history_lens = cptr<int32_t>(t[2]);
     r.prompt_lens = cptr<int32_t>(t[3]);
   }
+  if ((t[1].defined() ? t[1].size(1) : 0) + 64 * (t[11].defined() && t[12].dim() == 2 ? t[12].size(1) : 0) >= 1 << 19)
+    raise(PyExc_ValueError, "history of %lld tokens: with the path less than 2^19", (long long)(t[1].defined() ? t[1].size(1) : 0));
   r.repetition_penalty = cptr<float>(t[4]);
   r.presence_penalty = cptr<float>(t[5]);
   r.frequency_penalty = cptr<float>(t[6]);
@@ -639,7 +640,7 @@ PyObject* adjust_logits(Args a) {
   if (t[7].defined()) {
     row_matrix(t[7], at::kLong, n, 0, names[7]);
     row_matrix(t[8], at::kFloat, n, 0, names[8]);
-    if (t[7].size(1) != t[8].size(1) || t[7].size(1) > 1 << 30) raise(PyExc_ValueError, "bias_ids: %lld a request, bias_values %lld", (long long)t[7].size(1), (long long)t[8].size(1));
+    if (t[7].size(1) != t[8].size(1) || t[7].size(1) > 4095) raise(PyExc_ValueError, "bias_ids: %lld a request, bias_values %lld: as many, at most 4095", (long long)t[7].size(1), (long long)t[8].size(1));
     r.bias_ids = cptr<int64_t>(t[7]);
     r.bias_stride = row_stride(t[7]);
     r.n_bias = t[7].size(1);
@@ -655,7 +656,7 @@ PyObject* adjust_logits(Args a) {
   if (t[11].defined()) {
     vector_of(t[11], at::kLong, rows, names[11]);
     row_matrix(t[12], at::kLong, rows, rows > 0 ? 1 : 0, names[12]);
-    if (t[12].size(1) > 1 << 20) raise(PyExc_ValueError, "tree_mask: rows of %lld words", (long long)t[12].size(1));
+    if (t[12].size(1) > 1 << 12) raise(PyExc_ValueError, "tree_mask: rows of %lld words", (long long)t[12].size(1));
     r.draft_tokens = cptr<int64_t>(t[11]);
     r.tree_mask = cptr<int64_t>(t[12]);
     r.mask_stride = row_stride(t[12]);

@@ -127,6 +127,33 @@ def test_trees(ops, dtype):
     got = ops.adjust_logits(logits.to(DEV), **on_gpu(a))
     check(got, logits, a)
     assert torch.equal(got[-3:].cpu(), logits[-3:])  # rows behind the last request
+    x = logits.to(DEV)
+    ops.adjust_logits(x, **on_gpu(a), out=x)
+    assert torch.equal(x, got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_several_rows_of_a_request_without_drafts(ops, dtype):
+    counts = [5, 0, 70, 1, 12]
+    rows = sum(counts) + 3
+    logits, a = request(5, 9000, rows, seed=16, dtype=dtype)
+    a["cu_seqlens"] = ref.cumulative(counts)
+    check(ops.adjust_logits(logits.to(DEV), **on_gpu(a)), logits, a)
+
+
+def test_trees_over_several_slices_between_rows_without_a_path(ops):
+    """Rows with and without a path by turns, an odd number of them, more steps than CTAs."""
+    counts = [1, 2, 0, 3, 5, 1, 1]
+    rows = sum(counts)
+    logits, a = request(7, 60001, rows, seed=18, dtype=torch.bfloat16)
+    logits, a["allowed_mask"] = logits.repeat(40, 1), a["allowed_mask"].repeat(40, 1)
+    a = {k: v if k == "allowed_mask" else v.repeat(40, *[1] * (v.dim() - 1)) for k, v in a.items()}
+    a["cu_seqlens"] = ref.cumulative(counts * 40)
+    a["draft_tokens"] = torch.randint(0, 40, (rows * 40,), generator=torch.Generator().manual_seed(18))
+    a["tree_mask"] = ref.trees(counts * 40, 1, 18)
+    a["tree_mask"][::3] = 0
+    got = ops.adjust_logits(logits.to(DEV), **on_gpu(a))
+    check(got, logits, a)
 
 
 def test_trees_without_a_history(ops):
@@ -149,6 +176,30 @@ def test_many_rows_of_a_request(ops):
     a["draft_tokens"] = torch.randint(0, 40, (rows,), generator=torch.Generator().manual_seed(8))
     a["tree_mask"] = ref.trees(counts, 6, 8)
     check(ops.adjust_logits(logits.to(DEV), **on_gpu(a)), logits, a)
+
+
+def test_a_list_longer_than_a_block(ops):
+    """Every token of a slice in the history, and paths of more nodes than a block has threads."""
+    rows = 700
+    logits, a = request(1, 9000, rows, seed=17, history=9000, bias=40, dtype=torch.bfloat16)
+    a["history"][0] = torch.randperm(9000, generator=torch.Generator().manual_seed(17))
+    a["history_lens"][:], a["prompt_lens"][:] = 9000, 4000
+    a["cu_seqlens"] = ref.cumulative([rows])
+    a["draft_tokens"] = torch.randint(0, 200, (rows,), generator=torch.Generator().manual_seed(17))
+    a["tree_mask"] = ref.masks([(2 << i) - 1 for i in range(rows)], 11)
+    keep = [0, 1, 300, 699]
+    b = on_gpu(a)
+    got = ops.adjust_logits(logits.to(DEV), **b)
+    x = logits.to(DEV)
+    ops.adjust_logits(x, **b, out=x)
+    assert torch.equal(x, got)
+    # (the definition a few rows at a time: a row's path as the end of a longer history)
+    for row in keep:
+        one = dict(a, history=torch.cat([a["history"], a["draft_tokens"][:row + 1].view(1, -1)], 1), history_lens=torch.tensor([9000 + row + 1], dtype=torch.int32),
+                   allowed_mask=a["allowed_mask"][row:row + 1])
+        for name in ("cu_seqlens", "draft_tokens", "tree_mask"):
+            del one[name]
+        check(got[row:row + 1], logits[row:row + 1], one, f"row {row}")
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
