@@ -225,7 +225,10 @@ extern "C" int b2_batch_inputs(int32_t* block_tables, int64_t bt_stride, int bt_
   if (rc != B2_OK) return rc;
   const BatchArgs a{block_tables, bt_stride, bt_width, cached_lens, seq_lens, n, free_blocks, free_capacity, num_free, block_size, num_slots, max_tokens,
                     tree_mask, mask_stride, mask_words, positions, slot_mapping, cu_seqlens_q, cu_seqlens_k, last_token_index, context_lens, num_free_out};
-  const int grid = std::max(1, std::min(148, (std::max(max_tokens, n) + BI_THREADS - 1) / BI_THREADS));
+  // a thread for each token, and for every fourth block that the tables have room for: how many of them move is known on the device only (512 rows of 257
+  // blocks, a tenth of which finish and give 6500 back: 10.6 us with a CTA for every 512 tokens, 6.3 so)
+  const int64_t work = std::max<int64_t>(max_tokens, static_cast<int64_t>(n) * bt_width / 4);
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(64, (work + BI_THREADS - 1) / BI_THREADS)));
   B2_CUDA(b2_launch(batch_inputs_kernel, dim3(grid), dim3(BI_THREADS), batch_smem(n), static_cast<cudaStream_t>(stream), a));
   return B2_OK;
 }

@@ -510,6 +510,14 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
   return a.numel() > 0 && b.numel() > 0 && reinterpret_cast<uintptr_t>(a.const_data_ptr()) < end(b) && reinterpret_cast<uintptr_t>(b.const_data_ptr()) < end(a);
 }
 
+// several vectors in one allocation: each of them keeps all of it alive
+at::Tensor vector_in(const at::Tensor& base, int64_t offset_bytes, int64_t size, at::ScalarType type) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(offset_bytes / static_cast<int64_t>(c10::elementSize(type)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
+  return t;
+}
+
 // batch_inputs(block_tables, cached_lens, seq_lens, free_blocks, num_free, block_size, num_slots, max_tokens, tree_mask):
 // (positions, slot_mapping, cu_seqlens_q, cu_seqlens_k, last_token_index, context_lens, num_free)
 PyObject* batch_inputs(Args a) {
@@ -541,8 +549,13 @@ PyObject* batch_inputs(Args a) {
   on_current_gpu(tables, "block_tables");
   for (const auto& t : named) beside(*t.first, tables, t.second);
   beside(mask, tables, "tree_mask");
-  auto empty = [&](int64_t size, at::ScalarType type) { return at::detail::empty_cuda({size}, type, tables.device(), std::nullopt); };
-  const at::Tensor out[7] = {empty(max_tokens, at::kLong), empty(max_tokens, at::kInt), empty(n + 1, at::kInt), empty(n + 1, at::kInt), empty(n, at::kInt), empty(n, at::kInt), empty(1, at::kInt)};
+  // (one allocation and not seven, each of which takes the host as long as the kernel's launch; every vector on 16 bytes)
+  const int64_t sizes[7] = {max_tokens, max_tokens, n + 1, n + 1, n, n, 1};
+  int64_t at[8] = {};
+  for (int i = 0; i < 7; ++i) at[i + 1] = at[i] + (sizes[i] * (i == 0 ? 8 : 4) + 15) / 16 * 16;
+  const at::Tensor base = at::detail::empty_cuda({at[7]}, at::kByte, tables.device(), std::nullopt);
+  at::Tensor out[7];
+  for (int i = 0; i < 7; ++i) out[i] = vector_in(base, at[i], sizes[i], i == 0 ? at::kLong : at::kInt);
   auto ints = [&](int i) { return out[i].mutable_data_ptr<int32_t>(); };
   launch("b2_batch_inputs", b2_batch_inputs, tables.mutable_data_ptr<int32_t>(), row_stride(tables), width, cached.const_data_ptr<int32_t>(), wanted.const_data_ptr<int32_t>(), n,
          free.mutable_data_ptr<int32_t>(), free.numel(), num_free.const_data_ptr<int32_t>(), bs, num_slots, max_tokens, mask.defined() ? mask.const_data_ptr<int64_t>() : nullptr,

@@ -32,7 +32,7 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int TR_ROWS = 128, TR_KEYS = 64, TR_THREADS = TR_ROWS + 64, TR_CTAS_PER_SM = 2, TR_COLUMNS = 256;
 constexpr int TR_MAX_SEQS = 1024;
-constexpr int TR_ITEM_UNITS = 2;
+constexpr int TR_ITEM_UNITS = 2, TR_WHOLE_TILES = 8;
 constexpr float TR_GROWTH = 8.f;
 constexpr uint64_t TR_LIMIT_NS = 1000000000ull;
 template <int HD>
@@ -61,6 +61,7 @@ struct TreeArgs {
   float scale_log2;  // size of softmax scale * log2(e)
   uint16_t* out;
   float* parts;      // [2][gridDim.y][gridDim.x] slots: [0] of the item that a range begins in, [1] of the one it ends in
+  bool whole;        // every (sequence, KV head) is one CTA's: there are no parts
   int4* joins;       // [gridDim.y][gridDim.x]: parts of the item that the range ends in (0: none), its first token, its nodes in the tile, its KV head
   B2Status* status;
 };
@@ -81,8 +82,10 @@ __device__ __forceinline__ int tiles_of(int len) { return (len + TR_KEYS - 1) / 
 // is walked several times (pass).  A segment may hold no tiles (t0 >= t1).
 struct TreeWalk {
   const int* first_unit_of;  // [n_seqs + 1] units per KV head before each sequence
-  int nkv, pos, end, b, head, pass, tiles, t0, t1;
-  __device__ __forceinline__ TreeWalk(const int* fu, int n_seqs, int heads, int begin, int stop) : first_unit_of(fu), nkv(heads), pos(begin), end(stop), b(0) {
+  int nkv, pos, end, jump, again, b, head, pass, tiles, t0, t1;
+  // again: so many further ranges of the same length, `jump` units behind the end of the one before
+  __device__ __forceinline__ TreeWalk(const int* fu, int n_seqs, int heads, int begin, int stop, int jump, int again)
+      : first_unit_of(fu), nkv(heads), pos(begin), end(stop), jump(jump), again(again), b(0) {
     int hi = n_seqs - 1;
     while (b < hi) {
       const int mid = (b + hi + 1) >> 1;
@@ -91,7 +94,12 @@ struct TreeWalk {
     }
   }
   __device__ __forceinline__ bool next(const TreeArgs& a, Sequence& s) {
-    if (pos >= end) return false;
+    if (pos >= end) {
+      if (--again < 0) return false;
+      const int units = tiles + TR_ITEM_UNITS;
+      pos += jump;
+      end = pos + units;
+    }
     while (first_unit_of[b + 1] * nkv <= pos) ++b;
     s = sequence(a, b);
     tiles = tiles_of(s.len);
@@ -224,9 +232,18 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   const int base = ctas > 0 ? total / ctas : 0, rem = ctas > 0 ? total % ctas : 0;
   auto begin_of = [&](int i) { return i * base + min(i, rem); };
   auto cta_of = [&](int t) { const int big = rem * (base + 1); return t < big ? t / (base + 1) : rem + (t - big) / base; };
-  const int begin = x < ctas ? begin_of(x) : 0, end = x < ctas ? begin_of(x + 1) : 0;
-  TreeWalk walk(first_unit, a.n_seqs, a.nkv, begin, end);
+  int begin = x < ctas ? begin_of(x) : 0, end = x < ctas ? begin_of(x + 1) : 0, jump = 0, again = 0;
   Sequence s;
+  if (a.whole) {  // CTA x is (sequence, KV head) x: one range, or one for each pass
+    const int b = x / a.nkv;
+    s = sequence(a, b);
+    const int units = tiles_of(s.len) + TR_ITEM_UNITS;
+    begin = first_unit[b] * a.nkv + (x - b * a.nkv) * units;
+    end = s.len > 0 ? begin + units : begin;
+    jump = (a.nkv - 1) * units;
+    again = (first_unit[b + 1] - first_unit[b]) / units - 1;
+  }
+  TreeWalk walk(first_unit, a.n_seqs, a.nkv, begin, end, jump, again);
   auto all_wait = [&](uint32_t bar, uint32_t phase, int code) {
     return __all_sync(0xffffffffu, b2::mbar_wait(bar, phase, abort_flag, TR_LIMIT_NS, code)) != 0;
   };
@@ -236,7 +253,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 
   if (begin >= end) {
     if (warp < 4) clear_rows();
-    if (threadIdx.x == 0) a.joins[y * X + x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0 && !a.whole) a.joins[y * X + x] = make_int4(0, 0, 0, 0);
   } else if (warp == 4) {
     // ---------------- TMA (the whole warp walks and one thread issues, here and in the next warp) ----------------
     bool ok = true;
@@ -411,15 +428,17 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           for (int e = 0; e < 64; e += 4)
 #pragma unroll
             for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(r[e >> 5][(e & 31) + k]));
-          // The reference m moves when a row of the warp is TR_GROWTH past it (or has seen its first key): O then has to be rescaled, which takes as long
-          // as half a tile.  Until then probabilities are up to 2^TR_GROWTH, which costs no bits: they are rounded relative to themselves.
+          // The reference m moves when the row is TR_GROWTH past it (or has seen its first key): O then has to be rescaled, which takes as long as
+          // half a tile.  Until then probabilities are up to 2^TR_GROWTH, which costs no bits: they are rounded relative to themselves.
+          // (Each row for itself: its result does not depend on the rows beside it.)
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          const bool grown = __any_sync(0xffffffffu, (top - m) * a.scale_log2 > TR_GROWTH);
-          const float f = grown && top > m ? b2::ex2((m - top) * a.scale_log2) : 1.f;
+          const bool grown = (top - m) * a.scale_log2 > TR_GROWTH;
+          const float f = grown ? b2::ex2((m - top) * a.scale_log2) : 1.f;
           if (grown) m = top;
           const float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
           const uint64_t ref2 = b2::pair_of(-ref, -ref);
-          if (grown) {
+          const bool any_grown = __any_sync(0xffffffffu, grown);
+          if (any_grown) {
             l[0] = b2::mul_pair(l[0], b2::pair_of(f, f));
             l[1] = b2::mul_pair(l[1], b2::pair_of(f, f));
           }
@@ -437,7 +456,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             }
             b2::tmem_st_32x16(t_s + h * 16, p);  // (this row has read its columns)
           }
-          if (j > 0 && grown) {
+          if (j > 0 && any_grown) {
             ok = all_wait(o_done + ((i - 1) & 1) * 8, ((i - 1) >> 1) & 1, B2_WAIT_TMEM_FULL);
             if (!ok) break;
             b2::tc_fence_after();
@@ -514,7 +533,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       }
       ++seg;
     }
-    if (threadIdx.x == 0) a.joins[y * X + x] = join;
+    if (threadIdx.x == 0 && !a.whole) a.joins[y * X + x] = join;
   }
 
   __syncwarp();
@@ -679,6 +698,7 @@ __global__ void __launch_bounds__(TC_WARPS * 32, TC_CTAS_PER_SM) tree_combine_ke
 // How a call is launched: ranges, tiles of rows walked side by side.
 struct TreePlan {
   int x, y, npt;
+  bool whole;
   int64_t slot_bytes, bytes;
 };
 TreePlan plan_tree(const b2_ctx* ctx, int n_seqs, int max_q, int group, int nkv, int head_dim, int64_t max_len) {
@@ -687,8 +707,11 @@ TreePlan plan_tree(const b2_ctx* ctx, int n_seqs, int max_q, int group, int nkv,
   p.y = std::max(1, std::min((max_q + p.npt - 1) / p.npt, 8));
   const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(n_seqs) * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS + TR_ITEM_UNITS) * ((max_q + p.npt * p.y - 1) / (p.npt * p.y)));
   p.x = static_cast<int>(std::min<int64_t>(most, std::max(1, ctx->num_sms * TR_CTAS_PER_SM / p.y)));
+  // Contexts of at most TR_WHOLE_TILES tiles are not cut where there are CTAs for all of them: the second kernel takes as long as walking so many.
+  p.whole = max_len <= TR_WHOLE_TILES * TR_KEYS && n_seqs > 0 && static_cast<int64_t>(n_seqs) * nkv * p.y <= ctx->num_sms * TR_CTAS_PER_SM;
+  if (p.whole) p.x = n_seqs * nkv;
   p.slot_bytes = static_cast<int64_t>(head_dim == 128 ? Tree<128>::SLOT : Tree<64>::SLOT) * sizeof(float);
-  p.bytes = static_cast<int64_t>(p.x) * p.y * (2 * p.slot_bytes + sizeof(int4));
+  p.bytes = p.whole ? 0 : static_cast<int64_t>(p.x) * p.y * (2 * p.slot_bytes + sizeof(int4));
   return p;
 }
 
@@ -725,7 +748,7 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
   if (ctx == nullptr || n_seqs < 0 || tokens < 0 || nq <= 0 || nkv <= 0 || max_q < 0) return B2_ERR_ARG;
   if (tokens == 0) return B2_OK;
   if (!b2_tree_attention_supported(nq, nkv, head_dim, block_size)) return B2_ERR_UNSUPPORTED;
-  if (!q || !k_cache || !v_cache || !cu_q || !out || !workspace || (n_seqs > 0 && (!block_tables || !context_lens || !tree_mask))) return B2_ERR_ARG;
+  if (!q || !k_cache || !v_cache || !cu_q || !out || (n_seqs > 0 && (!block_tables || !context_lens || !tree_mask))) return B2_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(out) |
        reinterpret_cast<uintptr_t>(workspace)) & 15)
     return B2_ERR_ARG;
@@ -739,7 +762,7 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
   const int64_t passes = (static_cast<int64_t>(tokens) + p.npt * p.y - 1) / (p.npt * p.y) + n_seqs;
   if (static_cast<int64_t>(num_blocks) * block_size >= 1ll << 31 || max_len >= 1ll << 31 || passes * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS + TR_ITEM_UNITS) >= 1ll << 31)
     return b2::set_error(B2_ERR_SHAPE, "%lld slots, tables of %lld tokens", static_cast<long long>(num_blocks) * block_size, static_cast<long long>(max_len));
-  if (workspace_bytes < p.bytes) return B2_ERR_ARG;
+  if (workspace_bytes < p.bytes || (p.bytes > 0 && workspace == nullptr)) return B2_ERR_ARG;
   const int rc = configure_once();
   if (rc != B2_OK) return rc;
   TreeArgs a{};
@@ -764,8 +787,9 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
   a.negate = scale < 0.f ? b2::kUmmaNegateA : 0u;
   a.scale_log2 = b2::scale_size(scale);
   a.out = static_cast<uint16_t*>(out);
+  a.whole = p.whole;
   a.parts = static_cast<float*>(workspace);
-  a.joins = reinterpret_cast<int4*>(static_cast<char*>(workspace) + 2 * p.x * p.y * p.slot_bytes);
+  a.joins = p.whole ? nullptr : reinterpret_cast<int4*>(static_cast<char*>(workspace) + 2 * p.x * p.y * p.slot_bytes);
   a.status = ctx->status_dev;
   CUtensorMap tmQ, tmK, tmV;
   const uint64_t width = static_cast<uint64_t>(nkv) * head_dim, slots = static_cast<uint64_t>(num_blocks) * block_size;
@@ -776,7 +800,8 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
   const size_t smem = head_dim == 128 ? Tree<128>::smem(n_seqs) : Tree<64>::smem(n_seqs);
   B2_CUDA(b2_launch(head_dim == 128 ? tree_attention_kernel<128> : tree_attention_kernel<64>, dim3(p.x, p.y), dim3(TR_THREADS), smem, on, tmQ, tmK, tmV, a));
-  B2_CUDA(b2_launch(head_dim == 128 ? tree_combine_kernel<128> : tree_combine_kernel<64>, dim3(TC_CTAS_PER_SM * ctx->num_sms), dim3(TC_WARPS * 32), 0, on, a, p.x, p.y));
+  if (!p.whole)
+    B2_CUDA(b2_launch(head_dim == 128 ? tree_combine_kernel<128> : tree_combine_kernel<64>, dim3(TC_CTAS_PER_SM * ctx->num_sms), dim3(TC_WARPS * 32), 0, on, a, p.x, p.y));
   return B2_OK;
 }
 

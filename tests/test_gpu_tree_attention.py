@@ -125,6 +125,23 @@ def test_large_trees_and_wide_masks(ops, nodes, words):
     Case([33, 0, 500], [nodes, 3, nodes // 2 + 1], nq=4, nkv=1, words=words, seed=nodes, reach=40).check(ops)
 
 
+@pytest.mark.parametrize("nq, nkv, hd", [(8, 2, 128), (20, 4, 64), (16, 1, 128)])
+def test_a_table_wider_than_the_contexts(ops, nq, nkv, hd):
+    """Short contexts are one CTA's each where the table says that they are short, and are cut where it leaves room for longer ones."""
+    c = Case([0, 60, 64, 301, 440, 3], [5, 64, 1, 20, 33, 7], nq, nkv, hd=hd, bs=16, seed=nq)
+    c.check(ops, "narrow")
+    c.tables = torch.cat([c.tables, torch.full((6, 500), -1, dtype=torch.int32, device=DEV)], 1)
+    c.check(ops, "wide")
+
+
+@pytest.mark.parametrize("max_q", [1, 9, 200])
+def test_many_nodes_of_short_contexts(ops, max_q):
+    """More nodes than the CTAs that walk side by side have rows for, whatever max_seqlen_q says."""
+    c = Case([10, 0, 64], [200, 9, 130], nq=16, nkv=2, seed=26, reach=30)
+    c.max_q = max_q
+    c.check(ops)
+
+
 def test_chains(ops):
     """Every node sees all nodes before it: what causal attention of the last tokens computes."""
     c = Case([300, 77], [64, 40], nq=8, nkv=2, seed=4)
