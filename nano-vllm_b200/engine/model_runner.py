@@ -16,6 +16,7 @@ import numpy as np
 import torch
 import torch.distributed as dist
 
+from .. import ops
 from ..layers.sampler import Sampler
 from ..models.qwen3 import Qwen3ForCausalLM
 from ..runtime import get_runtime, init_runtime, shutdown_runtime
@@ -319,12 +320,58 @@ class ModelRunner:
             if self.rank == 0:
                 picked = Sampler.greedy(logits) if temps is None else self.sampler(logits, temps)
         if self.world > 1:
-            from .. import ops
             ops.broadcast_tokens(picked)  # rank 0's choice reaches every rank on the device
         tokens = picked.tolist()  # the step's synchronisation point
         reset_context()
         self.runtime.check_status()
         return tokens
+
+    @torch.inference_mode()
+    def verify(self, seqs: list[Seq], drafts: list[list[int]], parents: list[list[int]], rules: dict[str, torch.Tensor] | None = None) -> list[list[int]]:
+        """One forward pass over a tree of drafted tokens per sequence (speculative decoding): node 0 is the sequence's last token, as in a
+        decode step, and drafts[i][j] is node j + 1, whose parent is node parents[i][j] <= j.  Returns the greedy pick after every node, on every rank.  The
+        block tables must have room for all nodes; keys and values of node j are left at place len(seq) - 1 + j.  rules: arguments of
+        ops.adjust_logits that belong to the sequences (histories end before the last token: node 0 counts as part of every path) or,
+        allowed_mask, to the nodes in their order."""
+        if not (len(seqs) == len(drafts) == len(parents)) or any(len(d) != len(p) for d, p in zip(drafts, parents)):
+            raise ValueError("a list of drafted tokens and of their parents for each sequence")
+        counts = [len(d) + 1 for d in drafts]
+        total, words = sum(counts), -(-max(counts, default=1) // 64)
+        if total > self.max_num_seqs:
+            raise ValueError(f"{total} nodes: at most max_num_seqs ({self.max_num_seqs}), the rows of the logits")
+        ids, mask, at = np.empty(total, dtype=np.int64), np.zeros((total, words), dtype=np.uint64), 0
+        for s, d, p in zip(seqs, drafts, parents):
+            ids[at:at + len(d) + 1] = [s.token_ids[-1], *d]
+            for j in range(len(d) + 1):
+                if j > 0:
+                    if not 0 <= p[j - 1] < j:
+                        raise ValueError(f"node {j}: parent {p[j - 1]}")
+                    mask[at + j] = mask[at + p[j - 1]]
+                mask[at + j, j // 64] |= np.uint64(1 << (j % 64))
+            at += len(d) + 1
+        cached = np.array([len(s) - 1 for s in seqs], dtype=np.int32)
+        wanted = cached + np.array(counts, dtype=np.int32)
+        if any(n > len(s.block_table) * self.block_size for s, n in zip(seqs, wanted)):
+            raise ValueError("the block tables have no room for the drafted tokens")
+        # the caller has dealt the blocks: the stack holds the ones that the nodes open, the first of them on top
+        opened = [b for s, c, n in zip(seqs, cached, wanted) for b in s.block_table[-(-c // self.block_size):-(-n // self.block_size)]]
+        ids_t, cached_t, wanted_t, tables_t, mask_t, stack_t, height_t = self._to_device(
+            ids, cached, wanted, self._block_tables(seqs), mask.view(np.int64), np.array(opened[::-1], dtype=np.int32), np.array([len(opened)], dtype=np.int32))
+        inputs = ops.batch_inputs(tables_t, cached_t, wanted_t, stack_t, height_t, self.block_size, self.num_kvcache_blocks * self.block_size, total, tree_mask=mask_t)
+        set_context(False, inputs.cu_seqlens_q, inputs.cu_seqlens_k, max(counts), int(wanted.max()), inputs.slot_mapping, inputs.context_lens, tables_t, tree_mask=mask_t)
+        logits = self.model.compute_logits(self.model(ids_t, inputs.positions))
+        picked = torch.zeros(total, dtype=torch.int64, device=self.device)
+        if self.rank == 0:
+            if rules:
+                logits = ops.adjust_logits(logits, **rules, cu_seqlens=inputs.cu_seqlens_q, draft_tokens=ids_t, tree_mask=mask_t, out=logits)
+            ops.argmax(logits, out=picked)
+        if self.world > 1:
+            ops.broadcast_tokens(picked)
+        flat = picked.tolist()  # the step's synchronisation point
+        reset_context()
+        self.runtime.check_status()
+        ends = np.cumsum(counts)
+        return [flat[e - c:e] for e, c in zip(ends, counts)]
 
     # ---- CUDA graphs (reference :222-257) -----------------------------------------
     @torch.inference_mode()

@@ -97,10 +97,13 @@ class Attention(nn.Module):
         self.k_cache = self.v_cache = torch.tensor([])
 
     def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
-        """Attention over K/V that are already in the paged cache (decode, or
-        prefill with a cached prefix) or passed in (plain prefill)."""
+        """Attention over K/V that are already in the paged cache (decode,
+        prefill with a cached prefix, or trees of drafted tokens) or passed in (plain prefill)."""
         ctx = get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
+        tree_mask = getattr(ctx, "tree_mask", None)  # (a context of the reference's fields has none)
+        if tree_mask is not None:  # trees of drafted tokens: own kernel whatever the backend, there is no library call
+            return ops.tree_attention(q, k_cache, v_cache, ctx.cu_seqlens_q, ctx.context_lens, ctx.block_tables, tree_mask, ctx.max_seqlen_q, self.scale)
         if Attention.backend == "sdpa":
             if ctx.is_prefill:
                 cu_q, cu_k = ctx.cu_seqlens_q.tolist(), ctx.cu_seqlens_k.tolist()

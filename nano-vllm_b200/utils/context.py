@@ -11,12 +11,12 @@ import torch
 
 class Context:
     __slots__ = ("is_prefill", "cu_seqlens_q", "cu_seqlens_k", "max_seqlen_q", "max_seqlen_k", "slot_mapping",
-                 "context_lens", "block_tables", "last_token_index")
+                 "context_lens", "block_tables", "last_token_index", "tree_mask")
 
     def __init__(self, is_prefill: bool = False, cu_seqlens_q: torch.Tensor | None = None, cu_seqlens_k: torch.Tensor | None = None,
                  max_seqlen_q: int = 0, max_seqlen_k: int = 0, slot_mapping: torch.Tensor | None = None,
                  context_lens: torch.Tensor | None = None, block_tables: torch.Tensor | None = None,
-                 last_token_index: torch.Tensor | None = None):
+                 last_token_index: torch.Tensor | None = None, tree_mask: torch.Tensor | None = None):
         self.is_prefill = is_prefill
         self.cu_seqlens_q, self.cu_seqlens_k = cu_seqlens_q, cu_seqlens_k
         self.max_seqlen_q, self.max_seqlen_k = max_seqlen_q, max_seqlen_k
@@ -25,6 +25,8 @@ class Context:
         if last_token_index is None and is_prefill and cu_seqlens_q is not None:
             last_token_index = (cu_seqlens_q[1:] - 1).to(torch.int32)
         self.last_token_index = last_token_index
+        # not a prefill, and not None: the step's tokens are a tree of drafted tokens per sequence (ops.tree_attention)
+        self.tree_mask = tree_mask
 
 
 _current = Context()
@@ -35,10 +37,10 @@ def get_context() -> Context:
 
 
 def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0, max_seqlen_k=0, slot_mapping=None,
-                context_lens=None, block_tables=None, last_token_index=None) -> None:
+                context_lens=None, block_tables=None, last_token_index=None, tree_mask=None) -> None:
     global _current
     _current = Context(is_prefill, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, slot_mapping, context_lens, block_tables,
-                       last_token_index)
+                       last_token_index, tree_mask)
 
 
 def reset_context() -> None:
