@@ -15,7 +15,9 @@ namespace {
 // are shifted out of its words and its other scores replaced by -inf.
 //
 // Bound: HBM for up to 128 rows (every K and V row read once: 64 keys are 32 KB, and 128 rows of products on them take half as long as
-// bringing them), the softmax's units and the tensor core's operands beyond.
+// bringing them), the softmax's units and the tensor core's operands beyond.  64 sequences of 4096 tokens with trees of 32, 32 / 8 heads (128 rows):
+// 199 us, 5.5 TB/s, of which the walk takes 172 and the joining of the parts 13.  One of 32768 with a tree of 64, 64 / 8 heads (512 rows): 80 to 92 us by
+// the clock, 0.75 to 0.86 PFLOP/s, the tensor pipe 49 % and the exponentials' 52 % busy.
 //
 // Work split: the tiles of the batch in the order (sequence, head, position) are dealt in contiguous equal ranges to CTAs, two per SM,
 // whose lengths are read on the device, so that a captured call stays balanced for any batch.  The tiles of 128 rows of an item go to different
@@ -32,7 +34,8 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int TR_ROWS = 128, TR_KEYS = 64, TR_THREADS = TR_ROWS + 64, TR_CTAS_PER_SM = 2, TR_COLUMNS = 256;
 constexpr int TR_MAX_SEQS = 1024;
-constexpr int TR_ITEM_UNITS = 2, TR_WHOLE_TILES = 8;
+constexpr int TR_ITEM_UNITS = 2;   // what an item costs beside its tiles, in tiles (21 ragged sequences, the longest CTA 32 us without them, 26 with)
+constexpr int TR_WHOLE_TILES = 8;  // (one sequence of 300 tokens, 16 / 8 heads: 11.9 us cut into 40 parts and joined, 10.3 whole)
 constexpr float TR_GROWTH = 8.f;
 constexpr uint64_t TR_LIMIT_NS = 1000000000ull;
 template <int HD>
