@@ -380,7 +380,7 @@ int b2_advance_decode(const int64_t* tokens, int64_t* input_ids, int64_t* positi
  * block_tables and free_blocks are updated in place: entries past a row's blocks, and places of the stack above its top, keep what they
  * held.  No output may overlap an input.  The other inputs are not changed, so that the same call again gives the same results.
  * tree_mask (may be NULL): int64 [>= max_tokens, mask_words] with row stride mask_stride, the new tokens' ancestors as for b2_tree_attention;
- * a token's position is then cached_lens[i] + its visible nodes - 1 (its depth), not below cached_lens[i]; its slot stays in the tokens' order.
+ * a token's position is then cached_lens[i] + its visible nodes of the row's own - 1 (its depth), not below cached_lens[i]; its slot stays in the tokens' order.
  * A row is not served when more than max_tokens are asked for by it and those before it - it then has no tokens - or when it needs
  * blocks and more than there are are asked for by it and those before it - its tokens then keep their places with slot -1 -; its
  * length and blocks stay.  A token whose table entry is negative or whose slot would be >= num_slots gets slot -1.  A row with a length

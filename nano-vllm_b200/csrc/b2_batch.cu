@@ -170,8 +170,9 @@ __global__ void __launch_bounds__(BI_THREADS) batch_inputs_kernel(const BatchArg
       const int r = row_of(s_tok, a.n, t), c = s_c[r], i = t - s_tok[r], place = c + i, j = place / bs;
       position = place;
       if (a.mask != nullptr) {
-        int sees = 0;
-        for (int w = 0; w < a.words; ++w) sees += __popcll(__ldg(reinterpret_cast<const unsigned long long*>(a.mask + t * a.mask_stride + w)));
+        int sees = 0;  // of the row's own nodes
+        for (int w = 0, left = s_tok[r + 1] - s_tok[r]; w < a.words && left > 0; ++w, left -= 64)
+          sees += __popcll(__ldg(reinterpret_cast<const unsigned long long*>(a.mask + t * a.mask_stride + w)) & (left < 64 ? (1ull << left) - 1 : ~0ull));
         position = c + max(0, sees - 1);
       }
       if (s_w[r] >= 0) {

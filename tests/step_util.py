@@ -34,7 +34,7 @@ def cumulative(counts):
     return torch.tensor([0] + list(counts)).cumsum(0).to(torch.int32)
 
 
-def batch_inputs(tables, cached, wanted, free, num_free, bs, num_slots, max_tokens, depths=None):
+def batch_inputs(tables, cached, wanted, free, num_free, bs, num_slots, max_tokens, mask=None):
     """The requests one after the other, on lists.  Returns tables, free, then the results in their order."""
     tables, free, width = [list(t) for t in tables], list(free), len(tables[0]) if tables else 0
     full = width * bs
@@ -59,7 +59,8 @@ def batch_inputs(tables, cached, wanted, free, num_free, bs, num_slots, max_toke
             for j in range(need):
                 tables[i][blocks(c) + j] = stack.pop()
         for p in range(c, w) if fits else ():
-            positions.append(p if depths is None else c + max(0, depths[len(positions)] - 1))
+            at = len(positions)
+            positions.append(p if mask is None else c + max(0, int(bits(mask[at:at + 1], min(add, 64 * mask.shape[1])).sum()) - 1))
             slot = tables[i][p // bs] * bs + p % bs if granted else -1
             slots.append(slot if granted and tables[i][p // bs] >= 0 and slot < num_slots else -1)
         lens.append(w if w < c or granted else c)

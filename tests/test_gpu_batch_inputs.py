@@ -39,8 +39,7 @@ def check(ops, tables, cached, wanted, stack, bs, max_tokens, num_slots=None, ca
     num_free = len(stack) if num_free is None else num_free
     free = (stack + [-7] * capacity)[:capacity]
     num_slots = num_slots or (1 << 30)
-    depths = None if mask is None else ref.bits(mask, 64 * mask.shape[1]).sum(1).tolist()
-    want = ref.batch_inputs(tables, cached, wanted, free, num_free, bs, num_slots, max_tokens, depths)
+    want = ref.batch_inputs(tables, cached, wanted, free, num_free, bs, num_slots, max_tokens, mask)
     t, f = on_gpu(tables) if tables else torch.zeros(0, 4, dtype=torch.int32, device=DEV), on_gpu(free)
     args = (t, on_gpu(cached), on_gpu(wanted), f, on_gpu([num_free]), bs, num_slots, max_tokens)
     for again in range(2):  # the same call on the same state gives the same
@@ -109,10 +108,13 @@ def test_positions_of_trees_follow_the_depth(ops, words):
     counts = [r.randint(0, 64 * words) for _ in range(11)]
     mask = ref.trees(counts, words, seed=words)
     mask[3] = 0  # a node that sees nothing stays at the tree's beginning
+    mask[4:9] = -1  # bits past the tree are ignored: no position lies behind the tree's last place
     cached = [r.randint(0, 90) for _ in counts]
     wanted = [c + t for c, t in zip(cached, counts)]
     got, _ = check(ops, [[i * 16 + j for j in range(16)] for i in range(11)], cached, wanted, list(range(200, 300)), 16, sum(counts), mask=mask)
-    assert (got.positions.cpu() >= 0).all()
+    first = torch.tensor(cached).repeat_interleave(torch.tensor(counts))
+    last = torch.tensor(wanted).repeat_interleave(torch.tensor(counts)) - 1
+    assert ((got.positions.cpu() >= first) & (got.positions.cpu() <= last)).all()
 
 
 def test_rows_of_a_wider_table_and_a_wider_mask(ops):
@@ -128,7 +130,7 @@ def test_rows_of_a_wider_table_and_a_wider_mask(ops):
     assert got.num_free.tolist() == [4]
     untouched = torch.cat([big[:, :3], big[:, 9:]], 1)
     assert (untouched == -9).all()
-    assert got.positions[:1].tolist() == [5]
+    assert got.positions.tolist() == [3] + [5] * 17 + [0] * 32  # one node sees itself only, the others three
 
 
 def test_a_captured_call_serves_later_batches(ops):

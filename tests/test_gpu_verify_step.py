@@ -44,8 +44,7 @@ def test_three_steps_of_a_batch(ops):
     def step(lens, counts, mask, drafts):
         nonlocal num_free, cached
         tokens = sum(counts)
-        depths = None if mask is None else ref.bits(mask, 64).sum(1).tolist()
-        want = ref.batch_inputs(host["tables"], host["cached"], lens, host["free"], host["num_free"], bs, 64 * bs, tokens, depths)
+        want = ref.batch_inputs(host["tables"], host["cached"], lens, host["free"], host["num_free"], bs, 64 * bs, tokens, mask)
         got = ops.batch_inputs(tables, cached, torch.tensor(lens, dtype=torch.int32, device=DEV), free, num_free, bs, 64 * bs, tokens, None if mask is None else mask.to(DEV))
         assert [x.tolist() for x in got] == list(want[2:]) and tables.tolist() == want[0]
         host.update(tables=want[0], free=want[1], num_free=want[8][0], cached=want[7])
