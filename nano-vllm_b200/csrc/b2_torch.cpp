@@ -541,6 +541,7 @@ PyObject* batch_inputs(Args a) {
   if (mask.defined()) {
     if (mask.dim() != 2 || mask.size(0) < max_tokens || mask.size(1) < 1) raise(PyExc_ValueError, "tree_mask: expected a row for each of %lld tokens", (long long)max_tokens);
     row_matrix(mask, at::kLong, mask.size(0), 1, "tree_mask");
+    if (mask.size(0) > 1 && mask.stride(0) < mask.size(1)) raise(PyExc_AssertionError, "tree_mask: rows must not overlap");
   }
   const std::pair<const at::Tensor*, const char*> named[] = {{&tables, "block_tables"}, {&cached, "cached_lens"}, {&wanted, "seq_lens"}, {&free, "free_blocks"}, {&num_free, "num_free"}};
   for (int i : {0, 3})
@@ -587,6 +588,8 @@ PyObject* tree_attention(Args a) {
   vector_of(cu_q, at::kInt, n_seqs + 1, "cu_seqlens_q");
   row_matrix(tables, at::kInt, n_seqs, n_seqs > 0 ? 1 : 0, "block_tables");
   row_matrix(mask, at::kLong, n, n > 0 ? 1 : 0, "tree_mask");
+  if (n_seqs > 1 && tables.stride(0) < tables.size(1)) raise(PyExc_AssertionError, "block_tables: rows must not overlap");
+  if (n > 1 && mask.stride(0) < mask.size(1)) raise(PyExc_AssertionError, "tree_mask: rows must not overlap");
   if (max_q < 0 || (n > 0 && n_seqs > 0 && max_q < 1)) raise(PyExc_ValueError, "tree_attention: max_seqlen_q %lld", (long long)max_q);
   forward_only({&q, &kc, &vc}, "tree_attention");
   on_current_gpu(q, "q");
@@ -603,7 +606,7 @@ PyObject* tree_attention(Args a) {
   if (bytes < 0) check(B2_ERR_UNSUPPORTED, "b2_tree_attention_workspace");
   const at::Tensor ws = at::detail::empty_cuda({bytes}, at::kByte, q.device(), std::nullopt);
   launch("b2_tree_attention", b2_tree_attention, ctx, q.data_ptr(), n > 1 ? q.stride(0) : nq * hd, kc.data_ptr(), vc.data_ptr(), kc.size(0), bs, tables.const_data_ptr<int32_t>(),
-         std::max(row_stride(tables), tables.size(1)), tables.size(1), cu_q.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(), mask.const_data_ptr<int64_t>(), row_stride(mask),
+         row_stride(tables), tables.size(1), cu_q.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(), mask.const_data_ptr<int64_t>(), row_stride(mask),
          mask.size(1), n_seqs, max_q, n, nq, nkv, hd, number(a[9]), out.data_ptr(), ws.data_ptr(), bytes, stream());
   return wrap(out);
 }
@@ -662,6 +665,7 @@ PyObject* adjust_logits(Args a) {
   }
   if (t[9].defined()) {
     row_matrix(t[9], at::kInt, rows, (vocab + 31) / 32, names[9]);
+    if (rows > 1 && t[9].stride(0) < (vocab + 31) / 32) raise(PyExc_AssertionError, "allowed_mask: rows must not overlap");
     r.allowed_mask = cptr<int32_t>(t[9]);
     r.allowed_stride = row_stride(t[9]);
   }
@@ -669,6 +673,7 @@ PyObject* adjust_logits(Args a) {
   if (t[11].defined()) {
     vector_of(t[11], at::kLong, rows, names[11]);
     row_matrix(t[12], at::kLong, rows, rows > 0 ? 1 : 0, names[12]);
+    if (rows > 1 && t[12].stride(0) < t[12].size(1)) raise(PyExc_AssertionError, "tree_mask: rows must not overlap");
     if (t[12].size(1) > 1 << 12) raise(PyExc_ValueError, "tree_mask: rows of %lld words", (long long)t[12].size(1));
     r.draft_tokens = cptr<int64_t>(t[11]);
     r.tree_mask = cptr<int64_t>(t[12]);

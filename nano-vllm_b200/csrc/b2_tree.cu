@@ -225,6 +225,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       const Sequence s = sequence(a, b);
       if (s.len == 0) clear(s.q0, s.q0 + s.nodes);
     }
+    if (cta == 0 && a.n_seqs > 0) clear(0, __ldg(a.cu_q));
     const int behind = a.n_seqs > 0 ? max(0, __ldg(a.cu_q + a.n_seqs)) : 0;
     for (int t = behind + cta; t < a.tokens; t += ctas) clear(t, t + 1);
   };
@@ -707,8 +708,9 @@ struct TreePlan {
 TreePlan plan_tree(const b2_ctx* ctx, int n_seqs, int max_q, int group, int nkv, int head_dim, int64_t max_len) {
   TreePlan p;
   p.npt = TR_ROWS / group;
-  p.y = std::max(1, std::min((max_q + p.npt - 1) / p.npt, 8));
-  const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(n_seqs) * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS + TR_ITEM_UNITS) * ((max_q + p.npt * p.y - 1) / (p.npt * p.y)));
+  p.y = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((static_cast<int64_t>(max_q) + p.npt - 1) / p.npt, 8)));
+  const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(n_seqs) * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS + TR_ITEM_UNITS) *
+                                              ((static_cast<int64_t>(max_q) + p.npt * p.y - 1) / (p.npt * p.y)));
   p.x = static_cast<int>(std::min<int64_t>(most, std::max(1, ctx->num_sms * TR_CTAS_PER_SM / p.y)));
   // Contexts of at most TR_WHOLE_TILES tiles are not cut where there are CTAs for all of them: the second kernel takes as long as walking so many.
   p.whole = max_len <= TR_WHOLE_TILES * TR_KEYS && n_seqs > 0 && static_cast<int64_t>(n_seqs) * nkv * p.y <= ctx->num_sms * TR_CTAS_PER_SM;

@@ -178,6 +178,21 @@ def test_nodes_that_see_nothing_and_sequences_without_a_context(ops):
     assert not got[1].any() and not got[11:].any()
 
 
+def test_tokens_before_the_first_sequence_are_zero(ops):
+    c = Case([20, 300], [4, 7], seed=27)
+    q, k, v, cu, lens, tables, mask, max_q, scale = c.args()
+    got = ops.tree_attention(q, k, v, cu[1:], lens[1:], tables[1:], mask, max_q, scale)
+    want = ops.tree_attention(q, k, v, cu, lens, tables, mask, max_q, scale)
+    assert not got[:4].any() and torch.equal(got[4:], want[4:])
+
+
+@pytest.mark.parametrize("max_q", [2 ** 31 - 1, 10 ** 6])
+def test_a_larger_max_seqlen_q(ops, max_q):
+    c = Case([200, 30], [9, 4], seed=28)
+    c.max_q = max_q
+    c.check(ops)
+
+
 @pytest.mark.parametrize("short", [-5, 0, 1, 3])
 def test_a_context_shorter_than_its_tree(ops, short):
     c = Case([20, 30], [4, 4], seed=12)
@@ -212,10 +227,12 @@ def test_what_a_node_does_not_see_may_hold_anything(ops, bad, where):
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
-def test_values_that_a_node_sees_reach_it(ops, bad):
-    c = Case([70, 3], [6, 30], nq=8, nkv=2, seed=15)
+@pytest.mark.parametrize("prefix", [70, 61, 3000])
+def test_values_that_a_node_sees_reach_it(ops, prefix, bad):
+    """Over contexts of one CTA and cut ones, in trees inside a tile and across two."""
+    c = Case([prefix, 3], [6, 30], nq=8, nkv=2, seed=15)
     c.mask[:6] = ref.masks([0b000001, 0b000011, 0b000101, 0b001011, 0b010101, 0b100011], 1).to(DEV)
-    c.v.view(-1, 2, 128)[c.slots(0, [72]), :, ::3] = bad
+    c.v.view(-1, 2, 128)[c.slots(0, [prefix + 2]), :, ::3] = bad
     got = c.check(ops)
     assert not torch.isfinite(got[[2, 4]].float()[:, :, ::3]).any()
 

@@ -46,6 +46,7 @@ STACK = torch.zeros(12, dtype=I32)
     (ValueError, dict(tree_mask=torch.zeros(7, 1, dtype=I64))),
     (ValueError, dict(tree_mask=torch.zeros(8, 0, dtype=I64))),
     (TypeError, dict(tree_mask=torch.zeros(8, 1, dtype=I32))),
+    (AssertionError, dict(tree_mask=torch.zeros(1, 2, dtype=I64).expand(8, 2))),
     (ValueError, dict(block_tables=STACK.view(3, 4), free_blocks=STACK)),
     (ValueError, dict(free_blocks=STACK, num_free=STACK[:1])),
     (ValueError, dict(block_tables=torch.zeros(8193, 1, dtype=I32), cached_lens=torch.zeros(8193, dtype=I32), seq_lens=torch.zeros(8193, dtype=I32))),
@@ -94,6 +95,8 @@ def tree_args(**kw):
     (ValueError, dict(tree_mask=torch.zeros(5, 0, dtype=I64))),
     (TypeError, dict(tree_mask=torch.zeros(5, 1, dtype=torch.bool))),
     (ValueError, dict(max_seqlen_q=0)),
+    (AssertionError, dict(block_tables=torch.zeros(1, 2, dtype=I32).expand(2, 2))),
+    (AssertionError, dict(tree_mask=torch.zeros(1, 2, dtype=I64).expand(5, 2))),
     (ValueError, dict(q=torch.zeros(5, 4, 128, dtype=BF16, requires_grad=True))),
 ])
 def test_tree_attention_refusals(ops, error, change):
@@ -144,6 +147,10 @@ ROWS = torch.zeros(5, 70)
     (ValueError, dict(draft_tokens=None)),
     (ValueError, dict(tree_mask=torch.zeros(4, 0, dtype=I64))),
     (ValueError, dict(draft_tokens=torch.zeros(3, dtype=I64))),
+    (AssertionError, dict(tree_mask=torch.zeros(1, 2, dtype=I64).expand(4, 2))),
+    (AssertionError, dict(allowed_mask=torch.zeros(1, 3, dtype=I32).expand(4, 3))),
+    (ValueError, dict(bias_ids=torch.zeros(2, 4096, dtype=I64), bias_values=torch.zeros(2, 4096))),
+    (ValueError, dict(history=torch.zeros(1, 1 << 19, dtype=I64).expand(2, 1 << 19))),
     (TypeError, dict(out=torch.zeros(4, 70, dtype=BF16))),
     (ValueError, dict(out=torch.zeros(4, 71))),
     (AssertionError, dict(out=torch.zeros(70, 4).t())),
