@@ -489,6 +489,7 @@ int b2_prefill_attention_supported(int nq, int nkv, int head_dim, int block_size
  *   out = softmax(scale q K^T over what the node sees) V, [tokens, nq, head_dim] contiguous, fp32 scores and sums
  * What a node does not see may hold anything.  A node that sees nothing, rows of a sequence whose context is shorter than its tree
  * (0: a padded sequence) and rows behind the last sequence are zero.  max_q: the most nodes of a sequence.  scale: of either sign, or zero.
+ * The sums are kept unnormalised with weights of up to 2^8: 256 * the keys seen * the largest |value| has to stay below the type's maximum (3.4e38).
  * b2_tree_attention_supported says (1 / 0) whether the shape is served: head_dim 64 or 128, up to 128 query heads per KV head, blocks of
  * a multiple of 16 tokens.  b2_tree_attention_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant; calls
  * that may run at the same time need one each), or -1 where the shape is not served; at most 1024 sequences. */
@@ -527,7 +528,8 @@ typedef struct b2_logit_rules {
   const int64_t* tree_mask;    /* [rows, mask_words], as for b2_tree_attention: the nodes a row sees are its path */
   int64_t mask_stride;
   int mask_words;
-} b2_logit_rules; /* token ids outside the vocabulary are ignored; n_bias <= 4095, history_width + 64 mask_words < 2^19 (B2_ERR_SHAPE otherwise) */
+} b2_logit_rules; /* token ids outside the vocabulary are ignored; n_bias <= 4095, mask_words <= 4096,
+                      history_width + 64 mask_words < 2^19 (an error otherwise); cu_seqlens[0] is 0 */
 int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, int fp32, int rows, int vocab, const b2_logit_rules* rules, void* stream);
 
 /* Greedy pick: out[i] = argmax_j logits[i, j] (first index on ties), int64.

@@ -571,7 +571,7 @@ PyObject* batch_inputs(Args a) {
 PyObject* tree_attention(Args a) {
   const at::Tensor &q = tensor(a[1], "q"), &kc = tensor(a[2], "k_cache"), &vc = tensor(a[3], "v_cache"), &cu_q = tensor(a[4], "cu_seqlens_q"), &lens = tensor(a[5], "context_lens"),
                    &tables = tensor(a[6], "block_tables"), &mask = tensor(a[7], "tree_mask");
-  const int64_t max_q = integer(a[8]);
+  int64_t max_q = integer(a[8]);
   if (q.dim() != 3 || kc.dim() != 4) raise(PyExc_ValueError, "tree_attention: q of 3 and caches of 4 dimensions, got %lld and %lld", (long long)q.dim(), (long long)kc.dim());
   const int64_t n = q.size(0), nq = q.size(1), hd = q.size(2), nkv = kc.size(2), bs = kc.size(1), n_seqs = lens.numel();
   if (q.scalar_type() != at::kBFloat16) raise(PyExc_TypeError, "q: expected bf16, got %s", c10::toString(q.scalar_type()));
@@ -591,6 +591,7 @@ PyObject* tree_attention(Args a) {
   if (n_seqs > 1 && tables.stride(0) < tables.size(1)) raise(PyExc_AssertionError, "block_tables: rows must not overlap");
   if (n > 1 && mask.stride(0) < mask.size(1)) raise(PyExc_AssertionError, "tree_mask: rows must not overlap");
   if (max_q < 0 || (n > 0 && n_seqs > 0 && max_q < 1)) raise(PyExc_ValueError, "tree_attention: max_seqlen_q %lld", (long long)max_q);
+  max_q = std::min(max_q, n);  // no sequence has more nodes
   forward_only({&q, &kc, &vc}, "tree_attention");
   on_current_gpu(q, "q");
   beside(kc, q, "k_cache");

@@ -335,6 +335,8 @@ class ModelRunner:
         allowed_mask, to the nodes in their order."""
         if not (len(seqs) == len(drafts) == len(parents)) or any(len(d) != len(p) for d, p in zip(drafts, parents)):
             raise ValueError("a list of drafted tokens and of their parents for each sequence")
+        if not seqs:
+            return []
         counts = [len(d) + 1 for d in drafts]
         total, words = sum(counts), -(-max(counts, default=1) // 64)
         if total > self.max_num_seqs:
@@ -353,22 +355,26 @@ class ModelRunner:
         wanted = cached + np.array(counts, dtype=np.int32)
         if any(n > len(s.block_table) * self.block_size for s, n in zip(seqs, wanted)):
             raise ValueError("the block tables have no room for the drafted tokens")
+        if max(wanted) > self.max_model_len:
+            raise ValueError(f"{max(wanted)} tokens: at most max_model_len ({self.max_model_len})")
         # the caller has dealt the blocks: the stack holds the ones that the nodes open, the first of them on top
         opened = [b for s, c, n in zip(seqs, cached, wanted) for b in s.block_table[-(-c // self.block_size):-(-n // self.block_size)]]
         ids_t, cached_t, wanted_t, tables_t, mask_t, stack_t, height_t = self._to_device(
             ids, cached, wanted, self._block_tables(seqs), mask.view(np.int64), np.array(opened[::-1], dtype=np.int32), np.array([len(opened)], dtype=np.int32))
         inputs = ops.batch_inputs(tables_t, cached_t, wanted_t, stack_t, height_t, self.block_size, self.num_kvcache_blocks * self.block_size, total, tree_mask=mask_t)
         set_context(False, inputs.cu_seqlens_q, inputs.cu_seqlens_k, max(counts), int(wanted.max()), inputs.slot_mapping, inputs.context_lens, tables_t, tree_mask=mask_t)
-        logits = self.model.compute_logits(self.model(ids_t, inputs.positions))
-        picked = torch.zeros(total, dtype=torch.int64, device=self.device)
-        if self.rank == 0:
-            if rules:
-                logits = ops.adjust_logits(logits, **rules, cu_seqlens=inputs.cu_seqlens_q, draft_tokens=ids_t, tree_mask=mask_t, out=logits)
-            ops.argmax(logits, out=picked)
-        if self.world > 1:
-            ops.broadcast_tokens(picked)
-        flat = picked.tolist()  # the step's synchronisation point
-        reset_context()
+        try:
+            logits = self.model.compute_logits(self.model(ids_t, inputs.positions))
+            picked = torch.zeros(total, dtype=torch.int64, device=self.device)
+            if self.rank == 0:
+                if rules:
+                    logits = ops.adjust_logits(logits, **rules, cu_seqlens=inputs.cu_seqlens_q, draft_tokens=ids_t, tree_mask=mask_t, out=logits)
+                ops.argmax(logits, out=picked)
+            if self.world > 1:
+                ops.broadcast_tokens(picked)
+            flat = picked.tolist()  # the step's synchronisation point
+        finally:
+            reset_context()
         self.runtime.check_status()
         ends = np.cumsum(counts)
         return [flat[e - c:e] for e, c in zip(ends, counts)]

@@ -89,3 +89,20 @@ def test_refusals(runner):
     with pytest.raises(ValueError, match="room"):
         from nanovllm_b200.engine.model_runner import Seq
         runner.verify([Seq(list(range(250)), [0])], [[1] * 10], [[0] * 10])
+
+
+def test_no_sequences_and_an_error_inside_a_step(runner):
+    from nanovllm_b200.utils.context import get_context
+    assert runner.verify([], [], []) == []
+    seqs = sequences(runner, [20], seed=8)
+    with pytest.raises(ValueError):
+        runner.verify(seqs, [[1]], [[0]], rules=dict(bias_ids=torch.zeros(2, 1, dtype=torch.int64, device="cuda"), bias_values=torch.zeros(2, 1, device="cuda")))
+    assert get_context().tree_mask is None
+    assert len(runner.step(seqs, False)) == 1
+    assert runner.verify(seqs, [[]], [[]]) == runner.verify(seqs, [[]], [[]])
+
+
+def test_nodes_past_the_longest_context_are_refused(runner):
+    from nanovllm_b200.engine.model_runner import Seq
+    with pytest.raises(ValueError, match="max_model_len"):
+        runner.verify([Seq(list(range(1020)), list(range(5)))], [[1] * 5], [[0] * 5])
