@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(BI_THREADS) batch_inputs_kernel(const BatchArg
   b2::pdl_wait();
 
   const int bs = a.block_size, full = a.bt_width * bs;  // (the host has checked that n * full is below 2^31)
-  auto blocks = [&](int tokens) { return (tokens + bs - 1) / bs; };
+  auto blocks = [&](int tokens) { return static_cast<int>((static_cast<uint32_t>(tokens) + bs - 1) / bs); };  // (the sum may pass 2^31, not 2^32)
   const int per = (a.n + BI_THREADS - 1) / BI_THREADS, r0 = min(a.n, tid * per), r1 = min(a.n, r0 + per);
   Sums mine = {0, 0, 0};
   for (int r = r0; r < r1; ++r) {

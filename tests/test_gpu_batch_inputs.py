@@ -117,6 +117,16 @@ def test_positions_of_trees_follow_the_depth(ops, words):
     assert ((got.positions.cpu() >= first) & (got.positions.cpu() <= last)).all()
 
 
+@pytest.mark.parametrize("bs, width", [(2 ** 31 - 1, 1), (2 ** 30, 1), (715827882, 3), (16, (2 ** 31 - 1) // 16)])
+def test_the_longest_rows(ops, bs, width):
+    full = bs * width
+    tables = torch.zeros(1, width, dtype=torch.int32, device=DEV)
+    got = ops.batch_inputs(tables, on_gpu([full - 9]), on_gpu([full]), on_gpu([5]), on_gpu([1]), bs, 2 ** 31 - 1, 12)
+    assert got.positions.tolist() == list(range(full - 9, full)) + [0] * 3 and got.context_lens.tolist() == [full] and got.num_free.tolist() == [1]
+    place = (full - 9) % bs
+    assert got.slot_mapping.tolist() == list(range(place, place + 9)) + [-1] * 3
+
+
 def test_rows_of_a_wider_table_and_a_wider_mask(ops):
     big = torch.full((5, 40), -9, dtype=torch.int32, device=DEV)
     tables = big[:, 3:9]
