@@ -16,7 +16,7 @@ namespace {
 //
 // Bound: HBM for up to 128 rows (every K and V row read once: 64 keys are 32 KB, and 128 rows of products on them take half as long as
 // bringing them), the softmax's units and the tensor core's operands beyond.  64 sequences of 4096 tokens with trees of 32, 32 / 8 heads (128 rows):
-// 199 us, 5.5 TB/s, of which the walk takes 172 and the joining of the parts 13.  One of 32768 with a tree of 64, 64 / 8 heads (512 rows): 80 to 92 us by
+// 199 to 227 us by the clock; of 199 (5.5 TB/s) the walk takes 172 and the joining of the parts 13.  One of 32768 with a tree of 64, 64 / 8 heads (512 rows): 80 to 92 us by
 // the clock, 0.75 to 0.86 PFLOP/s, the tensor pipe 49 % and the exponentials' 52 % busy.
 //
 // Work split: the tiles of the batch in the order (sequence, head, position) are dealt in contiguous equal ranges to CTAs, two per SM,

@@ -192,6 +192,12 @@ def test_a_larger_max_seqlen_q(ops, max_q):
     c.check(ops)
 
 
+def test_the_most_sequences_and_one_more(ops):
+    Case([i % 40 for i in range(1024)], [1 + i % 3 for i in range(1024)], nq=2, nkv=1, hd=64, seed=29).check(ops)
+    with pytest.raises(ValueError, match="1025 sequences"):
+        ops.tree_attention(*Case([0] * 1025, [1] * 1025, nq=2, nkv=1, hd=64, seed=30).args())
+
+
 @pytest.mark.parametrize("short", [-5, 0, 1, 3])
 def test_a_context_shorter_than_its_tree(ops, short):
     c = Case([20, 30], [4, 4], seed=12)

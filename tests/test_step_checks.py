@@ -145,6 +145,7 @@ ROWS = torch.zeros(5, 70)
     (ValueError, dict(cu_seqlens=None)),
     (ValueError, dict(cu_seqlens=torch.zeros(0, dtype=I32))),
     (ValueError, dict(draft_tokens=None)),
+    (ValueError, dict(tree_mask=None)),
     (ValueError, dict(tree_mask=torch.zeros(4, 0, dtype=I64))),
     (ValueError, dict(draft_tokens=torch.zeros(3, dtype=I64))),
     (AssertionError, dict(tree_mask=torch.zeros(1, 2, dtype=I64).expand(4, 2))),
