@@ -190,9 +190,7 @@ __global__ void __launch_bounds__(BI_THREADS) batch_inputs_kernel(const BatchArg
     a.tables[static_cast<int64_t>(r) * a.bt_stride + blocks(s_c[r]) + k - s_need[r]] = stacked(top - 1 - k);
   }
   for (int i = num_free + first; i < min(a.capacity, top - taken); i += step) a.free_blocks[i] = returned(i - num_free);
-  // later kernels may read the lengths and tables ahead of their dependency wait: released only now
-  __threadfence();
-  b2::pdl_launch_dependents();
+  b2::pdl_release_results();  // later kernels may read the lengths and tables ahead of their dependency wait
 }
 
 int configure_once() {

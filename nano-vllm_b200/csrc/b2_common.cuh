@@ -102,6 +102,13 @@ __device__ __forceinline__ void report_timeout(B2Status* st, int detail) {
 // completed and its writes are visible.  Both are no-ops for a plain launch.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// The same for a kernel whose results are read ahead of the dependency wait.  A CTA counts as released when the first of its threads
+// is, so all of them meet here behind their last store.
+__device__ __forceinline__ void pdl_release_results() {
+  __threadfence();
+  __syncthreads();
+  pdl_launch_dependents();
+}
 
 // ---- thread-block clusters / distributed shared memory --------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
