@@ -535,9 +535,7 @@ __global__ void advance_decode_kernel(const int64_t* __restrict__ tokens, int64_
   b2::pdl_wait();
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i < n) advance_row(i, tokens, input_ids, positions, context_lens, slot_mapping, block_tables, bt_stride, bt_width, block_size, num_slots);
-  // later kernels may read the new lengths ahead of their dependency wait: released only now
-  __threadfence();
-  b2::pdl_launch_dependents();
+  b2::pdl_release_results();  // later kernels may read the new lengths ahead of their dependency wait
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

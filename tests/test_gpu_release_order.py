@@ -91,3 +91,43 @@ def test_decode_attention_behind_batch_inputs(ops, cache, n, store):
         t.copy_(i32(tables))
         _, eager = step(wait=False)
         assert torch.equal(eager, want), f"call {i}"
+
+
+@pytest.mark.parametrize("n", [1, 33, 128, 500])
+def test_decode_attention_behind_advance_decode(ops, cache, n):
+    """Contexts on both sides of a block's end; the last row of each warp is frozen, so that its threads have less to do than the others."""
+    r = random.Random(n)
+    lens = [r.choice((1, 31, BS - 1, BS, BS + 1, 2 * BS - 1)) for _ in range(n)]
+    blocks = r.sample(range(BLOCKS), 3 * n)
+    t = i32(blocks).view(n, 3)
+    q = queries(n, 4)
+    tokens, ids = torch.arange(n, device=DEV), torch.zeros(n, dtype=torch.int64, device=DEV)
+    start = i32(lens)
+    slot = i32([-1 if i % 32 == 31 else blocks[3 * i + (x - 1) // BS] * BS + (x - 1) % BS for i, x in enumerate(lens)])
+    position, c, s = torch.zeros(n, dtype=torch.int64, device=DEV), torch.zeros_like(start), torch.zeros_like(slot)
+
+    def reset():
+        position.copy_(start - 1)
+        c.copy_(start)
+        s.copy_(slot)
+
+    def step(wait):
+        ops.advance_decode(tokens, ids, position, c, s, t, BS, BLOCKS * BS)
+        if wait:
+            torch.cuda.synchronize()
+        return ops.paged_attention(q, *cache, c, t, HD ** -0.5)
+
+    reset()
+    want = step(wait=True)
+    after = [x + (i % 32 != 31) for i, x in enumerate(lens)]
+    assert c.tolist() == after
+    hold_against_definition(want, q, cache, after, t)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(wait=False)
+    for i in range(50):
+        reset()
+        graph.replay()
+        assert torch.equal(got, want), f"replay {i}"
+        reset()
+        assert torch.equal(step(wait=False), want), f"call {i}"

@@ -31,7 +31,7 @@ def test_a_release_of_results_waits_for_the_whole_cta():
 
 
 # kernels whose lengths and tables decode attention reads ahead of its dependency wait
-@pytest.mark.parametrize("name, kernel", [("b2_batch.cu", "batch_inputs_kernel")])
+@pytest.mark.parametrize("name, kernel", [("b2_batch.cu", "batch_inputs_kernel"), ("b2_elementwise.cu", "advance_decode_kernel")])
 def test_what_is_read_ahead_is_released_at_the_end(name, kernel):
     text = body(code(name), kernel)
     assert "pdl_launch_dependents" not in text and "return;" not in text
