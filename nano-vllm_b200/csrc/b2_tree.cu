@@ -178,7 +178,6 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     b2::tmem_alloc(b2::smem_u32(&s_tmem), TR_COLUMNS);
     b2::tmem_relinquish();
   }
-  b2::pdl_launch_dependents();
   b2::pdl_wait();
 
   // ---- units per sequence, prefix-summed by one warp ----
@@ -209,6 +208,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   __syncthreads();
   b2::tc_fence_after();
   const uint32_t tmem = b2::uniform(s_tmem);
+  // (Only now: a kernel that waits for this one with columns of tensor memory in hand must not get the ones that this CTA has yet to allocate.)
+  b2::pdl_launch_dependents();
   const int x = blockIdx.x, y = blockIdx.y, total = first_unit[a.n_seqs] * a.nkv;
 
   // ---- rows without anything to see: of sequences with a context shorter than their tree, and behind the last sequence (by the warps of the

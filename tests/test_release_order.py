@@ -36,3 +36,25 @@ def test_what_is_read_ahead_is_released_at_the_end(name, kernel):
     text = body(code(name), kernel)
     assert "pdl_launch_dependents" not in text and "return;" not in text
     assert text.rstrip().endswith("b2::pdl_release_results();")
+
+
+def kernels(text):
+    return re.findall(r"__global__\s+void\s+(?:__launch_bounds__\([^;{]*?\)\s+)?(\w+)\(", text)
+
+
+def test_columns_are_allocated_before_the_next_kernel_is_let_in():
+    """A kernel that is let in early keeps its columns of tensor memory until this one has ended, so this one's CTA must have its own by then: the
+    release stands behind a barrier that the allocating warp meets with its columns."""
+    found = []
+    for name in sorted(os.listdir(CSRC)):
+        text = code(name)
+        for kernel in kernels(text):
+            inside = body(text, kernel)
+            if "tmem_alloc" not in inside:
+                continue
+            found.append(kernel)
+            before, after = inside.split("tmem_alloc", 1)
+            assert "pdl_launch_dependents" not in before, kernel
+            if "pdl_launch_dependents" in after:  # (or in a function that runs at the end)
+                assert "__syncthreads();" in after[:after.index("pdl_launch_dependents")], kernel
+    assert {"tree_attention_kernel", "prefill_attention_kernel", "gemm_kernel", "gemm_tile_kernel", "gemm_pair_kernel"} <= set(found), found
