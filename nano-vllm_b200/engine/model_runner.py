@@ -332,7 +332,7 @@ class ModelRunner:
         decode step, and drafts[i][j] is node j + 1, whose parent is node parents[i][j] <= j.  Returns the greedy pick after every node, on every rank.  The
         block tables must have room for all nodes; keys and values of node j are left at place len(seq) - 1 + j.  rules: arguments of
         ops.adjust_logits that belong to the sequences (histories end before the last token: node 0 counts as part of every path) or,
-        allowed_mask, to the nodes in their order."""
+        allowed_mask, to the nodes in their order; they are looked at on rank 0 only, whose error makes every rank raise."""
         if not (len(seqs) == len(drafts) == len(parents)) or any(len(d) != len(p) for d, p in zip(drafts, parents)):
             raise ValueError("a list of drafted tokens and of their parents for each sequence")
         if not seqs:
@@ -365,17 +365,25 @@ class ModelRunner:
         set_context(False, inputs.cu_seqlens_q, inputs.cu_seqlens_k, max(counts), int(wanted.max()), inputs.slot_mapping, inputs.context_lens, tables_t, tree_mask=mask_t)
         try:
             logits = self.model.compute_logits(self.model(ids_t, inputs.positions))
-            picked = torch.zeros(total, dtype=torch.int64, device=self.device)
+            picked, failed = torch.zeros(total, dtype=torch.int64, device=self.device), None
             if self.rank == 0:
-                if rules:
-                    logits = ops.adjust_logits(logits, **rules, cu_seqlens=inputs.cu_seqlens_q, draft_tokens=ids_t, tree_mask=mask_t, out=logits)
-                ops.argmax(logits, out=picked)
+                try:
+                    if rules:
+                        logits = ops.adjust_logits(logits, **rules, cu_seqlens=inputs.cu_seqlens_q, draft_tokens=ids_t, tree_mask=mask_t, out=logits)
+                    ops.argmax(logits, out=picked)
+                except Exception as error:  # (the other ranks are on their way to the broadcast: they get a token that there is not)
+                    failed = error
+                    picked.fill_(self.config.vocab_size)
             if self.world > 1:
                 ops.broadcast_tokens(picked)
             flat = picked.tolist()  # the step's synchronisation point
         finally:
             reset_context()
         self.runtime.check_status()
+        if failed is not None:
+            raise failed
+        if flat[0] >= self.config.vocab_size:
+            raise RuntimeError("rank 0 could not apply the step's rules or pick its tokens; its own error says why")
         ends = np.cumsum(counts)
         return [flat[e - c:e] for e, c in zip(ends, counts)]
 
