@@ -507,8 +507,8 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
  *   count > 0:  x = x - frequency_penalty[s] * count - presence_penalty[s]     (count: in the output part of history and the path)
  *   x = x + the bias of v;   not allowed: x = -inf
  * then rounded to the logits' type; logits that no rule touches are copied bit for bit.  out may be logits itself, with the same stride.
- * Every rule may be left out (NULL).  Request s's rows are cu_seqlens[s] .. cu_seqlens[s+1], rows behind the last request are copied; with
- * cu_seqlens NULL row i is request i and n_seqs = rows. */
+ * Every rule may be left out (NULL).  Request s's rows are cu_seqlens[s] .. cu_seqlens[s+1], rows before the first request and behind the
+ * last are copied; with cu_seqlens NULL row i is request i and n_seqs = rows. */
 typedef struct b2_logit_rules {
   int n_seqs;
   const int32_t* cu_seqlens;
@@ -529,7 +529,7 @@ typedef struct b2_logit_rules {
   int64_t mask_stride;
   int mask_words;
 } b2_logit_rules; /* token ids outside the vocabulary are ignored; n_bias <= 4095, mask_words <= 4096,
-                      history_width + 64 mask_words < 2^19 (an error otherwise); cu_seqlens[0] is 0 */
+                      history_width + 64 mask_words < 2^19 (an error otherwise) */
 int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, int fp32, int rows, int vocab, const b2_logit_rules* rules, void* stream);
 
 /* Greedy pick: out[i] = argmax_j logits[i, j] (first index on ties), int64.

@@ -166,8 +166,9 @@ __global__ void __launch_bounds__(AL_THREADS, Slice<T>::CTAS_PER_SM) adjust_logi
 
     // ---- the row's request ----
     int s = row;
+    bool ruled = true;  // rows before the first request and behind the last are copied
     if (a.cu != nullptr) {
-      if (seq >= 0 && row < seq_end) {
+      if (seq >= 0 && row >= node0 && row < seq_end) {
         s = seq;
       } else {
         s = 0;
@@ -177,9 +178,9 @@ __global__ void __launch_bounds__(AL_THREADS, Slice<T>::CTAS_PER_SM) adjust_logi
           if (__ldg(a.cu + mid + 1) > row) hi = mid;
           else s = mid + 1;
         }
+        ruled = s < a.n_seqs && __ldg(a.cu + s) <= row;
       }
     }
-    const bool ruled = s < a.n_seqs;  // rows behind the last request are copied
     if (ruled && s != seq) {
       seq = s;
       seq_end = row + 1;

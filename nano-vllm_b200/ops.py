@@ -298,7 +298,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     output part, and presence_penalty once, are taken off.  bias_ids int64 / bias_values fp32 [n, k] are added (of equal ids the last counts; ids outside the
     vocabulary are ignored).  allowed_mask int32 [rows, (vocab + 31) / 32]: tokens whose bit is not set get -inf.
 
-    Row i belongs to request i, or with cu_seqlens int32 [n + 1] request s has rows cu_seqlens[s] .. cu_seqlens[s + 1] (rows behind the last are
-    copied); with draft_tokens int64 [rows] and tree_mask (as for tree_attention) the drafted tokens that a row's node sees count as its output."""
+    Row i belongs to request i, or with cu_seqlens int32 [n + 1] request s has rows cu_seqlens[s] .. cu_seqlens[s + 1] (rows before the first
+    and behind the last are copied); with draft_tokens int64 [rows] and tree_mask (as for tree_attention) the drafted tokens that a row's node sees count as its output."""
     return _native.adjust_logits(logits, history, history_lens, prompt_lens, repetition_penalty, presence_penalty, frequency_penalty, bias_ids, bias_values, allowed_mask,
                                  cu_seqlens, draft_tokens, tree_mask, out)

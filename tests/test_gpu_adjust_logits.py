@@ -278,3 +278,20 @@ def test_captured_and_on_another_stream(ops):
     stream.synchronize()
     check(out, other, c)
     assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("rules", ["all", "mask", "trees"])
+@pytest.mark.parametrize("first", [1, 5])
+def test_rows_before_the_first_request_are_copied(ops, first, rules):
+    """cu_seqlens need not begin at 0: the rows before its first element belong to nobody, like those behind its last, in every slice of the vocabulary."""
+    cu = torch.tensor([first, first, first + 3, first + 4], dtype=torch.int32)
+    rows = first + 6
+    logits, a = request(3, 9001, rows, seed=first, penalties=rules != "mask", bias=0 if rules == "mask" else 4)
+    a["cu_seqlens"] = cu
+    if rules == "trees":
+        a["draft_tokens"] = torch.arange(rows) * 700
+        a["tree_mask"] = torch.full((rows, 1), -1, dtype=torch.int64)
+    got = ops.adjust_logits(logits.to(DEV), **on_gpu(a))
+    check(got, logits, a)
+    assert torch.equal(got[:first].cpu(), logits[:first]) and torch.equal(got[first + 4:].cpu(), logits[first + 4:])
+    assert not torch.equal(got[first:first + 4].cpu(), logits[first:first + 4])
