@@ -383,7 +383,7 @@ int b2_advance_decode(const int64_t* tokens, int64_t* input_ids, int64_t* positi
  * a token's position is then cached_lens[i] + its visible nodes of the row's own - 1 (its depth), not below cached_lens[i]; its slot stays in the tokens' order.
  * A row is not served when more than max_tokens are asked for by it and those before it - it then has no tokens - or when it needs
  * blocks and more than there are are asked for by it and those before it - its tokens then keep their places with slot -1 -; its
- * length and blocks stay.  A token whose table entry is negative or whose slot would be >= num_slots gets slot -1.  A row with a length
+ * length and blocks stay.  (Attention over such a row's tokens with its context_lens takes its last cached tokens for the new ones; what it gives means nothing.)  A token whose table entry is negative or whose slot would be >= num_slots gets slot -1.  A row with a length
  * that is negative or more than bt_width * block_size counts as a row without tokens.  A block may belong to one row only.
  * n <= 8192 and n * bt_width * block_size < 2^31 (B2_ERR_SHAPE otherwise). */
 int b2_batch_inputs(int32_t* block_tables, int64_t bt_stride, int bt_width, const int32_t* cached_lens, const int32_t* seq_lens, int n,

@@ -272,7 +272,7 @@ def batch_inputs(block_tables: torch.Tensor, cached_lens: torch.Tensor, seq_lens
     block_tables [n, width] and free_blocks are updated in place, the new stack's height is the result's num_free.  max_tokens: room for the
     step's new tokens (a captured call serves any batch that fits).  tree_mask int64 [max_tokens or more, words]: the new tokens are trees of drafted tokens,
     whose positions follow their depth.  A request for which there are no blocks or no room is not served: its context_lens
-    stays cached_lens[i].  The rules in full are at b2_batch_inputs."""
+    stays cached_lens[i], and what attention gives for such tokens of it as keep their rows (they have no slots) means nothing.  The rules in full are at b2_batch_inputs."""
     return BatchInputs(*_native.batch_inputs(block_tables, cached_lens, seq_lens, free_blocks, num_free, block_size, num_slots, max_tokens, tree_mask))
 
 

@@ -98,3 +98,28 @@ def test_three_steps_of_a_batch(ops):
         num_free, cached = got.num_free, got.context_lens
         for i in range(n):
             keys[i], values[i] = [torch.cat(keys[i])[:lens[i]]], [torch.cat(values[i])[:lens[i]]]
+
+
+def test_a_request_that_is_not_served(ops):
+    """Too few blocks for one of three requests: the others' rows are right, and its own are zero where its length is replaced by 0."""
+    nq, nkv, hd, bs = 8, 2, 128, 16
+    g = torch.Generator(device=DEV).manual_seed(2)
+
+    def normal(*shape):
+        return torch.empty(*shape, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+
+    def i32(values):
+        return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+    k_cache, v_cache, counts, cached = normal(8, bs, nkv, hd), normal(8, bs, nkv, hd), [4, 5, 3], [12, 14, 3]
+    tables, seq_lens, mask = i32([[1, -1], [2, -1], [3, -1]]), i32([16, 19, 6]), ref.trees(counts, 1, 2)
+    inp = ops.batch_inputs(tables, i32(cached), seq_lens, i32([7]), i32([0]), bs, 8 * bs, 12, mask.to(DEV))
+    assert inp.context_lens.tolist() == [16, 14, 6] and inp.slot_mapping.tolist()[4:9] == [-1] * 5 and inp.cu_seqlens_q.tolist() == [0, 4, 9, 12]
+    ops.store_kvcache(normal(12, nkv, hd), normal(12, nkv, hd), k_cache, v_cache, inp.slot_mapping)
+    q = normal(12, nq, hd)
+    lens = torch.where(inp.context_lens == seq_lens, inp.context_lens, 0)
+    o = ops.tree_attention(q, k_cache, v_cache, inp.cu_seqlens_q, lens, tables, mask.to(DEV), 5, hd ** -0.5)
+    want, size = ref.tree_attention(q, k_cache, v_cache, counts, [16, 0, 6], tables, mask, hd ** -0.5)
+    assert (o[4:9] == 0).all() and ((o.double() - want).abs() <= 2.0 ** -7 * size + 2.0 ** -9 * size).all()
+    unserved = ops.tree_attention(q, k_cache, v_cache, inp.cu_seqlens_q, inp.context_lens, tables, mask.to(DEV), 5, hd ** -0.5)
+    assert torch.equal(unserved[:4], o[:4]) and torch.equal(unserved[9:], o[9:])
