@@ -330,7 +330,8 @@ class ModelRunner:
     def verify(self, seqs: list[Seq], drafts: list[list[int]], parents: list[list[int]], rules: dict[str, torch.Tensor] | None = None) -> list[list[int]]:
         """One forward pass over a tree of drafted tokens per sequence (speculative decoding): node 0 is the sequence's last token, as in a
         decode step, and drafts[i][j] is node j + 1, whose parent is node parents[i][j] <= j.  Returns the greedy pick after every node, on every rank.  The
-        block tables must have room for all nodes; keys and values of node j are left at place len(seq) - 1 + j.  rules: arguments of
+        block tables must have room for all nodes, of which there are at most max_num_seqs in all; keys and values of node j are left at place
+        len(seq) - 1 + j.  Whoever keeps a path other than nodes 0, 1, 2, ... moves its nodes together in kv_cache first: node j of the path to place len(seq) - 1 + j.  rules: arguments of
         ops.adjust_logits that belong to the sequences (histories end before the last token: node 0 counts as part of every path) or,
         allowed_mask, to the nodes in their order; they are looked at on rank 0 only, whose error makes every rank raise."""
         if not (len(seqs) == len(drafts) == len(parents)) or any(len(d) != len(p) for d, p in zip(drafts, parents)):

@@ -106,3 +106,48 @@ def test_nodes_past_the_longest_context_are_refused(runner):
     from nanovllm_b200.engine.model_runner import Seq
     with pytest.raises(ValueError, match="max_model_len"):
         runner.verify([Seq(list(range(1020)), list(range(5)))], [[1] * 5], [[0] * 5])
+
+
+def keep(runner, seq, path, drafts, pick):
+    """The path's keys and values behind the sequence's, its tokens and the pick after it appended: what a program does with a step's result."""
+    bs = runner.block_size
+
+    def slots(places):
+        return torch.tensor([seq.block_table[p // bs] * bs + p % bs for p in places], device="cuda")
+
+    first = len(seq) - 1
+    rows = runner.kv_cache.view(2, runner.kv_cache.shape[1], -1, *runner.kv_cache.shape[4:])
+    rows[:, :, slots(first + j for j in range(len(path)))] = rows[:, :, slots(first + node for node in path)]
+    seq.token_ids += [drafts[node - 1] for node in path[1:]] + [pick]
+
+
+@pytest.mark.parametrize("path", [[0, 1, 2], [0, 2, 4], [0, 3], [0]])
+def test_a_kept_path_is_the_next_steps_context(runner, path):
+    """Trees with two branches, across a block's end: after a kept path, wherever its nodes lay, the next step's picks are those of plain decoding over the same tokens."""
+    from nanovllm_b200.engine.model_runner import Seq
+    seqs = sequences(runner, [40, 253], seed=9)
+    drafts, parents = [[11, 12, 13, 14], [21, 22, 23, 24]], [[0, 0, 0, 2], [0, 0, 0, 2]]
+    if path == [0, 1, 2]:
+        parents = [[0, 1, 2, 3]] * 2
+    plain = [Seq(list(s.token_ids), [b + 8 for b in s.block_table]) for s in seqs]  # the same requests in blocks of their own
+    for p in plain:
+        p.token_ids.pop()
+    runner.step(plain, True)
+    for p, s in zip(plain, seqs):
+        p.token_ids.append(s.token_ids[-1])
+    picked = runner.verify(seqs, drafts, parents)
+    for node in path[1:]:
+        runner.step(plain, False)
+        for p, d in zip(plain, drafts):
+            p.token_ids.append(d[node - 1])
+    runner.step(plain, False)
+    for s, p, d, picks in zip(seqs, plain, drafts, picked):
+        keep(runner, s, path, d, picks[path[-1]])
+        p.token_ids.append(picks[path[-1]])
+        assert s.token_ids == p.token_ids
+    # (plain decoding rounds its keys in launches of other shapes: the logits are held to the path's tolerance, not to the bit)
+    ids, pos = runner.prepare_decode(plain)
+    want = runner.run_model(ids, pos, False).float().clone()
+    ids, pos = runner.prepare_decode(seqs)
+    got = runner.run_model(ids, pos, False).float()
+    assert ((got - want).abs() <= 2e-2 + 1e-2 * want.abs()).all(), (got - want).abs().max().item()

@@ -123,3 +123,34 @@ def test_a_request_that_is_not_served(ops):
     assert (o[4:9] == 0).all() and ((o.double() - want).abs() <= 2.0 ** -7 * size + 2.0 ** -9 * size).all()
     unserved = ops.tree_attention(q, k_cache, v_cache, inp.cu_seqlens_q, inp.context_lens, tables, mask.to(DEV), 5, hd ** -0.5)
     assert torch.equal(unserved[:4], o[:4]) and torch.equal(unserved[9:], o[9:])
+
+
+def test_paths_are_kept_and_the_rest_is_given_back(ops):
+    """The lines between two steps: each tree's kept path moved to the places behind what was cached, then the lengths cut."""
+    nkv, hd, bs, layers = 2, 128, 16, 3
+    g = torch.Generator(device=DEV).manual_seed(4)
+    kv_cache = torch.empty(2, layers, 16, bs, nkv, hd, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    cached, counts, paths = [14, 0, 33], [7, 3, 6], [[0, 2, 5, 6], [0], [0, 1, 4]]
+    block_tables = torch.tensor([[5, -1, -1], [-1, -1, -1], [3, 9, 1]], dtype=torch.int32, device=DEV)
+    free_blocks = torch.tensor([0, 2, 4, 6], dtype=torch.int32, device=DEV)
+    lens, num_free = torch.tensor(cached, dtype=torch.int32, device=DEV), torch.tensor([4], dtype=torch.int32, device=DEV)
+    inp = ops.batch_inputs(block_tables, lens, lens + torch.tensor(counts, dtype=torch.int32, device=DEV), free_blocks, num_free, bs, 16 * bs, sum(counts))
+    old = kv_cache.clone().view(2, layers, -1, nkv, hd)
+    first = torch.tensor([c for c, p in zip([0, 7, 10], paths) for _ in p], device=DEV)
+    j, path = torch.tensor([i for p in paths for i in range(len(p))], device=DEV), torch.tensor([n for p in paths for n in p], device=DEV)
+
+    dst, src = inp.slot_mapping[first + j], inp.slot_mapping[first + path]
+    rows = kv_cache.view(2, layers, -1, nkv, hd)
+    rows[:, :, dst] = rows[:, :, src]
+    kept_lens = lens + torch.tensor([len(p) for p in paths], dtype=torch.int32, device=DEV)
+    kept = ops.batch_inputs(block_tables, inp.context_lens, kept_lens, free_blocks, inp.num_free, bs, 16 * bs, 0)
+
+    assert kept.context_lens.tolist() == [18, 1, 36] and kept.num_free.tolist() == [2] and block_tables[:, 0].tolist()[0] == 5
+    tables = block_tables.tolist()
+    for i, (c, p) in enumerate(zip(cached, paths)):
+        def slot(place):
+            return tables[i][place // bs] * bs + place % bs
+        for place in range(c):
+            assert torch.equal(rows[:, :, slot(place)], old[:, :, slot(place)])
+        for k, node in enumerate(p):
+            assert torch.equal(rows[:, :, slot(c + k)], old[:, :, slot(c + node)]), (i, k)
