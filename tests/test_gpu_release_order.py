@@ -131,3 +131,42 @@ def test_decode_attention_behind_advance_decode(ops, cache, n):
         assert torch.equal(got, want), f"replay {i}"
         reset()
         assert torch.equal(step(wait=False), want), f"call {i}"
+
+
+@pytest.mark.parametrize("n, heads", [(40, (4, 2)), (512, (4, 2)), (300, (8, 2))])
+def test_steps_one_after_the_other(ops, cache, n, heads):
+    """Eight steps back to back, each of which changes lengths and tables that the attention before it has read: nothing of the step before is seen."""
+    r = random.Random(n)
+    cached = [r.choice((0, 1, BS - 5, BS - 1, BS)) for _ in range(n)]
+    free = r.sample(range(1, BLOCKS), BLOCKS - 1)
+    tables = [[free.pop() for _ in range(-(-c // BS))] + [-1] * (3 - -(-c // BS)) for c in cached]
+    q = torch.empty(n, heads[0], HD, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(5))
+    t, f, height, start = i32(tables), i32(free), i32([len(free)]), i32(cached)
+    wanted = [start + r.choice((3, 5)) * (i + 1) for i in range(8)]
+
+    def steps(wait):
+        lens, left, out = start, height, []
+        for w in wanted:
+            inp = ops.batch_inputs(t, lens, w, f, left, BS, BLOCKS * BS, 5 * n)
+            if wait:
+                torch.cuda.synchronize()
+            out.append(ops.paged_attention(q, *cache, inp.context_lens, t, HD ** -0.5))
+            if wait:
+                torch.cuda.synchronize()
+            lens, left = inp.context_lens, inp.num_free
+        return torch.stack(out)
+
+    def reset():
+        t.copy_(i32(tables))
+        f.copy_(i32(free))
+
+    want = steps(wait=True)
+    assert len({x.sum().item() for x in want.double()}) == 8
+    reset()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = steps(wait=False)
+    for i in range(30):
+        reset()
+        graph.replay()
+        assert torch.equal(got, want), f"replay {i}"
