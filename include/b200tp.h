@@ -488,7 +488,8 @@ int b2_prefill_attention_supported(int nq, int nkv, int head_dim, int block_size
  * node sees node k of its sequence, itself included; bits past the tree are ignored, nodes past 64 * mask_words are not seen.
  *   out = softmax(scale q K^T over what the node sees) V, [tokens, nq, head_dim] contiguous, fp32 scores and sums
  * What a node does not see may hold anything.  A node that sees nothing, rows of a sequence whose context is shorter than its tree
- * (0: a padded sequence) and rows behind the last sequence are zero.  max_q: the most nodes of a sequence.  scale: of either sign, or zero.
+ * (0: a padded sequence) and rows behind the last sequence are zero.  max_q: the most nodes of a sequence (the work is dealt by it: any number from
+ * 1 is served, and one far above the truth costs several times the time).  scale: of either sign, or zero.
  * The sums are kept unnormalised with weights of up to 2^8: 256 * the keys seen * the largest |value| has to stay below the type's maximum (3.4e38).
  * b2_tree_attention_supported says (1 / 0) whether the shape is served: head_dim 64 or 128, up to 128 query heads per KV head, blocks of
  * a multiple of 16 tokens.  b2_tree_attention_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant; calls

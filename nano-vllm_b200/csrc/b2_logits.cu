@@ -26,10 +26,12 @@ namespace {
 // token is one thread's, so that the order changes nothing.
 //
 // Measured (one row of 151936 with penalties and biases / 33 rows of 50257 in fp32 after 15000 to 30000 tokens / 64 rows with all rules / 512 rows of 32 trees):
-// 7.0 / 30 / 22 / 87 us; the bytes alone take - / 3 / 6.4 / 49.  What is left is the counting - a warp's atomic takes as long for the few lanes whose
-// token is in the slice as for all of them - and the barriers between a step's phases.  Tried: a CTA for each step, loads and phases one after the other
-// 7 / 26 / 33 / 220; 512 threads, whose registers spill, 172 for the trees; pieces by bulk copies through a ring 7 / 34 / 26 / 88; one kernel that
-// copies and masks and one that counts and stores the listed tokens 11 / 26 / 20 / 116; lists from a kernel of their own 12 / 32 / 26 / 79.
+// device time of calls one after the other 3.9 / 29 / 22 / 86 us; the bytes alone take - / 3 / 6.4 / 49.  What is left for long histories is the counting: each
+// of 13 or 19 slices reads all of them, and no unit is full (issue slots 55 and 49 %, HBM 5 and 11 %); for the trees the barriers between a step's phases, where
+// a warp waits longest (4.7 of 13.7 cycles an instruction).  Tried, passes timed with the host, on which this kernel took 7.0 / 30 / 22 / 87: a CTA for
+// each step, loads and phases one after the other 7 / 26 / 33 / 220 (better for the 33 rows, which have no drafts and few rules, and for nothing else); 512 threads,
+// whose registers spill, 172 for the trees; pieces by bulk copies through a ring 7 / 34 / 26 / 88; one kernel that copies and masks and one that counts and
+// stores the listed tokens 11 / 26 / 20 / 116; lists from a kernel of their own 12 / 32 / 26 / 79.
 // ---------------------------------------------------------------------------
 constexpr int AL_THREADS = 256;
 constexpr int AL_PIECE = 16384;  // bytes

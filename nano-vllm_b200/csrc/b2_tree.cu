@@ -21,7 +21,9 @@ namespace {
 //
 // Work split: the tiles of the batch in the order (sequence, head, position) are dealt in contiguous equal ranges to CTAs, two per SM,
 // whose lengths are read on the device, so that a captured call stays balanced for any batch.  The tiles of 128 rows of an item go to different
-// CTAs that walk the same ranges (blockIdx.y), at the same time, so that HBM is read once and the others find the keys in L2.  An item that several
+// CTAs that walk the same ranges (blockIdx.y), at the same time, so that HBM is read once and the others find the keys in L2.  There are as many side by side as the
+// batch's longest tree needs, by max_q, and the ranges are that much fewer: sequences with smaller trees leave the CTAs of the higher tiles idle (21 ragged
+// sequences, 25 nodes to a tile: 24 us where the longest tree has 25, 30 with 27, and 72 where max_q says 200 of the 27).  An item that several
 // ranges share leaves its parts - unnormalised sums in 32 bits with their maxima - in the workspace, and tree_combine_kernel joins
 // them in the order of the ranges.
 //
@@ -35,7 +37,10 @@ namespace {
 constexpr int TR_ROWS = 128, TR_KEYS = 64, TR_THREADS = TR_ROWS + 64, TR_CTAS_PER_SM = 2, TR_COLUMNS = 256;
 constexpr int TR_MAX_SEQS = 1024;
 constexpr int TR_ITEM_UNITS = 2;   // what an item costs beside its tiles, in tiles (21 ragged sequences, the longest CTA 32 us without them, 26 with)
-constexpr int TR_WHOLE_TILES = 8;  // (one sequence of 300 tokens, 16 / 8 heads: 11.9 us cut into 40 parts and joined, 10.3 whole)
+// Contexts whole and cut (tables as narrow as they can be, 16 / 8 heads, trees of 5; one sequence: 8 items, eight: 64): 4 tiles 9.3 and 10.1 us, 10.1 and 14.8;
+// 6 tiles 11.0 and 11.0, 11.8 and 15.1; 8 tiles 12.6 and 11.1, 13.5 and 16.3; 12 tiles 15.9 and 11.7, 16.9 and 17.5.  The line lies at 6 tiles for one sequence and behind 12
+// for eight; 8 gives away an eighth of the one to win a sixth of the other.
+constexpr int TR_WHOLE_TILES = 8;
 constexpr float TR_GROWTH = 8.f;
 constexpr uint64_t TR_LIMIT_NS = 1000000000ull;
 template <int HD>
@@ -434,7 +439,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 #pragma unroll
             for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(r[e >> 5][(e & 31) + k]));
           // The reference m moves when the row is TR_GROWTH past it (or has seen its first key): O then has to be rescaled, which takes as long as
-          // half a tile.  Until then probabilities are up to 2^TR_GROWTH, which costs no bits: they are rounded relative to themselves.
+          // half a tile.  Until then probabilities are up to 2^TR_GROWTH and rounded relative to themselves, the largest one too, which would be exactly one
+          // at a reference that is the maximum.  What that costs, as the norm of the error over the norm (64 / 8 heads, a tree of 64 behind 8192 tokens, queries
+          // of size 0.3 / 1 / 2): 2.32e-3 / 2.32e-3 / 2.26e-3, with every growth taken up at once 2.31e-3 / 2.21e-3 / 1.81e-3 (1.66e-3 is the result's own rounding);
+          // what it saves: 77 instead of 88 us for one context of 32768, 199 instead of 204 for 64 of 4096.
           // (Each row for itself: its result does not depend on the rows beside it.)
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           const bool grown = (top - m) * a.scale_log2 > TR_GROWTH;
@@ -713,7 +721,7 @@ TreePlan plan_tree(const b2_ctx* ctx, int n_seqs, int max_q, int group, int nkv,
   const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(n_seqs) * nkv * ((max_len + TR_KEYS - 1) / TR_KEYS + TR_ITEM_UNITS) *
                                               ((static_cast<int64_t>(max_q) + p.npt * p.y - 1) / (p.npt * p.y)));
   p.x = static_cast<int>(std::min<int64_t>(most, std::max(1, ctx->num_sms * TR_CTAS_PER_SM / p.y)));
-  // Contexts of at most TR_WHOLE_TILES tiles are not cut where there are CTAs for all of them: the second kernel takes as long as walking so many.
+  // Contexts of at most TR_WHOLE_TILES tiles are not cut where there are CTAs for all of them.  (By the tables' width: the lengths are on the device.)
   p.whole = max_len <= TR_WHOLE_TILES * TR_KEYS && n_seqs > 0 && static_cast<int64_t>(n_seqs) * nkv * p.y <= ctx->num_sms * TR_CTAS_PER_SM;
   if (p.whole) p.x = n_seqs * nkv;
   p.slot_bytes = static_cast<int64_t>(head_dim == 128 ? Tree<128>::SLOT : Tree<64>::SLOT) * sizeof(float);

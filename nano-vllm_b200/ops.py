@@ -281,7 +281,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     """Attention of a tree of drafted tokens per sequence, q [tokens, nq, head_dim], over the paged cache, which holds the trees' keys and
     values already: the last tokens of each context, in the nodes' order.  Every node sees what is before the tree, and of the tree the nodes
     whose bit is set in its row of tree_mask (int64 [tokens, words], bit k % 64 of word k / 64 for node k, itself included).  What a node
-    does not see may hold anything; a node that sees nothing and tokens behind the last sequence come back as zeros.  Shapes that the kernel
+    does not see may hold anything; a node that sees nothing and tokens behind the last sequence come back as zeros.  max_seqlen_q: the most nodes of a
+    sequence; the work is dealt by it, so that a bound far above costs time.  Shapes that the kernel
     does not serve (head_dim other than 64 and 128, blocks that are no multiple of 16 tokens) raise.  Forward only."""
     return _native.tree_attention(get_runtime().handle, q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, tree_mask, max_seqlen_q, scale)
 
