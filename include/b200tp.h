@@ -533,6 +533,44 @@ typedef struct b2_logit_rules {
                       history_width + 64 mask_words < 2^19 (an error otherwise) */
 int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, int fp32, int rows, int vocab, const b2_logit_rules* rules, void* stream);
 
+/* ---- beam search: the best continuations of each request, over its beams and the vocabulary (no counterpart in the reference, whose sampler
+ *      draws one token per row, nanovllm/layers/sampler.py:7-12) ------------------------------------------
+ * Request r's beam b has row r * beams + b of logits [n * beams, vocab] (bf16, or fp32 where fp32 is 1; row stride ld) and the score
+ * scores[r, b].  Continuing it with token v gives scores[r, b] + logits[v] - log sum_u exp(logits[u]); outputs [n, picks]: the best of the beams * vocab
+ * continuations, best first, of equal ones the lowest beam, then the lowest token.  The scores are formed in 64 bits where two continuations are near each other and rounded once.
+ * A beam whose score is -inf or NaN has no continuation.  A beam with finished (NULL: none) set has one: itself, with its score and token -1.  A logit of -inf or NaN is no continuation;
+ * +inf counts as the type's largest number.  Places for which there are no continuations: score -inf, parent -1, token -1, not finished.
+ * finished_out: the parent is finished or the token is eos_token (-1: none).
+ * beams <= 32, picks <= 64, n * beams <= 2^24.  b2_beam_select_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant;
+ * calls that may run at the same time need one each), or -1 where the shape is not served. */
+int64_t b2_beam_select_workspace(b2_ctx* ctx, int n, int beams, int vocab, int picks, int fp32);
+int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n, int beams, int vocab, const float* scores, const uint8_t* finished, int picks,
+                   int eos_token, float* scores_out, int32_t* parents_out, int64_t* tokens_out, uint8_t* finished_out, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* ---- beam search: tables, cache and token histories follow the beams that were selected (no counterpart in the reference, whose
+ *      block manager shares whole prompt blocks only, on the host) ------------------------------------------
+ * Row r * beams + b becomes a child of row r * beams + parents[r, b]; with a parent outside 0 .. beams - 1 it gets no tokens and no blocks.  Rows have
+ * context_lens tokens in the cache, in the blocks of block_tables [n * beams, bt_width] (row stride bt_stride).  Rows of a request may have a block in common, in
+ * the same column; two requests may not, but for the first first_blocks[r] columns (NULL: none), which are not given back.
+ *   tables_out [n * beams, bt_width]: the parent's blocks, -1 behind them.  A block with room left (the last of a length that is no multiple
+ *     of block_size) stays with the first row that has it; the others get a block from the stack free_blocks[num_free] and a copy of its tokens.
+ *   free_blocks is updated in place: blocks of columns from first_blocks[r] (but at most the row's full blocks) on that no row has any more are put on the
+ *     stack, ordered by request, column and row, and then the copies take theirs from the top, ordered by request and row; num_free_out: the new height.
+ *   lens_out: the parent's length.  A row for which there is no block has -1 in its place and loses the tokens in it (its length ends with its full blocks).
+ *   cache: planes (layers, keys and values) of [num_blocks, block_size] tokens of token_bytes bytes, plane_bytes apart; 16-byte aligned, a multiple of 16 bytes each.
+ *   history (NULL: none) [n * beams, history_width] int64 with row stride history_stride, of which history_lens count: history_out is the parent's, then the row's
+ *     token of tokens [n * beams] (NULL: none; negative: none) where there is room, then -1.
+ * Lengths that are negative or more than bt_width * block_size count as 0, block numbers outside the cache as none.  No output may overlap an input but free_blocks.  The
+ * inputs but free_blocks and the cache are not changed, and places of the stack below num_free neither, so that the same call again gives the same results.
+ * beams <= 32, n * beams <= 8192, n * beams * bt_width * block_size < 2^31.  b2_reorder_beams_workspace: bytes of device memory (16-byte aligned), or -1. */
+int64_t b2_reorder_beams_workspace(int n, int beams, int bt_width);
+int b2_reorder_beams(b2_ctx* ctx, const int32_t* parents, int n, int beams, const int32_t* block_tables, int64_t bt_stride, int bt_width, const int32_t* context_lens,
+                     const int32_t* first_blocks, int32_t* free_blocks, int free_capacity, const int32_t* num_free, int block_size, void* cache, int planes,
+                     int64_t plane_bytes, int num_blocks, int64_t token_bytes, const int64_t* history, int64_t history_stride, int history_width,
+                     const int32_t* history_lens, const int64_t* tokens, int32_t* tables_out, int32_t* lens_out, int32_t* num_free_out, int64_t* history_out,
+                     int32_t* history_lens_out, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Greedy pick: out[i] = argmax_j logits[i, j] (first index on ties), int64.
  * The reference's Sampler (nanovllm/layers/sampler.py:7-12) at temperature -> 0. */
 int b2_argmax(const void* logits, int64_t ld, int B, int V, int64_t* out, void* stream);

@@ -105,6 +105,10 @@ SIGNATURES = {
     "b2_tree_attention_supported": [_i, _i, _i, _i],
     "b2_tree_attention_workspace": [_p, _i, _i, _i, _i, _i, _i, _i],
     "b2_adjust_logits": [_p, _i64, _p, _i64, _i, _i, _i, C.POINTER(LogitRules), _p],
+    "b2_beam_select": [_p, _p, _i64, _i, _i, _i, _i, _p, _p, _i, _i, _p, _p, _p, _p, _p, _i64, _p],
+    "b2_beam_select_workspace": [_p, _i, _i, _i, _i, _i],
+    "b2_reorder_beams": [_p, _p, _i, _i, _p, _i64, _i, _p, _p, _p, _i, _p, _i, _p, _i, _i64, _i, _i64, _p, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
+    "b2_reorder_beams_workspace": [_i, _i, _i],
     "b2_argmax": [_p, _i64, _i, _i, _p, _p],
     "b2_broadcast_tokens": [_p, _p, _i, _p],
     "b2_batch_inputs": [_p, _i64, _i, _p, _p, _i, _p, _i, _p, _i, _i64, _i, _p, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _p],
@@ -129,7 +133,8 @@ for _name, _args in SIGNATURES.items():
     _fn.restype = _i
 lib.b2_last_error.restype = C.c_char_p
 lib.b2_last_error.argtypes = []
-lib.b2_launch_count.restype = lib.b2_decode_stack_workspace.restype = lib.b2_tree_attention_workspace.restype = _i64
+for _name in ("b2_launch_count", "b2_decode_stack_workspace", "b2_tree_attention_workspace", "b2_beam_select_workspace", "b2_reorder_beams_workspace"):
+    getattr(lib, _name).restype = _i64
 lib.b2_launch_count.argtypes = []
 
 EXPORTED = list(SIGNATURES) + ["b2_last_error", "b2_launch_count"]

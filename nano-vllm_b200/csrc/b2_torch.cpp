@@ -702,6 +702,147 @@ PyObject* adjust_logits(Args a) {
   return wrap(out);
 }
 
+// ---- beam search ---------------------------------------------------------------
+// [rows, cols] of one allocation, as vector_in
+at::Tensor matrix_in(const at::Tensor& base, int64_t offset_bytes, int64_t rows, int64_t cols, at::ScalarType type) {
+  at::Tensor t = vector_in(base, offset_bytes, rows * cols, type);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({rows, cols});
+  return t;
+}
+void matrix_of(const at::Tensor& t, at::ScalarType type, int64_t rows, int64_t cols, const char* what) {
+  if (t.scalar_type() != type) raise(PyExc_TypeError, "%s: expected %s, got %s", what, c10::toString(type), c10::toString(t.scalar_type()));
+  if (t.dim() != 2 || t.size(0) != rows || t.size(1) != cols)
+    raise(PyExc_ValueError, "%s: expected [%lld, %lld], got %lld elements in %lld dimensions", what, (long long)rows, (long long)cols, (long long)t.numel(), (long long)t.dim());
+  if (!t.is_contiguous()) raise(PyExc_AssertionError, "%s must be contiguous", what);
+}
+
+// beam_select(ctx, logits, scores, picks, finished, eos_token): (scores, parents, tokens, finished)
+PyObject* beam_select(Args a) {
+  at::Tensor x = tensor(a[1], "logits");
+  const at::Tensor& scores = tensor(a[2], "scores");
+  const at::Tensor finished = optional_tensor(a[4], "finished");
+  if (scores.dim() != 2) raise(PyExc_ValueError, "scores: expected [requests, beams], got %lld dimensions", (long long)scores.dim());
+  const int64_t n = scores.size(0), beams = scores.size(1), picks = integer(a[3]), eos = integer(a[5]);
+  matrix_of(scores, at::kFloat, n, beams, "scores");
+  if (x.dim() != 2) raise(PyExc_ValueError, "logits: expected [rows, vocabulary], got %lld dimensions", (long long)x.dim());
+  if (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat) raise(PyExc_TypeError, "logits: expected bf16 or fp32, got %s", c10::toString(x.scalar_type()));
+  const int64_t vocab = x.size(1);
+  if (beams < 1 || beams > 32 || picks < 1 || picks > 64 || n > (1 << 24) / beams || vocab < 1 || vocab > 1 << 30)
+    raise(PyExc_ValueError, "beam_select: %lld requests of %lld beams, %lld picks of %lld tokens: 1 to 32 beams and 1 to 64 picks", (long long)n, (long long)beams, (long long)picks, (long long)vocab);
+  if (x.size(0) != n * beams) raise(PyExc_ValueError, "logits: %lld rows for %lld requests of %lld beams", (long long)x.size(0), (long long)n, (long long)beams);
+  if (finished.defined()) matrix_of(finished, at::kBool, n, beams, "finished");
+  if (eos < -1 || eos > 1 << 30) raise(PyExc_ValueError, "eos_token: %lld", (long long)eos);
+  forward_only({&x, &scores}, "beam_select");
+  on_current_gpu(x, "logits");
+  beside(scores, x, "scores");
+  beside(finished, x, "finished");
+  if ((vocab > 1 && x.stride(1) != 1) || (x.size(0) > 1 && x.stride(0) < vocab)) x = x.contiguous();
+  const int64_t many = n * picks, at_scores = many * 8, at_parents = at_scores + many * 4, at_ended = at_parents + many * 4;
+  const at::Tensor base = at::detail::empty_cuda({at_ended + many}, at::kByte, x.device(), std::nullopt);
+  const at::Tensor tokens = matrix_in(base, 0, n, picks, at::kLong), out = matrix_in(base, at_scores, n, picks, at::kFloat), parents = matrix_in(base, at_parents, n, picks, at::kInt),
+                   ended = matrix_in(base, at_ended, n, picks, at::kBool);
+  if (n > 0) {
+    b2_ctx* const ctx = context(a[0]);
+    const bool fp32 = x.scalar_type() == at::kFloat;
+    const int64_t bytes = b2_beam_select_workspace(ctx, n, beams, vocab, picks, fp32);
+    if (bytes < 0) check(B2_ERR_UNSUPPORTED, "b2_beam_select_workspace");
+    const at::Tensor ws = at::detail::empty_cuda({bytes}, at::kByte, x.device(), std::nullopt);
+    launch("b2_beam_select", b2_beam_select, ctx, x.const_data_ptr(), row_stride(x), int(fp32), n, beams, vocab, scores.const_data_ptr<float>(),
+           finished.defined() ? static_cast<const uint8_t*>(finished.const_data_ptr()) : nullptr, picks, eos, out.mutable_data_ptr<float>(), parents.mutable_data_ptr<int32_t>(),
+           tokens.mutable_data_ptr<int64_t>(), static_cast<uint8_t*>(ended.data_ptr()), ws.data_ptr(), bytes, stream());
+  }
+  PyObject* p = PyTuple_New(4);
+  if (p == nullptr) throw Raised{};
+  PyTuple_SET_ITEM(p, 0, wrap(out));
+  PyTuple_SET_ITEM(p, 1, wrap(parents));
+  PyTuple_SET_ITEM(p, 2, wrap(tokens));
+  PyTuple_SET_ITEM(p, 3, wrap(ended));
+  return p;
+}
+
+// reorder_beams(ctx, parents, block_tables, context_lens, free_blocks, num_free, kv_cache, first_blocks, history, history_lens, tokens):
+// (block_tables, context_lens, num_free, history or None, history_lens or None)
+PyObject* reorder_beams(Args a) {
+  const at::Tensor &parents = tensor(a[1], "parents"), &tables = tensor(a[2], "block_tables"), &lens = tensor(a[3], "context_lens"), &free = tensor(a[4], "free_blocks"),
+                   &num_free = tensor(a[5], "num_free"), &cache = tensor(a[6], "kv_cache");
+  const at::Tensor first = optional_tensor(a[7], "first_blocks"), history = optional_tensor(a[8], "history"), history_lens = optional_tensor(a[9], "history_lens"),
+                   tokens = optional_tensor(a[10], "tokens");
+  if (parents.dim() != 2) raise(PyExc_ValueError, "parents: expected [requests, beams], got %lld dimensions", (long long)parents.dim());
+  const int64_t n = parents.size(0), beams = parents.size(1), rows = n * beams;
+  matrix_of(parents, at::kInt, n, beams, "parents");
+  if (beams < 1 || beams > 32 || rows > 8192) raise(PyExc_ValueError, "reorder_beams: %lld requests of %lld beams: 1 to 32 beams, at most 8192 rows", (long long)n, (long long)beams);
+  row_matrix(tables, at::kInt, rows, rows > 0 ? 1 : 0, "block_tables");
+  const int64_t width = tables.size(1);
+  if (rows > 1 && tables.stride(0) < width) raise(PyExc_AssertionError, "block_tables: rows must not overlap");
+  vector_of(lens, at::kInt, rows, "context_lens");
+  vector_of(free, at::kInt, free.numel(), "free_blocks");
+  vector_of(num_free, at::kInt, 1, "num_free");
+  if (first.defined()) vector_of(first, at::kInt, n, "first_blocks");
+  if (cache.dim() < 4) raise(PyExc_ValueError, "kv_cache: expected [..., blocks, block_size, KV heads, head_dim], got %lld dimensions", (long long)cache.dim());
+  const int64_t d = cache.dim(), blocks = cache.size(d - 4), bs = cache.size(d - 3), token_bytes = cache.size(d - 2) * cache.size(d - 1) * cache.element_size();
+  int64_t planes = 1, step = 1, plane_step = 0;  // (a dimension of one element may have any stride)
+  bool dense = true;
+  for (int64_t i = d - 1; i >= 0; --i) {
+    if (i >= d - 4) {
+      dense = dense && (cache.size(i) == 1 || cache.stride(i) == step);
+      step *= cache.size(i);
+    } else {
+      if (cache.size(i) != 1) {
+        if (plane_step == 0) plane_step = cache.stride(i);
+        else dense = dense && cache.stride(i) == plane_step * planes;
+      }
+      planes *= cache.size(i);
+    }
+  }
+  if (blocks < 1 || bs < 1 || token_bytes < 1) raise(PyExc_ValueError, "kv_cache: an empty cache");
+  if (planes > 0 && (!dense || plane_step < 0 || (planes > 1 && plane_step < step))) raise(PyExc_AssertionError, "kv_cache: layers must be contiguous and equally far apart");
+  const int64_t plane_bytes = plane_step * static_cast<int64_t>(cache.element_size());
+  if (token_bytes % 16 != 0 || (planes > 1 && plane_bytes % 16 != 0) || !on_16_bytes(cache)) raise(PyExc_AssertionError, "kv_cache: tokens must lie on 16-byte boundaries");
+  constexpr int64_t limit = (int64_t(1) << 31) - 1;
+  if (blocks > limit / bs || token_bytes > limit / bs || width > limit / bs / std::max<int64_t>(rows, 1) || rows * width + free.numel() > limit || planes > 65536 ||
+      planes * ((bs * token_bytes + 4095) / 4096) > limit)
+    raise(PyExc_ValueError, "reorder_beams: %lld rows of %lld blocks, a cache of %lld blocks of %lld tokens", (long long)rows, (long long)width, (long long)blocks, (long long)bs);
+  if (history.defined() != history_lens.defined() || (tokens.defined() && !history.defined())) raise(PyExc_ValueError, "history, its history_lens and tokens belong together");
+  if (history.defined()) {
+    row_matrix(history, at::kLong, rows, 0, "history");
+    if (history.size(1) > limit / std::max<int64_t>(rows, 1)) raise(PyExc_ValueError, "history: %lld rows of %lld", (long long)rows, (long long)history.size(1));
+    if (rows > 1 && history.stride(0) < history.size(1)) raise(PyExc_AssertionError, "history: rows must not overlap");
+    vector_of(history_lens, at::kInt, rows, "history_lens");
+    if (tokens.defined()) matrix_of(tokens, at::kLong, n, beams, "tokens");
+  }
+  const std::pair<const at::Tensor*, const char*> named[] = {{&free, "free_blocks"}, {&cache, "kv_cache"}, {&parents, "parents"}, {&tables, "block_tables"}, {&lens, "context_lens"},
+                                                             {&num_free, "num_free"}, {&first, "first_blocks"}, {&history, "history"}, {&history_lens, "history_lens"}, {&tokens, "tokens"}};
+  for (int i = 0; i < 2; ++i)
+    for (int k = i + 1; k < 10; ++k)
+      if (named[k].first->defined() && overlap(*named[i].first, *named[k].first)) raise(PyExc_ValueError, "%s, which is written, overlaps %s", named[i].second, named[k].second);
+  forward_only({&cache}, "reorder_beams");
+  on_current_gpu(parents, "parents");
+  for (const auto& t : named) beside(*t.first, parents, t.second);
+  const at::Tensor out = at::detail::empty_cuda({rows, width}, at::kInt, parents.device(), std::nullopt);
+  const int64_t lens_bytes = (rows * 4 + 15) / 16 * 16;
+  const at::Tensor base = at::detail::empty_cuda({2 * lens_bytes + 16}, at::kByte, parents.device(), std::nullopt);
+  const at::Tensor lens_out = vector_in(base, 0, rows, at::kInt), said = vector_in(base, lens_bytes, rows, at::kInt), left = vector_in(base, 2 * lens_bytes, 1, at::kInt);
+  at::Tensor text;
+  if (history.defined()) text = at::detail::empty_cuda({rows, history.size(1)}, at::kLong, parents.device(), std::nullopt);
+  const int64_t bytes = b2_reorder_beams_workspace(n, beams, width);
+  if (bytes < 0) check(B2_ERR_UNSUPPORTED, "b2_reorder_beams_workspace");
+  const at::Tensor ws = at::detail::empty_cuda({bytes}, at::kByte, parents.device(), std::nullopt);
+  launch("b2_reorder_beams", b2_reorder_beams, context(a[0]), parents.const_data_ptr<int32_t>(), n, beams, tables.const_data_ptr<int32_t>(), row_stride(tables), width,
+         lens.const_data_ptr<int32_t>(), cptr<int32_t>(first), free.mutable_data_ptr<int32_t>(), free.numel(), num_free.const_data_ptr<int32_t>(), bs, planes > 0 ? cache.data_ptr() : nullptr,
+         planes, plane_bytes, blocks, token_bytes, cptr<int64_t>(history), history.defined() ? row_stride(history) : 0, history.defined() ? history.size(1) : 0,
+         cptr<int32_t>(history_lens), cptr<int64_t>(tokens), out.mutable_data_ptr<int32_t>(), lens_out.mutable_data_ptr<int32_t>(), left.mutable_data_ptr<int32_t>(),
+         static_cast<int64_t*>(ptr(text)), history.defined() ? said.mutable_data_ptr<int32_t>() : nullptr, ws.data_ptr(), bytes, stream());
+  PyObject* p = PyTuple_New(5);
+  if (p == nullptr) throw Raised{};
+  PyTuple_SET_ITEM(p, 0, wrap(out));
+  PyTuple_SET_ITEM(p, 1, wrap(lens_out));
+  PyTuple_SET_ITEM(p, 2, wrap(left));
+  auto or_none = [&](const at::Tensor& t) { return history.defined() ? wrap(t) : Py_NewRef(Py_None); };
+  PyTuple_SET_ITEM(p, 3, or_none(text));
+  PyTuple_SET_ITEM(p, 4, or_none(said));
+  return p;
+}
+
 PyObject* init(Args a) {
   Py_INCREF(a[0]);
   Py_XDECREF(g_check);
@@ -728,7 +869,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {B2_ENTRY(init, 1), B2_ENTRY(gemm, 4), B2_ENTRY(gemm_silu_mul, 3), B2_ENTRY(qkv_fused, 15), B2_ENTRY(rowpar_fused, 7),
                          B2_ENTRY(rmsnorm, 3), B2_ENTRY(add_rmsnorm, 4), B2_ENTRY(silu_and_mul, 1), B2_ENTRY(store_kvcache, 5),
                          B2_ENTRY(qk_norm_rope_store, 12), B2_ENTRY(rope, 5), B2_ENTRY(embed, 5), B2_ENTRY(paged_attention, 7), B2_ENTRY(prefill_attention, 9),
-                         B2_ENTRY(decode_stack, 16), B2_ENTRY(batch_inputs, 9), B2_ENTRY(tree_attention, 10), B2_ENTRY(adjust_logits, 14), {nullptr, nullptr, 0, nullptr}};
+                         B2_ENTRY(decode_stack, 16), B2_ENTRY(batch_inputs, 9), B2_ENTRY(tree_attention, 10), B2_ENTRY(adjust_logits, 14), B2_ENTRY(beam_select, 6),
+                         B2_ENTRY(reorder_beams, 11), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_b2torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

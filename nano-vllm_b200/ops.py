@@ -303,3 +303,43 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     and behind the last are copied); with draft_tokens int64 [rows] and tree_mask (as for tree_attention) the drafted tokens that a row's node sees count as its output."""
     return _native.adjust_logits(logits, history, history_lens, prompt_lens, repetition_penalty, presence_penalty, frequency_penalty, bias_ids, bias_values, allowed_mask,
                                  cu_seqlens, draft_tokens, tree_mask, out)
+
+
+class BeamPicks(NamedTuple):
+    """The continuations that a step of beam search goes on with (see beam_select)."""
+    scores: torch.Tensor    # fp32 [n, picks], best first; -inf where there are no more
+    parents: torch.Tensor   # int32 [n, picks]: the beam that is continued; -1
+    tokens: torch.Tensor    # int64 [n, picks]; -1 for a beam that is finished
+    finished: torch.Tensor  # bool [n, picks]
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, picks: int | None = None, *, finished: torch.Tensor | None = None, eos_token: int | None = None) -> BeamPicks:
+    """The best continuations of n requests of some beams each: scores fp32 [n, beams] are the beams' sums of log-probabilities, logits [n * beams, vocab]
+    (bf16 or fp32) their rows.  Continuing beam b with token v scores scores[b] + log_softmax(logits[b])[v]; the `picks` (as many as beams where None)
+    best of all beams and tokens come back, best first, of equal ones the lowest beam, then the lowest token.  A beam with a score of -inf
+    has no continuations, one that is finished (bool [n, beams]) has itself, as it is, with token -1.  The result's finished: the parent is, or the token is
+    eos_token.  Tokens with a logit of -inf are not continued with; places for which there are no continuations have the score -inf and parent -1.
+    At most 32 beams and 64 picks.  The rules in full are at b2_beam_select.  Forward only."""
+    return BeamPicks(*_native.beam_select(get_runtime().handle, logits, scores, scores.shape[-1] if picks is None else picks, finished, -1 if eos_token is None else eos_token))
+
+
+class BeamState(NamedTuple):
+    """Rows of beams after a step's selection (see reorder_beams)."""
+    block_tables: torch.Tensor         # int32 [n * beams, width]; -1 behind a row's blocks
+    context_lens: torch.Tensor         # int32 [n * beams]
+    num_free: torch.Tensor             # int32 [1]
+    history: torch.Tensor | None       # int64 [n * beams, history width]; -1 behind a row's tokens
+    history_lens: torch.Tensor | None  # int32 [n * beams]
+
+
+def reorder_beams(parents: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, free_blocks: torch.Tensor, num_free: torch.Tensor, kv_cache: torch.Tensor, *,
+                  first_blocks: torch.Tensor | None = None, history: torch.Tensor | None = None, history_lens: torch.Tensor | None = None,
+                  tokens: torch.Tensor | None = None) -> BeamState:
+    """Rows of n requests of some beams each become children of the rows that parents int32 [n, beams] names (-1: an empty row): block_tables [n * beams, width]
+    with context_lens tokens in the cache, and the token histories [n * beams, width] with history_lens tokens, to which tokens int64 [n, beams] (beam_select's; negative:
+    none) is appended.  Full blocks are shared by all children.  A block with room left stays with its first child; the others get a copy, in
+    kv_cache [..., blocks, block_size, KV heads, head_dim] (all layers' keys and values), in a block from the stack free_blocks[:num_free].  Blocks that no row has any more go
+    onto the stack; the first first_blocks[r] columns of request r's tables (a prompt's full blocks, whose owner is the caller) do not.  free_blocks and kv_cache are updated
+    in place, the rest comes back new.  Rows of a request may share blocks in the same column, different requests only the first_blocks.  A row for which there is no block
+    loses the tokens in its last one: context_lens says so.  At most 32 beams.  The rules in full are at b2_reorder_beams."""
+    return BeamState(*_native.reorder_beams(get_runtime().handle, parents, block_tables, context_lens, free_blocks, num_free, kv_cache, first_blocks, history, history_lens, tokens))
