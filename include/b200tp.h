@@ -501,6 +501,24 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
                       const int64_t* tree_mask, int64_t mask_stride, int mask_words, int n_seqs, int max_q, int tokens, int nq, int nkv,
                       int head_dim, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- decode attention for sequences that share the beginning of their contexts: beams of a request, requests behind one prompt (no
+ *      counterpart in the reference, which walks every context for itself, nanovllm/layers/attention.py:70-74) --
+ * q [n_seqs, nq, head_dim] bf16 (row stride q_stride), one query token per sequence; group g has the sequences cu_groups[g] .. cu_groups[g+1], whose first
+ * prefix_lens[g] tokens are in the same blocks: their tables agree there (which of them is read is not said).  A sequence without a group sees nothing.
+ *   out = softmax(scale q K^T) V over the sequence's first context_lens tokens, [n_seqs, nq, head_dim] contiguous, fp32 scores and sums
+ * What lies behind a context may hold anything; a sequence without tokens (0: a padded one) comes back as zeros and may have any table.  A context that is shorter than the
+ * prefix shortens it for its group.  max_group: the most sequences of a group; the work is dealt by it, and any number gives the same result within rounding.  scale: of either sign, or zero.
+ * The sums are kept unnormalised with weights of up to 2^8: 256 * the keys seen * the largest |value| has to stay below the type's maximum (3.4e38).
+ * Lengths and tables are read after earlier kernels have completed.  Calls that may run at the same time need a workspace each (16-byte aligned, contents irrelevant).
+ * b2_prefix_attention_supported says (1 / 0) whether the shape is served: head_dim 64 or 128, up to 128 query heads per KV head, blocks of
+ * a multiple of 16 tokens.  b2_prefix_attention_workspace: bytes, or -1 where the shape is not served; at most 1024 sequences and groups, tables of less than 2^27 tokens. */
+int b2_prefix_attention_supported(int nq, int nkv, int head_dim, int block_size);
+int64_t b2_prefix_attention_workspace(b2_ctx* ctx, int n_seqs, int n_groups, int nq, int nkv, int head_dim, int block_size, int bt_width);
+int b2_prefix_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int num_blocks, int block_size,
+                        const int32_t* block_tables, int64_t bt_stride, int bt_width, const int32_t* cu_groups, const int32_t* prefix_lens,
+                        const int32_t* context_lens, int n_groups, int max_group, int n_seqs, int nq, int nkv, int head_dim, float scale, void* out,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- rules on logits, between b2_lm_head and the sampler (no counterpart in the reference, whose sampler takes the logits as they
  *      are, nanovllm/layers/sampler.py:7-12) ------------------------------------------
  * For row i of logits [rows, vocab] (bf16, or fp32 where fp32 is 1), its request s and token v, in 32 bits and in this order:

@@ -104,6 +104,9 @@ SIGNATURES = {
     "b2_tree_attention": [_p, _p, _i64, _p, _p, _i, _i, _p, _i64, _i, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _i, _f, _p, _p, _i64, _p],
     "b2_tree_attention_supported": [_i, _i, _i, _i],
     "b2_tree_attention_workspace": [_p, _i, _i, _i, _i, _i, _i, _i],
+    "b2_prefix_attention": [_p, _p, _i64, _p, _p, _i, _i, _p, _i64, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _p, _p, _i64, _p],
+    "b2_prefix_attention_supported": [_i, _i, _i, _i],
+    "b2_prefix_attention_workspace": [_p, _i, _i, _i, _i, _i, _i, _i],
     "b2_adjust_logits": [_p, _i64, _p, _i64, _i, _i, _i, C.POINTER(LogitRules), _p],
     "b2_beam_select": [_p, _p, _i64, _i, _i, _i, _i, _p, _p, _i, _i, _p, _p, _p, _p, _p, _i64, _p],
     "b2_beam_select_workspace": [_p, _i, _i, _i, _i, _i],
@@ -133,7 +136,7 @@ for _name, _args in SIGNATURES.items():
     _fn.restype = _i
 lib.b2_last_error.restype = C.c_char_p
 lib.b2_last_error.argtypes = []
-for _name in ("b2_launch_count", "b2_decode_stack_workspace", "b2_tree_attention_workspace", "b2_beam_select_workspace", "b2_reorder_beams_workspace"):
+for _name in ("b2_launch_count", "b2_decode_stack_workspace", "b2_tree_attention_workspace", "b2_prefix_attention_workspace", "b2_beam_select_workspace", "b2_reorder_beams_workspace"):
     getattr(lib, _name).restype = _i64
 lib.b2_launch_count.argtypes = []
 

@@ -702,6 +702,50 @@ PyObject* adjust_logits(Args a) {
   return wrap(out);
 }
 
+// shared_prefix_attention(ctx, q, k_cache, v_cache, cu_groups, prefix_lens, context_lens, block_tables, max_group, scale)
+PyObject* shared_prefix_attention(Args a) {
+  const at::Tensor &q = tensor(a[1], "q"), &kc = tensor(a[2], "k_cache"), &vc = tensor(a[3], "v_cache"), &cu = tensor(a[4], "cu_groups"), &prefix = tensor(a[5], "prefix_lens"),
+                   &lens = tensor(a[6], "context_lens"), &tables = tensor(a[7], "block_tables");
+  const int64_t max_group = integer(a[8]);
+  if (q.dim() != 3 || kc.dim() != 4) raise(PyExc_ValueError, "shared_prefix_attention: q of 3 and caches of 4 dimensions, got %lld and %lld", (long long)q.dim(), (long long)kc.dim());
+  const int64_t n = q.size(0), nq = q.size(1), hd = q.size(2), nkv = kc.size(2), bs = kc.size(1), groups = prefix.numel();
+  if (q.scalar_type() != at::kBFloat16) raise(PyExc_TypeError, "q: expected bf16, got %s", c10::toString(q.scalar_type()));
+  values_like_keys(kc, vc, hd);
+  if (nq > 8192 || bs > 1 << 20 || !b2_prefix_attention_supported(nq, nkv, hd, bs))
+    raise(PyExc_ValueError,
+          "shared_prefix_attention: %lld query and %lld KV heads of %lld, blocks of %lld tokens: head dimension 64 or 128, at most 128 query heads per KV head, blocks of a multiple of 16",
+          (long long)nq, (long long)nkv, (long long)hd, (long long)bs);
+  if (!row_layout(q, nq, hd)) raise(PyExc_AssertionError, "q: heads must lie side by side, in rows on 16-byte boundaries");
+  if (!kc.is_contiguous() || !vc.is_contiguous() || !on_16_bytes(kc) || !on_16_bytes(vc)) raise(PyExc_AssertionError, "k_cache and v_cache must be contiguous, on 16-byte boundaries");
+  constexpr int64_t limit = (int64_t(1) << 31) - 1;
+  if (kc.size(0) < 1 || kc.size(0) > limit / bs || tables.dim() != 2 || tables.size(1) > ((1 << 27) - 1) / bs || n > 1024 || groups > 1024)
+    raise(PyExc_ValueError, "shared_prefix_attention: %lld blocks, %lld sequences in %lld groups: at most 1024 of both, tables of less than 2^27 tokens", (long long)kc.size(0), (long long)n, (long long)groups);
+  vector_of(prefix, at::kInt, groups, "prefix_lens");
+  vector_of(cu, at::kInt, groups + 1, "cu_groups");
+  vector_of(lens, at::kInt, n, "context_lens");
+  row_matrix(tables, at::kInt, n, n > 0 ? 1 : 0, "block_tables");
+  if (n > 1 && tables.stride(0) < tables.size(1)) raise(PyExc_AssertionError, "block_tables: rows must not overlap");
+  if (max_group < 0 || (n > 0 && groups > 0 && max_group < 1)) raise(PyExc_ValueError, "shared_prefix_attention: max_group %lld", (long long)max_group);
+  forward_only({&q, &kc, &vc}, "shared_prefix_attention");
+  on_current_gpu(q, "q");
+  beside(kc, q, "k_cache");
+  beside(vc, q, "v_cache");
+  beside(cu, q, "cu_groups");
+  beside(prefix, q, "prefix_lens");
+  beside(lens, q, "context_lens");
+  beside(tables, q, "block_tables");
+  const at::Tensor out = at::detail::empty_cuda({n, nq, hd}, at::kBFloat16, q.device(), std::nullopt);
+  if (n == 0) return wrap(out);
+  b2_ctx* const ctx = context(a[0]);
+  const int64_t bytes = b2_prefix_attention_workspace(ctx, n, groups, nq, nkv, hd, bs, tables.size(1));
+  if (bytes < 0) check(B2_ERR_UNSUPPORTED, "b2_prefix_attention_workspace");
+  const at::Tensor ws = at::detail::empty_cuda({bytes}, at::kByte, q.device(), std::nullopt);
+  launch("b2_prefix_attention", b2_prefix_attention, ctx, q.data_ptr(), n > 1 ? q.stride(0) : nq * hd, kc.data_ptr(), vc.data_ptr(), kc.size(0), bs, tables.const_data_ptr<int32_t>(),
+         row_stride(tables), tables.size(1), cu.const_data_ptr<int32_t>(), prefix.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(), groups, std::min<int64_t>(max_group, n), n, nq, nkv,
+         hd, number(a[9]), out.data_ptr(), ws.data_ptr(), bytes, stream());
+  return wrap(out);
+}
+
 // ---- beam search ---------------------------------------------------------------
 // [rows, cols] of one allocation, as vector_in
 at::Tensor matrix_in(const at::Tensor& base, int64_t offset_bytes, int64_t rows, int64_t cols, at::ScalarType type) {
@@ -870,7 +914,7 @@ PyMethodDef methods[] = {B2_ENTRY(init, 1), B2_ENTRY(gemm, 4), B2_ENTRY(gemm_sil
                          B2_ENTRY(rmsnorm, 3), B2_ENTRY(add_rmsnorm, 4), B2_ENTRY(silu_and_mul, 1), B2_ENTRY(store_kvcache, 5),
                          B2_ENTRY(qk_norm_rope_store, 12), B2_ENTRY(rope, 5), B2_ENTRY(embed, 5), B2_ENTRY(paged_attention, 7), B2_ENTRY(prefill_attention, 9),
                          B2_ENTRY(decode_stack, 16), B2_ENTRY(batch_inputs, 9), B2_ENTRY(tree_attention, 10), B2_ENTRY(adjust_logits, 14), B2_ENTRY(beam_select, 6),
-                         B2_ENTRY(reorder_beams, 11), {nullptr, nullptr, 0, nullptr}};
+                         B2_ENTRY(shared_prefix_attention, 10), B2_ENTRY(reorder_beams, 11), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_b2torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -287,6 +287,16 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     return _native.tree_attention(get_runtime().handle, q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, tree_mask, max_seqlen_q, scale)
 
 
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_groups: torch.Tensor, prefix_lens: torch.Tensor, context_lens: torch.Tensor,
+                            block_tables: torch.Tensor, max_group: int, scale: float) -> torch.Tensor:
+    """Decode attention, one query token per sequence, q [n, nq, head_dim], over the paged cache, for sequences that share the beginning of their contexts (the beams of a
+    request, requests behind one prompt): group g has the sequences cu_groups[g] .. cu_groups[g + 1] (int32 [groups + 1]), whose block tables agree in the first
+    prefix_lens[g] tokens.  Those are read once for the group.  The result is that of paged_attention within rounding; sequences without tokens and
+    those of no group come back as zeros.  max_group: the most sequences of a group.  Shapes that the kernel does not serve (head_dim other than 64 and 128, blocks that are no
+    multiple of 16 tokens, more than 1024 sequences) raise.  The rules in full are at b2_prefix_attention.  Forward only."""
+    return _native.shared_prefix_attention(get_runtime().handle, q, k_cache, v_cache, cu_groups, prefix_lens, context_lens, block_tables, max_group, scale)
+
+
 def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, history_lens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
                   repetition_penalty: torch.Tensor | None = None, presence_penalty: torch.Tensor | None = None, frequency_penalty: torch.Tensor | None = None,
                   bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None, allowed_mask: torch.Tensor | None = None,
