@@ -27,8 +27,9 @@ namespace {
 constexpr int BS_THREADS = 256, BS_VECTORS = 4, BS_CTAS_PER_SM = 4;
 constexpr int BS_TILE_BYTES = BS_THREADS * BS_VECTORS * 16;
 constexpr int BS_MAX_PICKS = 64, BS_MAX_BEAMS = 32;
+constexpr int BP_THREADS = 512;
 constexpr int BS_COLLECT = 1024;  // candidates that a request ranks at once
-constexpr double BS_NEAR = 2e-6;
+constexpr double BS_NEAR = 4e-6;
 
 struct ScanArgs {
   const void* logits;
@@ -60,23 +61,37 @@ template <>
 struct Logits<float> {
   static constexpr int N = 4;
   static __device__ __forceinline__ float one(const float* p) { return plain_number(__ldg(p)); }
+  static __device__ __forceinline__ uint32_t clean(uint32_t w) { return __float_as_uint(plain_number(__uint_as_float(w))); }
+  static __device__ __forceinline__ uint4 clean(const uint4& v) { return make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w)); }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
-    f[0] = plain_number(__uint_as_float(v.x));
-    f[1] = plain_number(__uint_as_float(v.y));
-    f[2] = plain_number(__uint_as_float(v.z));
-    f[3] = plain_number(__uint_as_float(v.w));
+    f[0] = __uint_as_float(v.x);
+    f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z);
+    f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
 };
 template <>
 struct Logits<__nv_bfloat16> {
   static constexpr int N = 8;
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return fminf(fmaxf(__bfloat162float(*p), -INFINITY), b2::bf16_hi(0x7f7f0000u)); }
-  static __device__ __forceinline__ uint32_t clean(uint32_t w) {
-    const uint32_t low = 0xff80ff80u, high = 0x7f7f7f7fu;
-    const __nv_bfloat162 v = __hmin2(__hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&low)), *reinterpret_cast<const __nv_bfloat162*>(&high));
+  static __device__ __forceinline__ uint32_t max2(uint32_t x, uint32_t y) {
+    const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) { b2::unpack8(make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w)), f); }
+  static __device__ __forceinline__ uint32_t clean(uint32_t w) {
+    const uint32_t low = max2(w, 0xff80ff80u), high = 0x7f7f7f7fu;
+    const __nv_bfloat162 v = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&low), *reinterpret_cast<const __nv_bfloat162*>(&high));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ uint4 clean(const uint4& v) { return make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w)); }
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) { b2::unpack8(v, f); }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    const uint32_t w = max2(max2(v.x, v.y), max2(v.z, v.w));
+    return fmaxf(b2::bf16_lo(w), b2::bf16_hi(w));
+  }
 };
 
 // The 16 bytes at `chunk` (counted from the 16-byte boundary at or before the row), -inf in the places that are not the row's.
@@ -107,191 +122,192 @@ __device__ __forceinline__ uint4 load_chunk(const T* row, int vocab, int64_t fir
 
 // The list of candidates of a CTA
 struct List {
-  uint64_t* keys;
-  int* count;    // of those that were to go in: may be past the capacity
-  int* tally;    // [64] for the search
+  uint64_t *keys, *best;  // [capacity], [BS_MAX_PICKS]
+  int* count;             // of those that were to go in: may be past the capacity
   int capacity;
   __device__ __forceinline__ void push(uint64_t key) {
     const int at = atomicAdd(count, 1);
     if (at < capacity) keys[at] = key;
   }
-  // All threads: a key that exactly k of the n > k keys reach (the k-th best, or between it and the one behind).
-  __device__ uint64_t kth(int n, int k) {
-    for (int i = threadIdx.x; i < 64; i += BS_THREADS) tally[i] = 0;
+  // All threads: the k best of the n keys stay, in order.  Every thread counts the keys before its own.  Returns how many there are.
+  __device__ int rank(int n, int k) {
+    for (int i = threadIdx.x; i < n; i += BS_THREADS) {
+      const uint64_t mine = keys[i];
+      int before = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) before += keys[j] > mine ? 1 : 0;
+      if (before < k) best[before] = mine;
+    }
     __syncthreads();
-    uint64_t t = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t c = t | (1ull << bit);
-      int mine = 0;
-      for (int i = threadIdx.x; i < n; i += BS_THREADS) mine += keys[i] >= c ? 1 : 0;
-      mine = __reduce_add_sync(0xffffffffu, mine);
-      if ((threadIdx.x & 31) == 0 && mine > 0) atomicAdd(tally + bit, mine);
-      __syncthreads();
-      const int all = tally[bit];
-      if (all >= k) t = c;
-      if (all == k) break;
-    }
-    __syncthreads();  // (the tally has been read)
-    return t;
+    const int left = min(n, k);
+    if (static_cast<int>(threadIdx.x) < left) keys[threadIdx.x] = best[threadIdx.x];
+    if (threadIdx.x == 0) *count = left;
+    __syncthreads();
+    return left;
   }
-  // All threads: the k best of the n keys stay (in no order), where there are more.
-  __device__ uint64_t cut(int n, int k) {
-    const uint64_t t = kth(n, k);
-    if (threadIdx.x == 0) *count = 0;
-    // in steps of the block: what a step writes lies before what later ones read
-    for (int i0 = 0; i0 < n; i0 += BS_THREADS) {
-      const uint64_t mine = i0 + threadIdx.x < n ? keys[i0 + threadIdx.x] : 0;
-      __syncthreads();
-      if (mine >= t && mine != 0) keys[atomicAdd(count, 1)] = mine;
-      __syncthreads();
-    }
-    return t;
+};
+
+// Ranges of `total` tiles: CTA x of X
+struct ScanDeal {
+  int base, rem;
+  __device__ __forceinline__ ScanDeal(int total, int X) : base(total / X), rem(total % X) {}
+  __device__ __forceinline__ int begin_of(int x) const { return x * base + min(x, rem); }
+  __device__ __forceinline__ int cta_of(int t) const {
+    const int big = rem * (base + 1);
+    return t < big ? t / (base + 1) : rem + (t - big) / base;
   }
 };
 
 template <typename T>
 __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(const ScanArgs a) {
-  constexpr int N = Logits<T>::N;
-  extern __shared__ uint64_t s_keys[];
-  __shared__ int s_count, s_tally[64];
-  __shared__ float s_max[BS_THREADS / 32];
+  constexpr int N = Logits<T>::N, TILE = BS_THREADS * BS_VECTORS * N;
+  extern __shared__ __align__(16) uint64_t s_keys[];
+  __shared__ uint64_t s_best[BS_MAX_PICKS];
+  __shared__ int s_count;
+  __shared__ float s_top[BS_THREADS], s_bound, s_max[BS_THREADS / 32];
   __shared__ double s_sum[BS_THREADS / 32];
-  List list{s_keys, &s_count, s_tally, a.capacity};
+  List list{s_keys, s_best, &s_count, a.capacity};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.picks;
-  const int64_t total = static_cast<int64_t>(a.rows) * a.tiles;
-  auto begin_of = [&](int64_t x) { return total * x / gridDim.x; };
-  int64_t u = begin_of(blockIdx.x);
-  const int64_t end = begin_of(blockIdx.x + 1);
+  const ScanDeal deal(a.rows * a.tiles, gridDim.x);
+  int u = deal.begin_of(blockIdx.x);
+  const int end = deal.begin_of(blockIdx.x + 1);
   b2::pdl_launch_dependents();
   b2::pdl_wait();
   while (u < end) {
-    const int row = static_cast<int>(u / a.tiles), t0 = static_cast<int>(u - static_cast<int64_t>(row) * a.tiles), t1 = static_cast<int>(min(static_cast<int64_t>(a.tiles), t0 + end - u));
+    const int row = u / a.tiles, t0 = u - row * a.tiles, t1 = min(a.tiles, t0 + end - u);
     u += t1 - t0;
     if (!(a.scores[row] > -INFINITY) || (a.finished != nullptr && a.finished[row] != 0)) continue;  // (it has one continuation or none)
-    // the CTA that holds the row's first tile is the first of its parts
-    const int64_t first_tile = static_cast<int64_t>(row) * a.tiles;
-    int64_t x0 = first_tile * gridDim.x / total;
-    while (begin_of(x0 + 1) <= first_tile) ++x0;
-    while (begin_of(x0) > first_tile) --x0;
-    const int part = static_cast<int>(blockIdx.x - x0);
+    const int part = blockIdx.x - deal.cta_of(row * a.tiles);  // the CTA that holds the row's first tile is the first of its parts
     const T* p = static_cast<const T*>(a.logits) + row * a.ld;
-    const int64_t shift = (reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T);
-    auto first_of = [&](int tile, int v) { return ((static_cast<int64_t>(tile) * BS_VECTORS + v) * BS_THREADS + tid) * N - shift; };
-    uint4 next[BS_VECTORS];
+    const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));  // tiles begin at the 16-byte boundary before the row
+    const int limit = max(K + 32, min(2 * K + 64, a.capacity / 2));  // candidates at which the list is cut
+    auto load = [&](int tile, uint4 (&v)[BS_VECTORS]) {
+      const int64_t first = static_cast<int64_t>(tile) * TILE - shift;
+      if (first >= 0 && first + TILE <= a.vocab) {
+        const uint4* q = reinterpret_cast<const uint4*>(p + first) + tid;
 #pragma unroll
-    for (int v = 0; v < BS_VECTORS; ++v) next[v] = load_chunk(p, a.vocab, first_of(t0, v));
+        for (int i = 0; i < BS_VECTORS; ++i) v[i] = __ldg(q + i * BS_THREADS);
+      } else {
+#pragma unroll
+        for (int i = 0; i < BS_VECTORS; ++i) v[i] = load_chunk(p, a.vocab, first + (i * BS_THREADS + tid) * N);
+      }
+    };
+    uint4 next[BS_VECTORS];
+    load(t0, next);
     float m = -INFINITY, bound = -INFINITY;
     double sum = 0.0;
-    __syncthreads();
     if (tid == 0) s_count = 0;
-    __syncthreads();
     int count = 0;
     for (int tile = t0; tile < t1; ++tile) {
       uint4 now[BS_VECTORS];
 #pragma unroll
-      for (int v = 0; v < BS_VECTORS; ++v) now[v] = next[v];
-      if (tile + 1 < t1) {
+      for (int i = 0; i < BS_VECTORS; ++i) now[i] = Logits<T>::clean(next[i]);
+      if (tile + 1 < t1) load(tile + 1, next);
+      float best[BS_VECTORS];
 #pragma unroll
-        for (int v = 0; v < BS_VECTORS; ++v) next[v] = load_chunk(p, a.vocab, first_of(tile + 1, v));
-      }
-      float f[BS_VECTORS][N], best[BS_VECTORS];
-      float top = m;
-#pragma unroll
-      for (int v = 0; v < BS_VECTORS; ++v) {
-        Logits<T>::unpack(now[v], f[v]);
-        best[v] = f[v][0];
-#pragma unroll
-        for (int e = 1; e < N; ++e) best[v] = fmaxf(best[v], f[v][e]);
-        top = fmaxf(top, best[v]);
-      }
+      for (int i = 0; i < BS_VECTORS; ++i) best[i] = Logits<T>::largest(now[i]);
+      const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
       if (top > m) {
         sum = m == -INFINITY ? 0.0 : sum * b2::ex2((m - top) * 1.4426950408889634f);
         m = top;
       }
       if (m > -INFINITY) {
-        float s = 0.f;
+        uint64_t s[2] = {};
+        const uint64_t minus = b2::pair_of(-m, -m), scale = b2::pair_of(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
-        for (int v = 0; v < BS_VECTORS; ++v)
+        for (int i = 0; i < BS_VECTORS; ++i) {
+          float f[N];
+          Logits<T>::unpack(now[i], f);
 #pragma unroll
-          for (int e = 0; e < N; ++e) s += b2::ex2((f[v][e] - m) * 1.4426950408889634f);
-        sum += s;
+          for (int e = 0; e < N; e += 2) {
+            float x, y;
+            b2::halves_of(b2::mul_pair(b2::add_pair(b2::pair_of(f[e], f[e + 1]), minus), scale), x, y);
+            s[(e >> 1) & 1] = b2::add_pair(s[(e >> 1) & 1], b2::pair_of(b2::ex2(x), b2::ex2(y)));
+          }
+        }
+        float x, y;
+        b2::halves_of(b2::add_pair(s[0], s[1]), x, y);
+        sum += x + y;
       }
-      // the tile's candidates by the best of each thread
-      auto by_maxima = [&](uint64_t least) {
-        uint64_t mine = 0;
+      const int token0 = tile * TILE - shift + tid * N;
+      auto push_from = [&](float least, bool ties) {
 #pragma unroll
-        for (int v = 0; v < BS_VECTORS; ++v)
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (f[v][e] > -INFINITY) mine = max(mine, key_of(f[v][e], static_cast<int>(first_of(tile, v)) + e));
-        uint64_t t = 0;
-        for (int bit = 63; bit >= 0; --bit) {
-          const uint64_t c = t | (1ull << bit);
-          const int all = __syncthreads_count(mine >= c);
-          if (all >= K) t = c;
-          if (all >= K && all <= K + K / 2) break;
-        }
-        t = max(t, least);
-        if (mine >= t && mine != 0) {
-#pragma unroll
-          for (int v = 0; v < BS_VECTORS; ++v)
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-              const uint64_t key = key_of(f[v][e], static_cast<int>(first_of(tile, v)) + e);
-              if (f[v][e] > -INFINITY && key >= t) list.push(key);
-            }
-        }
-        return t;
-      };
-      if (tile == t0) {
-        by_maxima(0);
-        __syncthreads();
-        count = s_count;
-      } else {
-#pragma unroll
-        for (int v = 0; v < BS_VECTORS; ++v)
-          if (best[v] > bound) {
+        for (int i = 0; i < BS_VECTORS; ++i)
+          if (best[i] > least || (ties && best[i] == least)) {
+            float f[N];
+            Logits<T>::unpack(now[i], f);
 #pragma unroll
             for (int e = 0; e < N; ++e)
-              if (f[v][e] > bound) list.push(key_of(f[v][e], static_cast<int>(first_of(tile, v)) + e));
+              if (f[e] > least || (ties && f[e] == least)) list.push(key_of(f[e], token0 + i * BS_THREADS * N + e));
           }
+      };
+      if (tile == t0) {
+        // the K-th best of the threads' maxima, which each warp sorts
+        float x = top;
+#pragma unroll
+        for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+          for (int j = k >> 1; j > 0; j >>= 1) {
+            const float y = __shfl_xor_sync(0xffffffffu, x, j);
+            x = ((lane & j) == 0) == ((lane & k) == 0) ? fmaxf(x, y) : fminf(x, y);
+          }
+        s_top[tid] = x;
         __syncthreads();
-        int now_count = s_count;
-        if (now_count > a.capacity) {  // (a row that rises all along)
-          __syncthreads();
-          uint64_t least = 0;
-          if (count > K) least = list.cut(count, K);
-          else if (tid == 0) s_count = count;
-          __syncthreads();
-          by_maxima(least);
-          __syncthreads();
-          now_count = s_count;
+        int rank = lane;
+#pragma unroll
+        for (int w = 0; w < BS_THREADS / 32; ++w) {
+          if (w == warp) continue;
+          int lo = 0;  // how many of warp w come before
+#pragma unroll
+          for (int step = 16; step > 0; step >>= 1) {
+            const float y = s_top[w * 32 + lo + step - 1];
+            if (y > x || (y == x && w < warp)) lo += step;
+          }
+          const float y = s_top[w * 32 + lo];
+          if (lo < 32 && (y > x || (y == x && w < warp))) ++lo;
+          rank += lo;
         }
-        count = now_count;
-      }
-      if (count > 4 * K + 64 || (count >= K && bound == -INFINITY && tile + 1 < t1)) {
-        const uint64_t t = count > K ? list.cut(count, K) : list.kth(count, count);
-        count = s_count;
-        bound = number_of(static_cast<uint32_t>(t >> 32));
+        if (rank == K - 1) s_bound = x;
+        __syncthreads();
+        const float least = s_bound;
+        if (least == -INFINITY) push_from(least, false);  // (what is forbidden is no candidate)
+        else push_from(least, true);
+      } else {
+        push_from(bound, false);
       }
       __syncthreads();
+      const int seen = s_count;
+      __syncthreads();  // (the next tile's may go in)
+      if (seen > a.capacity) {
+        // Many equal logits, or a row that rises all along: 256 at a time.
+        if (tid == 0) s_count = count;
+        __syncthreads();
+        if (count >= K) count = list.rank(count, K);
+        for (int i = 0; i < BS_VECTORS; ++i)
+          for (int e = 0; e < N; ++e) {
+            const int token = token0 + i * BS_THREADS * N + e;
+            const uint64_t least = count >= K ? s_keys[K - 1] : 0;
+            __syncthreads();
+            if (token >= 0 && token < a.vocab) {
+              const float f = Logits<T>::one(p + token);
+              if (f > -INFINITY && key_of(f, token) > least) list.push(key_of(f, token));
+            }
+            __syncthreads();
+            count = list.rank(s_count, K);
+          }
+        if (count >= K) bound = number_of(static_cast<uint32_t>(s_keys[K - 1] >> 32));
+      } else {
+        count = seen;
+      }
+      if (tile + 1 < t1 && (count > limit || (tile == t0 && count >= K))) {
+        count = list.rank(count, K);
+        bound = number_of(static_cast<uint32_t>(s_keys[K - 1] >> 32));
+      }
     }
     // ---- the part: maximum and sum, and the K best in order ----
-    if (count > K) {
-      list.cut(count, K);
-      __syncthreads();
-      count = s_count;
-    }
+    count = list.rank(count, K);
     const int64_t at = static_cast<int64_t>(row) * a.parts + part;
-    if (tid < K) {
-      const uint64_t mine = tid < count ? s_keys[tid] : 0;
-      int rank = tid;
-      if (tid < count) {
-        rank = 0;
-        for (int i = 0; i < count; ++i) rank += s_keys[i] > mine ? 1 : 0;
-      }
-      a.keys[at * K + rank] = mine;
-    }
+    if (tid < K) a.keys[at * K + tid] = tid < count ? s_keys[tid] : 0;
     float top = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -300,7 +316,7 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(c
     top = s_max[0];
 #pragma unroll
     for (int w = 1; w < BS_THREADS / 32; ++w) top = fmaxf(top, s_max[w]);
-    double all = m == -INFINITY ? 0.0 : sum * exp(static_cast<double>(m) - static_cast<double>(top));
+    double all = m == -INFINITY ? 0.0 : sum * b2::ex2((m - top) * 1.4426950408889634f);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     if (lane == 0) s_sum[warp] = all;
@@ -333,97 +349,105 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const PickArgs a) {
+__global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a) {
   const ScanArgs& s = a.scan;
-  __shared__ double s_total[BS_MAX_BEAMS], s_score[BS_MAX_BEAMS], s_sum[BS_THREADS / 32];
+  constexpr int WARPS = BP_THREADS / 32;
+  __shared__ double s_total[BS_MAX_BEAMS], s_score[BS_MAX_BEAMS], s_sum[WARPS], s_top;
   __shared__ int s_parts[BS_MAX_BEAMS + 1], s_kind[BS_MAX_BEAMS], s_again[BS_MAX_BEAMS], s_tally[32], s_count, s_any;
   __shared__ Candidate s_got[BS_COLLECT], s_best[BS_MAX_PICKS + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = s.beams, K = s.picks, row0 = blockIdx.x * B;
+  const ScanDeal deal(s.rows * s.tiles, a.grid);
   b2::pdl_launch_dependents();
   b2::pdl_wait();
-  const int64_t total = static_cast<int64_t>(s.rows) * s.tiles;
-  if (tid < B) {
-    const float score = s.scores[row0 + tid];
-    const bool there = score > -INFINITY, ended = s.finished != nullptr && s.finished[row0 + tid] != 0;
-    s_score[tid] = score;
-    s_kind[tid] = !there ? 0 : ended ? 1 : 2;
-    s_again[tid] = 0;
-    // parts of the row: CTAs of the scan that hold its tiles
-    auto cta_of = [&](int64_t tile) {
-      int64_t x = tile * a.grid / total;
-      while (total * (x + 1) / a.grid <= tile) ++x;
-      while (total * x / a.grid > tile) --x;
-      return x;
-    };
-    const int64_t first = static_cast<int64_t>(row0 + tid) * s.tiles;
-    s_parts[tid + 1] = !there ? 0 : ended ? 1 : static_cast<int>(cta_of(first + s.tiles - 1) - cta_of(first)) + 1;
-  }
-  if (tid == 0) {
-    s_parts[0] = 0;
-    s_count = s_any = 0;
+  if (warp == 0) {
+    int parts = 0;
+    if (lane < B) {
+      const float score = s.scores[row0 + lane];
+      const bool there = score > -INFINITY, ended = s.finished != nullptr && s.finished[row0 + lane] != 0;
+      s_score[lane] = score;
+      s_kind[lane] = !there ? 0 : ended ? 1 : 2;
+      s_again[lane] = 0;
+      const int first = (row0 + lane) * s.tiles;
+      parts = !there ? 0 : ended ? 1 : deal.cta_of(first + s.tiles - 1) - deal.cta_of(first) + 1;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, parts, o);
+      if (lane >= o) parts += up;
+    }
+    if (lane < B) s_parts[lane + 1] = parts;
+    if (lane == 0) s_parts[0] = s_count = s_any = 0;
   }
   if (tid < 32) s_tally[tid] = 0;
   __syncthreads();
-  for (int b = warp; b < B; b += BS_THREADS / 32) {
-    if (s_kind[b] != 2) continue;
-    const int parts = s_parts[b + 1];
-    const int64_t at = static_cast<int64_t>(row0 + b) * s.parts;
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, s.maxima[at + i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    double all = 0.0;
-    for (int i = lane; i < parts; i += 32)
-      if (s.maxima[at + i] > -INFINITY) all += s.sums[at + i] * exp(static_cast<double>(s.maxima[at + i]) - static_cast<double>(top));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    if (lane == 0) s_total[b] = static_cast<double>(top) + log(all);
-  }
-  __syncthreads();
-  if (tid == 0)
-    for (int b = 0; b < B; ++b) s_parts[b + 1] += s_parts[b];
-  __syncthreads();
   const int lists = s_parts[B];
-  // entry `depth` of a list; false where there is none
-  auto entry = [&](int list, int depth, Candidate& c) {
+  auto beam_of = [&](int list) {
     int lo = 0, hi = B - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (s_parts[mid] <= list) lo = mid;
       else hi = mid - 1;
     }
-    c.beam = lo;
-    if (s_kind[lo] == 1) {
-      c.score = s_score[lo];
-      c.x = 0.f;
-      c.token = -1;
-      return depth == 0;
-    }
-    const uint64_t key = depth < K ? s.keys[(static_cast<int64_t>(row0 + lo) * s.parts + list - s_parts[lo]) * K + depth] : 0;
-    if (key == 0) return false;
-    c.x = number_of(static_cast<uint32_t>(key >> 32));
-    c.token = token_of(key);
-    c.score = s_score[lo] + (static_cast<double>(c.x) - s_total[lo]);
-    return true;
+    return lo;
   };
-  // ---- a bound that at least K + 1 of the lists' first entries reach ----
-  uint32_t t = 0;
-  if (lists > 0) {
-    const int deep = (K + lists) / lists, n = lists * deep;
-    constexpr int MOST = 8;  // entries of a thread that it keeps; (lists are at most a few per CTA of the scan)
-    uint32_t mine[MOST];
-    auto value = [&](int g) {
-      Candidate c;
-      return g < n && entry(g % lists, g / lists, c) ? ordered(static_cast<float>(c.score)) : 0u;
-    };
+  // entry `depth` of a list of beam b: its key, 0 where there is none
+  auto key_at = [&](int b, int list, int depth) -> uint64_t {
+    if (s_kind[b] == 1) return depth == 0 ? 1 : 0;
+    return depth < K ? s.keys[(static_cast<int64_t>(row0 + b) * s.parts + list - s_parts[b]) * K + depth] : 0;
+  };
+  auto candidate = [&](int b, uint64_t key) {
+    if (s_kind[b] == 1) return Candidate{s_score[b], 0.f, b, -1};
+    const float x = number_of(static_cast<uint32_t>(key >> 32));
+    return Candidate{s_score[b] + (static_cast<double>(x) - s_total[b]), x, b, token_of(key)};
+  };
+  // ---- the lists' first entries, while the rows' sums are on their way ----
+  const int deep = lists > 0 ? (K + lists) / lists : 0, n = lists * deep;
+  constexpr int MOST = 4;  // entries of a thread; (lists are a few more than the CTAs of the scan at most, and fewer entries than there are only lower the bound)
+  uint64_t head[MOST];
+  int of[MOST];
 #pragma unroll
-    for (int i = 0; i < MOST; ++i) mine[i] = value(tid + i * BS_THREADS);
+  for (int i = 0; i < MOST; ++i) {
+    const int g = tid + i * BP_THREADS;
+    head[i] = 0;
+    of[i] = 0;
+    if (g < n) {
+      of[i] = beam_of(g % lists);
+      head[i] = key_at(of[i], g % lists, g / lists);
+    }
+  }
+  for (int b = warp; b < B; b += WARPS) {
+    if (s_kind[b] != 2) continue;
+    const int parts = s_parts[b + 1] - s_parts[b];
+    const int64_t at = static_cast<int64_t>(row0 + b) * s.parts;
+    float top = -INFINITY;
+    double all = 0.0;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      const bool is = i0 + lane < parts;
+      const float m = is ? s.maxima[at + i0 + lane] : -INFINITY;
+      const double sum = is ? s.sums[at + i0 + lane] : 0.0;
+      float higher = fmaxf(top, m);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) higher = fmaxf(higher, __shfl_xor_sync(0xffffffffu, higher, o));
+      if (top > -INFINITY) all *= b2::ex2((top - higher) * 1.4426950408889634f);
+      if (m > -INFINITY) all += sum * b2::ex2((m - higher) * 1.4426950408889634f);
+      top = higher;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) s_total[b] = static_cast<double>(top) + log(all);
+  }
+  __syncthreads();
+  // ---- a bound that at least K + 1 of the entries reach ----
+  uint32_t t = 0;
+  {
+    uint32_t mine[MOST];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) mine[i] = head[i] != 0 ? ordered(static_cast<float>(candidate(of[i], head[i]).score)) : 0u;
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t c = t | (1u << bit);
       int reach = 0;
 #pragma unroll
-      for (int i = 0; i < MOST; ++i) reach += mine[i] >= c ? 1 : 0;
-      reach = __reduce_add_sync(0xffffffffu, reach);
+      for (int i = 0; i < MOST; ++i) reach += __popc(__ballot_sync(0xffffffffu, mine[i] >= c));
       if (lane == 0 && reach > 0) atomicAdd(s_tally + bit, reach);
       __syncthreads();
       const int all = s_tally[bit];
@@ -434,21 +458,36 @@ __global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const PickArgs a)
   // (a little lower: what lies as near as the sums' error belongs to it)
   double least = -INFINITY;
   if (t > 0x00800000u) least = static_cast<double>(number_of(t)) - 2 * BS_NEAR - 2.4e-7 * fabs(static_cast<double>(number_of(t)));
-  for (int l = tid; l < lists; l += BS_THREADS) {
-    Candidate c;
-    for (int d = 0; entry(l, d, c) && c.score >= least; ++d) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < BS_COLLECT) s_got[at] = c;
+  // ---- the entries that reach it: a warp takes a list, 32 entries at a time ----
+  for (int list = warp; list < lists; list += WARPS) {
+    const int b = beam_of(list);
+    for (int d = 0;; d += 32) {
+      const uint64_t key = key_at(b, list, d + lane);
+      Candidate c{};
+      bool reaches = key != 0;
+      if (reaches) {
+        c = candidate(b, key);
+        reaches = c.score >= least;
+      }
+      const unsigned all = __ballot_sync(0xffffffffu, reaches);
+      int at = 0;
+      if (lane == 0 && all != 0) at = atomicAdd(&s_count, __popc(all));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
+      if (reaches && at < BS_COLLECT) s_got[at] = c;
+      if (all != 0xffffffffu) break;
     }
   }
   __syncthreads();
-  const int got = s_count;
-  int best = min(got, K + 1);
+  const int got = s_count, best = min(got, K + 1);
   auto rank_all = [&]() {
-    for (int i = tid; i < got; i += BS_THREADS) {
+    for (int i = tid; i < got; i += BP_THREADS) {
       const Candidate mine = s_got[i];
       int rank = 0;
-      for (int k = 0; k < got; ++k) rank += before(s_got[k], mine) ? 1 : 0;
+#pragma unroll 4
+      for (int k = 0; k < got; ++k) {
+        const double other = s_got[k].score;
+        rank += other > mine.score || (other == mine.score && before(s_got[k], mine)) ? 1 : 0;
+      }
       if (rank < K + 1) s_best[rank] = mine;
     }
     __syncthreads();
@@ -457,10 +496,14 @@ __global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const PickArgs a)
   auto one_by_one = [&]() {
     Candidate last{INFINITY, 0.f, -1, -2};
     for (int k = 0; k < best; ++k) {
-      Candidate mine{-INFINITY, 0.f, BS_MAX_BEAMS, 0x7fffffff}, c;
-      for (int l = tid; l < lists; l += BS_THREADS)
-        for (int d = 0; entry(l, d, c) && c.score >= least; ++d)
-          if (before(last, c) && before(c, mine)) mine = c;
+      Candidate mine{-INFINITY, 0.f, BS_MAX_BEAMS, 0x7fffffff};
+      for (int g = tid; g < lists * K; g += BP_THREADS) {
+        const int b = beam_of(g / K);
+        const uint64_t key = key_at(b, g / K, g % K);
+        if (key == 0) continue;
+        const Candidate c = candidate(b, key);
+        if (before(last, c) && before(c, mine)) mine = c;
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const Candidate other{__shfl_xor_sync(0xffffffffu, mine.score, o), __shfl_xor_sync(0xffffffffu, mine.x, o), __shfl_xor_sync(0xffffffffu, mine.beam, o),
@@ -470,7 +513,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const PickArgs a)
       if (lane == 0) s_got[warp] = mine;
       __syncthreads();
       last = s_got[0];
-      for (int w = 1; w < BS_THREADS / 32; ++w)
+      for (int w = 1; w < WARPS; ++w)
         if (before(s_got[w], last)) last = s_got[w];
       if (tid == 0) s_best[k] = last;
       __syncthreads();
@@ -482,24 +525,32 @@ __global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const PickArgs a)
   // ---- continuations of different beams that are too near each other: those beams' sums in 64 bits ----
   if (tid + 1 < best) {
     const Candidate &c = s_best[tid], &d = s_best[tid + 1];
-    if (c.beam != d.beam && c.score - d.score <= BS_NEAR) s_again[c.beam] = s_again[d.beam] = s_any = 1;
+    if (c.beam != d.beam && c.score - d.score <= BS_NEAR && (s_kind[c.beam] == 2 || s_kind[d.beam] == 2)) s_again[c.beam] = s_again[d.beam] = s_any = 1;
   }
   __syncthreads();
   if (s_any) {
     for (int b = 0; b < B; ++b) {
       if (!s_again[b] || s_kind[b] != 2) continue;
       const T* p = static_cast<const T*>(s.logits) + (row0 + b) * s.ld;
-      double top = -INFINITY, all = 0.0;
-      for (int i = 0; i < s_parts[b + 1] - s_parts[b]; ++i) top = fmax(top, static_cast<double>(s.maxima[static_cast<int64_t>(row0 + b) * s.parts + i]));
+      if (warp == 0) {
+        float top = -INFINITY;
+        for (int i = lane; i < s_parts[b + 1] - s_parts[b]; i += 32) top = fmaxf(top, s.maxima[static_cast<int64_t>(row0 + b) * s.parts + i]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane == 0) s_top = top;
+      }
+      __syncthreads();
+      const double top = s_top;
+      double all = 0.0;
 #pragma unroll 4
-      for (int i = tid; i < s.vocab; i += BS_THREADS) all += exp(static_cast<double>(Logits<T>::one(p + i)) - top);
+      for (int i = tid; i < s.vocab; i += BP_THREADS) all += exp(static_cast<double>(Logits<T>::one(p + i)) - top);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
       if (lane == 0) s_sum[warp] = all;
       __syncthreads();
       if (tid == 0) {
         all = 0.0;
-        for (int w = 0; w < BS_THREADS / 32; ++w) all += s_sum[w];
+        for (int w = 0; w < WARPS; ++w) all += s_sum[w];
         s_total[b] = top + log(all);
       }
       __syncthreads();
@@ -507,7 +558,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_pick_kernel(const PickArgs a)
     if (many) {
       one_by_one();
     } else {
-      for (int i = tid; i < got; i += BS_THREADS)
+      for (int i = tid; i < got; i += BP_THREADS)
         if (s_kind[s_got[i].beam] == 2) s_got[i].score = s_score[s_got[i].beam] + (static_cast<double>(s_got[i].x) - s_total[s_got[i].beam]);
       __syncthreads();
       rank_all();
@@ -807,7 +858,7 @@ SelectPlan plan_select(int num_sms, int rows, int vocab, int picks, bool fp32) {
   p.grid = static_cast<int>(std::min<int64_t>(total, static_cast<int64_t>(num_sms) * BS_CTAS_PER_SM));
   const int64_t least = total / std::max(1, p.grid);  // tiles of the shortest range
   p.parts = static_cast<int>(std::min<int64_t>(p.tiles, (p.tiles + least - 1) / std::max<int64_t>(1, least) + 1));
-  p.capacity = (picks + picks / 2) * (fp32 ? 4 : 8) * BS_VECTORS + 5 * picks + 64;
+  p.capacity = picks * (fp32 ? 4 : 8) * BS_VECTORS + 256;  // (K threads' logits reach the bound of a first tile, or more where they are equal)
   p.keys_bytes = (static_cast<int64_t>(rows) * p.parts * picks * 8 + 15) / 16 * 16;
   p.sums_bytes = (static_cast<int64_t>(rows) * p.parts * 8 + 15) / 16 * 16;
   p.bytes = p.keys_bytes + p.sums_bytes + static_cast<int64_t>(rows) * p.parts * 4;
@@ -829,6 +880,9 @@ int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n,
   if (n == 0) return B2_OK;
   const int64_t need = b2_beam_select_workspace(ctx, n, beams, vocab, picks, fp32);
   if (need < 0) return b2::set_error(B2_ERR_SHAPE, "%d requests of %d beams, %d picks of %d: at most %d beams and %d picks", n, beams, picks, vocab, BS_MAX_BEAMS, BS_MAX_PICKS);
+  const int64_t row_tiles = (static_cast<int64_t>(vocab) * (fp32 ? 4 : 2) + 30) / BS_TILE_BYTES + 1;
+  if (row_tiles * n * beams >= 1ll << 31 || static_cast<int64_t>(vocab) + BS_TILE_BYTES >= 1ll << 31)
+    return b2::set_error(B2_ERR_SHAPE, "%d rows of %d tokens", n * beams, vocab);
   if (!logits || !scores || !scores_out || !parents_out || !tokens_out || !finished_out || ld < vocab) return B2_ERR_ARG;
   if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)) return B2_ERR_ARG;
   const SelectPlan p = plan_select(ctx->num_sms, n * beams, vocab, picks, fp32 != 0);
@@ -839,7 +893,7 @@ int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n,
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
   const size_t smem = static_cast<size_t>(p.capacity) * 8;
   B2_CUDA(b2_launch(fp32 ? beam_scan_kernel<float> : beam_scan_kernel<__nv_bfloat16>, dim3(p.grid), dim3(BS_THREADS), smem, on, s));
-  B2_CUDA(b2_launch(fp32 ? beam_pick_kernel<float> : beam_pick_kernel<__nv_bfloat16>, dim3(n), dim3(BS_THREADS), 0, on, k));
+  B2_CUDA(b2_launch(fp32 ? beam_pick_kernel<float> : beam_pick_kernel<__nv_bfloat16>, dim3(n), dim3(BP_THREADS), 0, on, k));
   return B2_OK;
 }
 
