@@ -24,11 +24,11 @@ namespace {
 //
 // Bound: HBM, every logit read once.
 // ---------------------------------------------------------------------------
-constexpr int BS_THREADS = 256, BS_VECTORS = 4, BS_CTAS_PER_SM = 4;
+constexpr int BS_THREADS = 256, BS_VECTORS = 4, BS_CTAS_PER_SM = 4, BS_GROUP = 4;
 constexpr int BS_TILE_BYTES = BS_THREADS * BS_VECTORS * 16;
 constexpr int BS_MAX_PICKS = 64, BS_MAX_BEAMS = 32;
-constexpr int BP_THREADS = 512;
-constexpr int BS_COLLECT = 1024;  // candidates that a request ranks at once
+constexpr int BP_THREADS = 512, BP_LISTS = 256;
+constexpr int BS_COLLECT = 1536, BP_RANKED = 192;  // candidates that a request collects, and that it ranks without another bound
 constexpr double BS_NEAR = 4e-6;
 
 struct ScanArgs {
@@ -40,8 +40,7 @@ struct ScanArgs {
   const float* scores;
   const uint8_t* finished;
   uint64_t* keys;  // [rows][parts][picks], best first, 0: none
-  float* maxima;   // [rows][parts]
-  double* sums;
+  double2* sums;   // [rows][parts] (M, sum of 2^(x log2(e) - M)); M is a whole number, -inf where there is nothing
 };
 
 __device__ __forceinline__ uint32_t ordered(float x) {  // unsigned order = order of the numbers; -0 is 0
@@ -52,6 +51,12 @@ __device__ __forceinline__ float number_of(uint32_t o) { return __uint_as_float(
 __device__ __forceinline__ uint64_t key_of(float x, int token) { return (static_cast<uint64_t>(ordered(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(token)); }
 __device__ __forceinline__ int token_of(uint64_t key) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)); }
 
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr double LOG2E_64 = 1.4426950408889634, LN2_64 = 0.6931471805599453;
+constexpr float BS_PLAIN = 65536.f;  // below this size x log2(e) is formed in 32 bits
+// 2^x of a whole number x <= 0, exactly; 0 below the normal range (and for NaN, the difference of two -inf)
+__device__ __forceinline__ double power_of_two(double x) { return x > -1023.0 ? __longlong_as_double(static_cast<long long>(1023 + static_cast<int>(x)) << 52) : 0.0; }
+
 // NaN counts as -inf, +inf as the largest number
 __device__ __forceinline__ float plain_number(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 
@@ -60,9 +65,8 @@ struct Logits;
 template <>
 struct Logits<float> {
   static constexpr int N = 4;
+  static __device__ __forceinline__ float most() { return FLT_MAX; }
   static __device__ __forceinline__ float one(const float* p) { return plain_number(__ldg(p)); }
-  static __device__ __forceinline__ uint32_t clean(uint32_t w) { return __float_as_uint(plain_number(__uint_as_float(w))); }
-  static __device__ __forceinline__ uint4 clean(const uint4& v) { return make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w)); }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x);
     f[1] = __uint_as_float(v.y);
@@ -76,17 +80,12 @@ struct Logits<float> {
 template <>
 struct Logits<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return fminf(fmaxf(__bfloat162float(*p), -INFINITY), b2::bf16_hi(0x7f7f0000u)); }
+  static __device__ __forceinline__ float most() { return b2::bf16_hi(0x7f7f0000u); }
+  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return fminf(fmaxf(__bfloat162float(*p), -INFINITY), most()); }
   static __device__ __forceinline__ uint32_t max2(uint32_t x, uint32_t y) {
     const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  static __device__ __forceinline__ uint32_t clean(uint32_t w) {
-    const uint32_t low = max2(w, 0xff80ff80u), high = 0x7f7f7f7fu;
-    const __nv_bfloat162 v = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&low), *reinterpret_cast<const __nv_bfloat162*>(&high));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  static __device__ __forceinline__ uint4 clean(const uint4& v) { return make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w)); }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) { b2::unpack8(v, f); }
   static __device__ __forceinline__ float largest(const uint4& v) {
     const uint32_t w = max2(max2(v.x, v.y), max2(v.z, v.w));
@@ -96,7 +95,7 @@ struct Logits<__nv_bfloat16> {
 
 // The 16 bytes at `chunk` (counted from the 16-byte boundary at or before the row), -inf in the places that are not the row's.
 template <typename T>
-__device__ __forceinline__ uint4 load_chunk(const T* row, int vocab, int64_t first) {  // first: the row's element at which the chunk begins, may be < 0
+__device__ __noinline__ uint4 load_chunk(const T* row, int vocab, int64_t first) {  // first: the row's element at which the chunk begins, may be < 0
   constexpr int N = Logits<T>::N;
   if (first >= 0 && first + N <= vocab) return __ldg(reinterpret_cast<const uint4*>(row + first));
   uint32_t w[4] = {0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
@@ -125,16 +124,16 @@ struct List {
   uint64_t *keys, *best;  // [capacity], [BS_MAX_PICKS]
   int* count;             // of those that were to go in: may be past the capacity
   int capacity;
-  __device__ __forceinline__ void push(uint64_t key) {
+  __device__ __forceinline__ void push(uint64_t key) const {
     const int at = atomicAdd(count, 1);
     if (at < capacity) keys[at] = key;
   }
   // All threads: the k best of the n keys stay, in order.  Every thread counts the keys before its own.  Returns how many there are.
-  __device__ int rank(int n, int k) {
+  __device__ __noinline__ int rank(int n, int k) const {
     for (int i = threadIdx.x; i < n; i += BS_THREADS) {
       const uint64_t mine = keys[i];
       int before = 0;
-#pragma unroll 8
+#pragma unroll 4
       for (int j = 0; j < n; ++j) before += keys[j] > mine ? 1 : 0;
       if (before < k) best[before] = mine;
     }
@@ -145,7 +144,112 @@ struct List {
     __syncthreads();
     return left;
   }
+  // All threads: those of the n keys stay, in no order, whose logits reach the bound.
+  __device__ __noinline__ int filter(int n, float bound) const {
+    const uint64_t least = static_cast<uint64_t>(ordered(bound)) << 32;
+    if (threadIdx.x == 0) *count = 0;
+    __syncthreads();
+    // in steps of the block: what a step writes lies before what later ones read
+    for (int i0 = 0; i0 < n; i0 += BS_THREADS) {
+      const uint64_t mine = i0 + static_cast<int>(threadIdx.x) < n ? keys[i0 + threadIdx.x] : 0;
+      __syncthreads();
+      if (mine >= least && mine != 0) keys[atomicAdd(count, 1)] = mine;
+      __syncthreads();
+    }
+    const int left = *count;
+    __syncthreads();
+    return left;
+  }
 };
+
+// (Out of line: rare, or little beside the loop over the tiles, which has to fit the instruction cache.)
+// All threads: the candidates among tokens first .. last, for which there was no room (many equal logits, or a row that rises all along): 256 at a time.
+template <typename T>
+__device__ __noinline__ int overflow(const List list, const T* p, int vocab, int k, int count, int first, int last) {
+  if (threadIdx.x == 0) *list.count = count;
+  __syncthreads();
+  if (count >= k) count = list.rank(count, k);
+  for (; first < last; first += BS_THREADS) {
+    const int token = first + threadIdx.x;
+    const uint64_t least = count >= k ? list.keys[k - 1] : 0;
+    __syncthreads();
+    if (token >= 0 && token < vocab) {
+      const float f = Logits<T>::one(p + token);
+      if (f > -INFINITY && key_of(f, token) > least) list.push(key_of(f, token));
+    }
+    __syncthreads();
+    count = list.rank(*list.count, k);
+  }
+  return count;
+}
+// largest logit of a thread's part of a tile
+template <typename T>
+__device__ __noinline__ float tile_maximum(const T* p, int vocab, int token0) {
+  constexpr int N = Logits<T>::N;
+  float top = -INFINITY;
+  for (int i = 0; i < BS_VECTORS * N; ++i) {
+    const int token = token0 + i / N * (BS_THREADS * N) + i % N;
+    if (token >= 0 && token < vocab) top = fmaxf(top, Logits<T>::one(p + token));
+  }
+  return top;
+}
+// sum of 2^(x log2(e) - ref) over it, in 64 bits
+template <typename T>
+__device__ __noinline__ double exact_sum(const T* p, int vocab, int token0, double ref) {
+  constexpr int N = Logits<T>::N;
+  double sum = 0.0;
+  for (int i = 0; i < BS_VECTORS * N; ++i) {
+    const int token = token0 + i / N * (BS_THREADS * N) + i % N;
+    if (token >= 0 && token < vocab) sum += exp2(__dmul_rn(Logits<T>::one(p + token), LOG2E_64) - ref);
+  }
+  return sum;
+}
+// All threads: a number that the numbers of at least k of them reach, quickly: each warp's ceil(k / warps)-th largest, and the least of those.
+__device__ __noinline__ float reached_by(float x, int k, float* of_warps) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (k + BS_THREADS / 32 - 1) / (BS_THREADS / 32);
+  for (int i = 1; i < each; ++i) {  // the largest is taken out
+    const unsigned best = __reduce_max_sync(0xffffffffu, ordered(x));
+    const unsigned who = __ballot_sync(0xffffffffu, ordered(x) == best);
+    if (lane == __ffs(who) - 1) x = -INFINITY;
+  }
+  const unsigned best = __reduce_max_sync(0xffffffffu, ordered(x));
+  if (lane == 0) of_warps[warp] = number_of(best);
+  __syncthreads();
+  x = of_warps[0];
+#pragma unroll
+  for (int w = 1; w < BS_THREADS / 32; ++w) x = fminf(x, of_warps[w]);
+  __syncthreads();
+  return x;
+}
+// All threads: the k-th largest of one number each.  The warps sort theirs, and every thread finds its own's place in the others.
+__device__ __noinline__ float kth_of_threads(float x, int k, float* sorted, float* found) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int j = n >> 1; j > 0; j >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, j);
+      x = ((lane & j) == 0) == ((lane & n) == 0) ? fmaxf(x, y) : fminf(x, y);
+    }
+  sorted[tid] = x;
+  __syncthreads();
+  int rank = lane;
+  for (int w = 0; w < BS_THREADS / 32; ++w) {
+    if (w == warp) continue;
+    int lo = 0;  // how many of warp w come before
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) {
+      const float y = sorted[w * 32 + lo + step - 1];
+      if (y > x || (y == x && w < warp)) lo += step;
+    }
+    const float y = sorted[w * 32 + lo];
+    if (y > x || (y == x && w < warp)) ++lo;
+    rank += lo;
+  }
+  if (rank == k - 1) *found = x;
+  __syncthreads();
+  return *found;
+}
 
 // Ranges of `total` tiles: CTA x of X
 struct ScanDeal {
@@ -164,8 +268,8 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(c
   extern __shared__ __align__(16) uint64_t s_keys[];
   __shared__ uint64_t s_best[BS_MAX_PICKS];
   __shared__ int s_count;
-  __shared__ float s_top[BS_THREADS], s_bound, s_max[BS_THREADS / 32];
-  __shared__ double s_sum[BS_THREADS / 32];
+  __shared__ float s_top[BS_THREADS], s_bound;
+  __shared__ double s_ref[BS_THREADS / 32], s_sum[BS_THREADS / 32];
   List list{s_keys, s_best, &s_count, a.capacity};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.picks;
   const ScanDeal deal(a.rows * a.tiles, gridDim.x);
@@ -194,26 +298,39 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(c
     };
     uint4 next[BS_VECTORS];
     load(t0, next);
-    float m = -INFINITY, bound = -INFINITY;
-    double sum = 0.0;
+    float bound = INFINITY;     // logits from here on are candidates; not known before the first tile has been read
+    float highest = -INFINITY;  // of the thread's logits
+    // The sum's reference is a power of two, so that raising it is exact, and x log2(e) - M is one rounding of an exact product.
+    double ref = -INFINITY, sum = 0.0;
+    float ref_low = -INFINITY;  // ref as far as 32 bits go
+    auto raise = [&](double to) {
+      if (to > ref) {
+        sum *= power_of_two(ref - to);
+        ref = to;
+        ref_low = static_cast<float>(to);
+      }
+    };
     if (tid == 0) s_count = 0;
     int count = 0;
-    for (int tile = t0; tile < t1; ++tile) {
-      uint4 now[BS_VECTORS];
-#pragma unroll
-      for (int i = 0; i < BS_VECTORS; ++i) now[i] = Logits<T>::clean(next[i]);
-      if (tile + 1 < t1) load(tile + 1, next);
+    // The first tile, and then BS_GROUP at a time: what they hold is noted by vectors, and looked at when they are through.
+#pragma unroll 1
+    for (int tile = t0; tile < t1;) {
+      const int group = tile, last = tile == t0 ? t0 + 1 : min(t1, tile + BS_GROUP);
+      unsigned reach = 0, odd = 0;  // vectors whose largest reaches the bound; tiles with infinities, NaN or very large numbers
       float best[BS_VECTORS];
+#pragma unroll 1
+      for (; tile < last; ++tile) {
+        uint4 now[BS_VECTORS];
 #pragma unroll
-      for (int i = 0; i < BS_VECTORS; ++i) best[i] = Logits<T>::largest(now[i]);
-      const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-      if (top > m) {
-        sum = m == -INFINITY ? 0.0 : sum * b2::ex2((m - top) * 1.4426950408889634f);
-        m = top;
-      }
-      if (m > -INFINITY) {
-        uint64_t s[2] = {};
-        const uint64_t minus = b2::pair_of(-m, -m), scale = b2::pair_of(1.4426950408889634f, 1.4426950408889634f);
+        for (int i = 0; i < BS_VECTORS; ++i) now[i] = next[i];
+        if (tile + 1 < t1) load(tile + 1, next);
+#pragma unroll
+        for (int i = 0; i < BS_VECTORS; ++i) best[i] = Logits<T>::largest(now[i]);
+        const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+        const float mine = rintf(top * LOG2E);
+        if (mine > ref_low && top < BS_PLAIN) raise(mine);
+        uint64_t sums[2] = {};
+        const uint64_t minus = b2::pair_of(-ref_low, -ref_low), scale = b2::pair_of(LOG2E, LOG2E);
 #pragma unroll
         for (int i = 0; i < BS_VECTORS; ++i) {
           float f[N];
@@ -221,102 +338,79 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(c
 #pragma unroll
           for (int e = 0; e < N; e += 2) {
             float x, y;
-            b2::halves_of(b2::mul_pair(b2::add_pair(b2::pair_of(f[e], f[e + 1]), minus), scale), x, y);
-            s[(e >> 1) & 1] = b2::add_pair(s[(e >> 1) & 1], b2::pair_of(b2::ex2(x), b2::ex2(y)));
+            b2::fma_pair(x, y, b2::pair_of(f[e], f[e + 1]), scale, minus);
+            sums[(e >> 1) & 1] = b2::add_pair(sums[(e >> 1) & 1], b2::pair_of(b2::ex2(x), b2::ex2(y)));
           }
+          if (best[i] >= bound) reach |= 1u << ((tile - group) * BS_VECTORS + i);
         }
         float x, y;
-        b2::halves_of(b2::add_pair(s[0], s[1]), x, y);
-        sum += x + y;
+        b2::halves_of(b2::add_pair(sums[0], sums[1]), x, y);
+        // (NaN among the logits makes the sum one; with nothing but -inf so far it is one as well, or has nothing to add)
+        if (fabsf(top) < BS_PLAIN && x + y < INFINITY) sum += x + y;
+        else if (top != -INFINITY) odd |= 1u << (tile - group);
+        highest = fmaxf(highest, top < INFINITY ? top : -INFINITY);
       }
-      const int token0 = tile * TILE - shift + tid * N;
-      auto push_from = [&](float least, bool ties) {
+      // ---- once a group ----
+      for (; odd != 0; odd &= odd - 1) {
+        const int t = __ffs(odd) - 1, token0 = (group + t) * TILE - shift + tid * N;
+        const float top = tile_maximum<T>(p, a.vocab, token0);
+        if (top > -INFINITY) {
+          raise(rint(__dmul_rn(top, LOG2E_64)));
+          sum += exact_sum<T>(p, a.vocab, token0, ref);
+        }
+        highest = fmaxf(highest, top);
+      }
+      if (group == t0) {
+        bound = reached_by(highest, K, s_top);
+        if (bound == -INFINITY) bound = fmaxf(-FLT_MAX, kth_of_threads(highest, K, s_top, &s_bound));
 #pragma unroll
         for (int i = 0; i < BS_VECTORS; ++i)
-          if (best[i] > least || (ties && best[i] == least)) {
-            float f[N];
-            Logits<T>::unpack(now[i], f);
+          if (best[i] >= bound) reach |= 1u << i;
+      }
+      for (; reach != 0; reach &= reach - 1) {
+        const int v = __ffs(reach) - 1, token = (group + v / BS_VECTORS) * TILE - shift + (v % BS_VECTORS * BS_THREADS + tid) * N;
+        const uint4 w = load_chunk(p, a.vocab, token);  // (from L2, where it has just been)
+        float f[N];
+        Logits<T>::unpack(w, f);
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (f[e] > least || (ties && f[e] == least)) list.push(key_of(f[e], token0 + i * BS_THREADS * N + e));
-          }
-      };
-      if (tile == t0) {
-        // the K-th best of the threads' maxima, which each warp sorts
-        float x = top;
-#pragma unroll
-        for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-          for (int j = k >> 1; j > 0; j >>= 1) {
-            const float y = __shfl_xor_sync(0xffffffffu, x, j);
-            x = ((lane & j) == 0) == ((lane & k) == 0) ? fmaxf(x, y) : fminf(x, y);
-          }
-        s_top[tid] = x;
-        __syncthreads();
-        int rank = lane;
-#pragma unroll
-        for (int w = 0; w < BS_THREADS / 32; ++w) {
-          if (w == warp) continue;
-          int lo = 0;  // how many of warp w come before
-#pragma unroll
-          for (int step = 16; step > 0; step >>= 1) {
-            const float y = s_top[w * 32 + lo + step - 1];
-            if (y > x || (y == x && w < warp)) lo += step;
-          }
-          const float y = s_top[w * 32 + lo];
-          if (lo < 32 && (y > x || (y == x && w < warp))) ++lo;
-          rank += lo;
-        }
-        if (rank == K - 1) s_bound = x;
-        __syncthreads();
-        const float least = s_bound;
-        if (least == -INFINITY) push_from(least, false);  // (what is forbidden is no candidate)
-        else push_from(least, true);
-      } else {
-        push_from(bound, false);
+        for (int e = 0; e < N; ++e)
+          if (f[e] >= bound) list.push(key_of(fminf(f[e], Logits<T>::most()), token + e));
       }
       __syncthreads();
-      const int seen = s_count;
-      __syncthreads();  // (the next tile's may go in)
-      if (seen > a.capacity) {
-        // Many equal logits, or a row that rises all along: 256 at a time.
-        if (tid == 0) s_count = count;
-        __syncthreads();
-        if (count >= K) count = list.rank(count, K);
-        for (int i = 0; i < BS_VECTORS; ++i)
-          for (int e = 0; e < N; ++e) {
-            const int token = token0 + i * BS_THREADS * N + e;
-            const uint64_t least = count >= K ? s_keys[K - 1] : 0;
-            __syncthreads();
-            if (token >= 0 && token < a.vocab) {
-              const float f = Logits<T>::one(p + token);
-              if (f > -INFINITY && key_of(f, token) > least) list.push(key_of(f, token));
-            }
-            __syncthreads();
-            count = list.rank(s_count, K);
-          }
-        if (count >= K) bound = number_of(static_cast<uint32_t>(s_keys[K - 1] >> 32));
-      } else {
+      const int seen = s_count, fresh = seen - count;
+      __syncthreads();  // (the next group's may go in)
+      if (seen <= a.capacity) {
         count = seen;
+      } else {
+        count = overflow<T>(list, p, a.vocab, K, count, group * TILE - shift, last * TILE - shift);
+        if (count >= K) bound = fmaxf(bound, number_of(static_cast<uint32_t>(s_keys[K - 1] >> 32) + 1));
       }
-      if (tile + 1 < t1 && (count > limit || (tile == t0 && count >= K))) {
-        count = list.rank(count, K);
-        bound = number_of(static_cast<uint32_t>(s_keys[K - 1] >> 32));
+      if (tile < t1 && fresh > K / 2) {
+        // Later tokens have to be above what K threads have seen: as high, they would come behind those.
+        const float higher = group == t0 && bound > -FLT_MAX ? bound : reached_by(highest, K, s_top);
+        if (higher >= bound) {
+          if (count > limit) count = list.filter(count, higher);
+          bound = number_of(ordered(higher) + 1);
+        }
       }
     }
     // ---- the part: maximum and sum, and the K best in order ----
+    if (count > 2 * K + 32) {
+      const float higher = kth_of_threads(highest, K, s_top, &s_bound);
+      if (higher >= bound) count = list.filter(count, higher);
+    }
     count = list.rank(count, K);
     const int64_t at = static_cast<int64_t>(row) * a.parts + part;
     if (tid < K) a.keys[at * K + tid] = tid < count ? s_keys[tid] : 0;
-    float top = m;
+    double top = ref;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) s_max[warp] = top;
+    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) s_ref[warp] = top;
     __syncthreads();
-    top = s_max[0];
+    top = s_ref[0];
 #pragma unroll
-    for (int w = 1; w < BS_THREADS / 32; ++w) top = fmaxf(top, s_max[w]);
-    double all = m == -INFINITY ? 0.0 : sum * b2::ex2((m - top) * 1.4426950408889634f);
+    for (int w = 1; w < BS_THREADS / 32; ++w) top = fmax(top, s_ref[w]);
+    double all = sum * power_of_two(ref - top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     if (lane == 0) s_sum[warp] = all;
@@ -324,8 +418,7 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(c
     if (tid == 0) {
       all = 0.0;
       for (int w = 0; w < BS_THREADS / 32; ++w) all += s_sum[w];
-      a.maxima[at] = top;
-      a.sums[at] = all;
+      a.sums[at] = make_double2(top, all);
     }
   }
 }
@@ -352,8 +445,9 @@ template <typename T>
 __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a) {
   const ScanArgs& s = a.scan;
   constexpr int WARPS = BP_THREADS / 32;
-  __shared__ double s_total[BS_MAX_BEAMS], s_score[BS_MAX_BEAMS], s_sum[WARPS], s_top;
-  __shared__ int s_parts[BS_MAX_BEAMS + 1], s_kind[BS_MAX_BEAMS], s_again[BS_MAX_BEAMS], s_tally[32], s_count, s_any;
+  __shared__ double s_total[BS_MAX_BEAMS], s_score[BS_MAX_BEAMS], s_sum[WARPS], s_ref[BS_MAX_BEAMS];
+  __shared__ int s_parts[BS_MAX_BEAMS + 1], s_kind[BS_MAX_BEAMS], s_again[BS_MAX_BEAMS], s_tally[32], s_count, s_any, s_reach, s_list[BP_LISTS];
+  __shared__ uint32_t s_low, s_high;
   __shared__ Candidate s_got[BS_COLLECT], s_best[BS_MAX_PICKS + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = s.beams, K = s.picks, row0 = blockIdx.x * B;
   const ScanDeal deal(s.rows * s.tiles, a.grid);
@@ -376,7 +470,11 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
       if (lane >= o) parts += up;
     }
     if (lane < B) s_parts[lane + 1] = parts;
-    if (lane == 0) s_parts[0] = s_count = s_any = 0;
+    if (lane == 0) {
+      s_parts[0] = s_count = s_any = s_reach = 0;
+      s_low = 0xffffffffu;
+      s_high = 0;
+    }
   }
   if (tid < 32) s_tally[tid] = 0;
   __syncthreads();
@@ -401,8 +499,9 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     return Candidate{s_score[b] + (static_cast<double>(x) - s_total[b]), x, b, token_of(key)};
   };
   // ---- the lists' first entries, while the rows' sums are on their way ----
-  const int deep = lists > 0 ? (K + lists) / lists : 0, n = lists * deep;
-  constexpr int MOST = 4;  // entries of a thread; (lists are a few more than the CTAs of the scan at most, and fewer entries than there are only lower the bound)
+  constexpr int MOST = 8;  // entries of a thread
+  const bool all_here = lists * K <= MOST * BP_THREADS;
+  const int deep = lists > 0 ? (all_here ? K : (K + lists) / lists) : 0, n = lists * deep;
   uint64_t head[MOST];
   int of[MOST];
 #pragma unroll
@@ -411,70 +510,153 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     head[i] = 0;
     of[i] = 0;
     if (g < n) {
-      of[i] = beam_of(g % lists);
-      head[i] = key_at(of[i], g % lists, g / lists);
+      const int list = all_here ? g / K : g % lists;
+      of[i] = beam_of(list);
+      head[i] = key_at(of[i], list, all_here ? g - list * K : g / lists);
     }
   }
   for (int b = warp; b < B; b += WARPS) {
     if (s_kind[b] != 2) continue;
     const int parts = s_parts[b + 1] - s_parts[b];
-    const int64_t at = static_cast<int64_t>(row0 + b) * s.parts;
-    float top = -INFINITY;
-    double all = 0.0;
+    const double2* sums = s.sums + static_cast<int64_t>(row0 + b) * s.parts;
+    double top = -INFINITY, all = 0.0;
     for (int i0 = 0; i0 < parts; i0 += 32) {
-      const bool is = i0 + lane < parts;
-      const float m = is ? s.maxima[at + i0 + lane] : -INFINITY;
-      const double sum = is ? s.sums[at + i0 + lane] : 0.0;
-      float higher = fmaxf(top, m);
+      const double2 mine = i0 + lane < parts ? sums[i0 + lane] : make_double2(-INFINITY, 0.0);
+      double higher = fmax(top, mine.x);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) higher = fmaxf(higher, __shfl_xor_sync(0xffffffffu, higher, o));
-      if (top > -INFINITY) all *= b2::ex2((top - higher) * 1.4426950408889634f);
-      if (m > -INFINITY) all += sum * b2::ex2((m - higher) * 1.4426950408889634f);
+      for (int o = 16; o > 0; o >>= 1) higher = fmax(higher, __shfl_xor_sync(0xffffffffu, higher, o));
+      all = all * power_of_two(top - higher) + mine.y * power_of_two(mine.x - higher);
       top = higher;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    if (lane == 0) s_total[b] = static_cast<double>(top) + log(all);
+    if (lane == 0) {
+      s_ref[b] = top;
+      // log2(e) has 24 bits in the sum's exponents, which makes them this much too large; what carries the sum lies near M
+      const double off = fabs(top) < 2 * BS_PLAIN ? top * (static_cast<double>(LOG2E) * LN2_64 - 1.0) : 0.0;
+      s_total[b] = (top - off) * LN2_64 + log(all);
+    }
   }
   __syncthreads();
+  // All threads: a number that `enough` of the entries reach, and not many more than `most`; 0 where there are not as many.  Entries are 0 where there are none.
+  auto reached = [&](const uint32_t (&mine)[MOST], int enough, int most) {
+    uint32_t low = 0xffffffffu, high = 0;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i)
+      if (mine[i] != 0) {
+        low = min(low, mine[i]);
+        high = max(high, mine[i]);
+      }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if (lane == 0 && high != 0) {
+      atomicMin(&s_low, low);
+      atomicMax(&s_high, high);
+    }
+    __syncthreads();
+    low = s_low;
+    high = s_high;
+    if (high == 0) return 0u;
+    // the bits that all of them have in common are the bound's
+    const int bits = low == high ? 0 : 32 - __clz(low ^ high);
+    uint32_t reach = bits == 32 ? 0u : low >> bits << bits;
+    bool any = false;
+    for (int bit = bits - 1; bit >= 0; --bit) {
+      const uint32_t c = reach | (1u << bit);
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < MOST; ++i) count += __popc(__ballot_sync(0xffffffffu, mine[i] >= c));
+      if (lane == 0 && count > 0) atomicAdd(s_tally + bit, count);
+      __syncthreads();
+      const int all = s_tally[bit];
+      if (all < enough) continue;
+      reach = c;
+      any = true;
+      if (all <= most) break;
+    }
+    return any ? reach : 0u;
+  };
   // ---- a bound that at least K + 1 of the entries reach ----
   uint32_t t = 0;
   {
     uint32_t mine[MOST];
 #pragma unroll
     for (int i = 0; i < MOST; ++i) mine[i] = head[i] != 0 ? ordered(static_cast<float>(candidate(of[i], head[i]).score)) : 0u;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t c = t | (1u << bit);
-      int reach = 0;
-#pragma unroll
-      for (int i = 0; i < MOST; ++i) reach += __popc(__ballot_sync(0xffffffffu, mine[i] >= c));
-      if (lane == 0 && reach > 0) atomicAdd(s_tally + bit, reach);
-      __syncthreads();
-      const int all = s_tally[bit];
-      if (all >= K + 1) t = c;
-      if (all >= K + 1 && all <= K + 1 + K / 4) break;
-    }
+    t = reached(mine, K + 1, K + 16);
   }
   // (a little lower: what lies as near as the sums' error belongs to it)
-  double least = -INFINITY;
-  if (t > 0x00800000u) least = static_cast<double>(number_of(t)) - 2 * BS_NEAR - 2.4e-7 * fabs(static_cast<double>(number_of(t)));
-  // ---- the entries that reach it: a warp takes a list, 32 entries at a time ----
-  for (int list = warp; list < lists; list += WARPS) {
-    const int b = beam_of(list);
-    for (int d = 0;; d += 32) {
-      const uint64_t key = key_at(b, list, d + lane);
-      Candidate c{};
-      bool reaches = key != 0;
-      if (reaches) {
-        c = candidate(b, key);
-        reaches = c.score >= least;
+  auto below = [&](uint32_t reach) {
+    if (reach <= 0x00800000u) return static_cast<double>(-INFINITY);
+    const double x = number_of(reach);
+    return x - 2 * BS_NEAR - 2.4e-7 * fabs(x);
+  };
+  double least = below(t);
+  // ---- the entries that reach it ----
+  if (all_here) {
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      if (head[i] == 0) continue;
+      const Candidate c = candidate(of[i], head[i]);
+      if (c.score >= least) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < BS_COLLECT) s_got[at] = c;
       }
-      const unsigned all = __ballot_sync(0xffffffffu, reaches);
-      int at = 0;
-      if (lane == 0 && all != 0) at = atomicAdd(&s_count, __popc(all));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
-      if (reaches && at < BS_COLLECT) s_got[at] = c;
-      if (all != 0xffffffffu) break;
+    }
+  } else {
+    // of the lists whose first entry does; a warp takes a list, 32 entries at a time
+#pragma unroll
+    for (int i = 0; i < MOST; ++i)
+      if (tid + i * BP_THREADS < lists && head[i] != 0 && candidate(of[i], head[i]).score >= least) {
+        const int at = atomicAdd(&s_reach, 1);
+        if (at < BP_LISTS) s_list[at] = tid + i * BP_THREADS;
+      }
+    __syncthreads();
+    const int reach = s_reach;
+    if (reach <= BP_LISTS) {
+      for (int l = warp; l < reach; l += WARPS) {
+        const int list = s_list[l], b = beam_of(list);
+        for (int d = 0; d < K; d += 32) {
+          const uint64_t key = key_at(b, list, d + lane);
+          Candidate c{};
+          bool reaches = key != 0;
+          if (reaches) {
+            c = candidate(b, key);
+            reaches = c.score >= least;
+          }
+          const unsigned all = __ballot_sync(0xffffffffu, reaches);
+          int at = 0;
+          if (lane == 0 && all != 0) at = atomicAdd(&s_count, __popc(all));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
+          if (reaches && at < BS_COLLECT) s_got[at] = c;
+          if (all != 0xffffffffu) break;
+        }
+      }
+    } else if (tid == 0) {
+      s_count = BS_COLLECT + 1;
+    }
+    __syncthreads();
+    // most lists are short of it and some hold much: the bound again, of what they hold
+    const int held = s_count;
+    if (held > BP_RANKED && held <= BS_COLLECT) {
+      uint32_t mine[MOST];
+#pragma unroll
+      for (int i = 0; i < MOST; ++i) mine[i] = tid + i * BP_THREADS < held ? ordered(static_cast<float>(s_got[tid + i * BP_THREADS].score)) : 0u;
+      if (tid < 32) s_tally[tid] = 0;
+      if (tid == 0) {
+        s_low = 0xffffffffu;
+        s_high = s_count = 0;
+      }
+      __syncthreads();
+      least = below(reached(mine, K + 1, K + 16));
+      constexpr int KEPT = BS_COLLECT / BP_THREADS;
+      Candidate kept[KEPT];
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i)
+        if (tid + i * BP_THREADS < held) kept[i] = s_got[tid + i * BP_THREADS];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i)
+        if (tid + i * BP_THREADS < held && kept[i].score >= least) s_got[atomicAdd(&s_count, 1)] = kept[i];
     }
   }
   __syncthreads();
@@ -532,15 +714,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     for (int b = 0; b < B; ++b) {
       if (!s_again[b] || s_kind[b] != 2) continue;
       const T* p = static_cast<const T*>(s.logits) + (row0 + b) * s.ld;
-      if (warp == 0) {
-        float top = -INFINITY;
-        for (int i = lane; i < s_parts[b + 1] - s_parts[b]; i += 32) top = fmaxf(top, s.maxima[static_cast<int64_t>(row0 + b) * s.parts + i]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (lane == 0) s_top = top;
-      }
-      __syncthreads();
-      const double top = s_top;
+      const double top = s_ref[b] * LN2_64;
       double all = 0.0;
 #pragma unroll 4
       for (int i = tid; i < s.vocab; i += BP_THREADS) all += exp(static_cast<double>(Logits<T>::one(p + i)) - top);
@@ -847,7 +1021,7 @@ int configure_once() {
 
 struct SelectPlan {
   int tiles, grid, parts, capacity;
-  int64_t keys_bytes, sums_bytes, bytes;
+  int64_t keys_bytes, bytes;
 };
 SelectPlan plan_select(int num_sms, int rows, int vocab, int picks, bool fp32) {
   SelectPlan p;
@@ -860,8 +1034,7 @@ SelectPlan plan_select(int num_sms, int rows, int vocab, int picks, bool fp32) {
   p.parts = static_cast<int>(std::min<int64_t>(p.tiles, (p.tiles + least - 1) / std::max<int64_t>(1, least) + 1));
   p.capacity = picks * (fp32 ? 4 : 8) * BS_VECTORS + 256;  // (K threads' logits reach the bound of a first tile, or more where they are equal)
   p.keys_bytes = (static_cast<int64_t>(rows) * p.parts * picks * 8 + 15) / 16 * 16;
-  p.sums_bytes = (static_cast<int64_t>(rows) * p.parts * 8 + 15) / 16 * 16;
-  p.bytes = p.keys_bytes + p.sums_bytes + static_cast<int64_t>(rows) * p.parts * 4;
+  p.bytes = p.keys_bytes + static_cast<int64_t>(rows) * p.parts * static_cast<int64_t>(sizeof(double2));
   return p;
 }
 
@@ -888,7 +1061,7 @@ int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n,
   const SelectPlan p = plan_select(ctx->num_sms, n * beams, vocab, picks, fp32 != 0);
   char* ws = static_cast<char*>(workspace);
   const ScanArgs s{logits, ld, n * beams, beams, vocab, picks, p.tiles, p.parts, p.capacity, scores, finished, reinterpret_cast<uint64_t*>(ws),
-                   reinterpret_cast<float*>(ws + p.keys_bytes + p.sums_bytes), reinterpret_cast<double*>(ws + p.keys_bytes)};
+                   reinterpret_cast<double2*>(ws + p.keys_bytes)};
   const PickArgs k{s, p.grid, eos_token, scores_out, parents_out, tokens_out, finished_out};
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
   const size_t smem = static_cast<size_t>(p.capacity) * 8;
