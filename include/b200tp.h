@@ -559,7 +559,7 @@ int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, 
  * A beam whose score is -inf or NaN has no continuation.  A beam with finished (NULL: none) set has one: itself, with its score and token -1.  A logit of -inf or NaN is no continuation;
  * +inf counts as the type's largest number.  Places for which there are no continuations: score -inf, parent -1, token -1, not finished.
  * finished_out: the parent is finished or the token is eos_token (-1: none).
- * beams <= 32, picks <= 64, n * beams <= 2^24.  b2_beam_select_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant;
+ * beams <= 32, picks <= 64, n * beams <= 2^24, logits of less than 2^42 bytes.  b2_beam_select_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant;
  * calls that may run at the same time need one each), or -1 where the shape is not served. */
 int64_t b2_beam_select_workspace(b2_ctx* ctx, int n, int beams, int vocab, int picks, int fp32);
 int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n, int beams, int vocab, const float* scores, const uint8_t* finished, int picks,

@@ -9,37 +9,40 @@ namespace {
 // ---------------------------------------------------------------------------
 // beam_scan_kernel, beam_pick_kernel
 //
-// A continuation of beam b by token v has the score s_b + x_bv - log sum_u exp x_bu.  Within a beam the order is that of the logits, so that
-// one pass over them gives all that is needed: the running maximum and sum of each row, and its K best tokens.
+// A continuation of beam b by token v has the score s_b + x_bv - log sum_u exp x_bu.  One pass over the logits gives the sums, and the largest
+// logit of each chunk of 2 KB.  With those, the K best are in at most K chunks: a chunk that K others have a larger maximum than (or the same, and
+// lie before it) holds none of them.  So the second kernel reads 2 KB for each of about K maxima, and the first does nothing for the selection but to store
+// the maxima.  (Before, the first kernel kept a list of candidates with a rising bound: 33 instructions a logit and threads of a warp that had parted, 53 us
+// for 64 requests of 8 beams over 151936 tokens.)
 //
-// beam_scan_kernel: the rows in tiles of 16 KB, dealt in contiguous equal ranges to the CTAs, so that every SM streams whatever the
-// batch.  A thread keeps its own maximum and sum.  Candidates go to a list in shared memory: of the first tile of a range those that reach
-// the K-th best of the threads' maxima (a lower bound of the K-th best logit), later those above the bound, which rises when the list is cut back
-// to K.  A key is (logit, lowest token first), so that keys are never equal and the list is bounded: a bound that c threads' maxima reach is
-// reached by at most 32 c logits.
+// beam_scan_kernel: the chunks of all rows are dealt to the warps in contiguous equal ranges, so that every SM streams whatever the batch; warps have
+// nothing to do with each other.  Exponentials of the hardware, sums of a thread's 32 or 16 logits of a chunk in 32 bits, and of those in 64.
 //
-// beam_pick_kernel: a CTA per request joins its rows' parts.  Scores are formed in 64 bits.  The sums' error (exponentials of the hardware, sums
-// in 32 bits) could turn the order of continuations of two beams that lie closer than BS_NEAR; where that is so among the K + 1 best, those
-// beams' sums are formed again in 64 bits from the logits.
+// beam_pick_kernel: a CTA per request.  Scores are formed in 64 bits.  The sums' error could turn the order of continuations of two beams that lie
+// closer than BS_NEAR: 2^-22 of an exponential, 2^-20 log(2) of an exponent's rounding where it is below 32 (what lies further down weighs less than 2^-14 even over
+// 2^18 tokens), for each of the two.  Where that is so among the K + 1 best, those beams' sums are formed again in 64 bits from the logits.
 //
 // Bound: HBM, every logit read once.
 // ---------------------------------------------------------------------------
-constexpr int BS_THREADS = 256, BS_VECTORS = 4, BS_CTAS_PER_SM = 4, BS_GROUP = 4;
-constexpr int BS_TILE_BYTES = BS_THREADS * BS_VECTORS * 16;
+constexpr int BS_THREADS = 128, BS_VECTORS = 4, BS_CTAS_PER_SM = 8, BS_WARPS = BS_THREADS / 32;
+constexpr int BS_CHUNK_BYTES = 32 * BS_VECTORS * 16;
 constexpr int BS_MAX_PICKS = 64, BS_MAX_BEAMS = 32;
-constexpr int BP_THREADS = 512, BP_LISTS = 256;
-constexpr int BS_COLLECT = 1536, BP_RANKED = 192;  // candidates that a request collects, and that it ranks without another bound
-constexpr double BS_NEAR = 4e-6;
+constexpr int BP_THREADS = 512, BP_WARPS = BP_THREADS / 32;
+constexpr int BP_CHUNKS = 512, BP_COLLECT = 1536;  // chunks and candidates that a request looks at
+constexpr double BS_NEAR = 2e-6;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr double LOG2E_64 = 1.4426950408889634, LN2_64 = 0.6931471805599453;
+constexpr float BS_PLAIN = 65536.f;  // below this size x log2(e) is formed in 32 bits
+constexpr float BS_ABOVE = 24.f;     // the sum's reference is raised when a logit is this far above it: e^24 a term is far from too much
 
 struct ScanArgs {
   const void* logits;
   int64_t ld;
   int rows, beams, vocab, picks;
-  int tiles, parts;  // per row: tiles, most parts
-  int capacity;      // of the list of candidates
+  int chunks, parts, warps;  // of a row: chunks, most parts; of the scan: warps
   const float* scores;
   const uint8_t* finished;
-  uint64_t* keys;  // [rows][parts][picks], best first, 0: none
+  float* maxima;   // [rows][chunks]
   double2* sums;   // [rows][parts] (M, sum of 2^(x log2(e) - M)); M is a whole number, -inf where there is nothing
 };
 
@@ -48,215 +51,106 @@ __device__ __forceinline__ uint32_t ordered(float x) {  // unsigned order = orde
   return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float number_of(uint32_t o) { return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xffffffffu)); }
-__device__ __forceinline__ uint64_t key_of(float x, int token) { return (static_cast<uint64_t>(ordered(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(token)); }
-__device__ __forceinline__ int token_of(uint64_t key) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)); }
-
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr double LOG2E_64 = 1.4426950408889634, LN2_64 = 0.6931471805599453;
-constexpr float BS_PLAIN = 65536.f;  // below this size x log2(e) is formed in 32 bits
 // 2^x of a whole number x <= 0, exactly; 0 below the normal range (and for NaN, the difference of two -inf)
 __device__ __forceinline__ double power_of_two(double x) { return x > -1023.0 ? __longlong_as_double(static_cast<long long>(1023 + static_cast<int>(x)) << 52) : 0.0; }
 
-// NaN counts as -inf, +inf as the largest number
-__device__ __forceinline__ float plain_number(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
-
+// NaN counts as -inf, +inf as the type's largest number
 template <typename T>
 struct Logits;
 template <>
 struct Logits<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ float most() { return FLT_MAX; }
-  static __device__ __forceinline__ float one(const float* p) { return plain_number(__ldg(p)); }
+  static __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
+  static __device__ __forceinline__ float one(const float* p) { return clean(__ldg(p)); }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x);
     f[1] = __uint_as_float(v.y);
     f[2] = __uint_as_float(v.z);
     f[3] = __uint_as_float(v.w);
   }
-  static __device__ __forceinline__ float largest(const uint4& v) {
-    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  static __device__ __forceinline__ float largest(const uint4 (&v)[BS_VECTORS]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < BS_VECTORS; ++i)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[i].x), __uint_as_float(v[i].y)), fmaxf(__uint_as_float(v[i].z), __uint_as_float(v[i].w))));
+    return m;
   }
 };
 template <>
 struct Logits<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ float most() { return b2::bf16_hi(0x7f7f0000u); }
-  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return fminf(fmaxf(__bfloat162float(*p), -INFINITY), most()); }
+  static __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), b2::bf16_hi(0x7f7f0000u)); }
+  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return clean(__uint_as_float(static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(p))) << 16)); }
   static __device__ __forceinline__ uint32_t max2(uint32_t x, uint32_t y) {
     const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) { b2::unpack8(v, f); }
-  static __device__ __forceinline__ float largest(const uint4& v) {
-    const uint32_t w = max2(max2(v.x, v.y), max2(v.z, v.w));
-    return fmaxf(b2::bf16_lo(w), b2::bf16_hi(w));
+  static __device__ __forceinline__ float largest(const uint4 (&v)[BS_VECTORS]) {
+    uint32_t w = 0xff80ff80u;
+#pragma unroll
+    for (int i = 0; i < BS_VECTORS; ++i) w = max2(w, max2(max2(v[i].x, v[i].y), max2(v[i].z, v[i].w)));
+    return fmaxf(fmaxf(b2::bf16_lo(w), b2::bf16_hi(w)), -INFINITY);
   }
 };
 
-// The 16 bytes at `chunk` (counted from the 16-byte boundary at or before the row), -inf in the places that are not the row's.
+// A row begins anywhere; its chunks are counted from the 16-byte boundary at or before it.
 template <typename T>
-__device__ __noinline__ uint4 load_chunk(const T* row, int vocab, int64_t first) {  // first: the row's element at which the chunk begins, may be < 0
-  constexpr int N = Logits<T>::N;
-  if (first >= 0 && first + N <= vocab) return __ldg(reinterpret_cast<const uint4*>(row + first));
-  uint32_t w[4] = {0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
-  if constexpr (N == 8) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = 0xff80ff80u;
+struct Row {
+  static constexpr int N = Logits<T>::N, CHUNK = BS_CHUNK_BYTES / static_cast<int>(sizeof(T));
+  const T* p;
+  int vocab, shift;
+  __device__ __forceinline__ Row(const ScanArgs& a, int row) : p(static_cast<const T*>(a.logits) + row * a.ld), vocab(a.vocab) {
+    shift = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
   }
-  if (first < vocab && first + N > 0) {
+  // the token of element 0 of lane `lane`'s vector i; may lie before or behind the row
+  __device__ __forceinline__ int token(int chunk, int i, int lane) const { return chunk * CHUNK - shift + (i * 32 + lane) * N; }
+  // (by value: an array would go through memory, and a load would be waited for as soon as it is made)
+  static __device__ __noinline__ uint4 edge(const T* p, int vocab, int first) {
+    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int64_t i = first + e;
-      if (i < 0 || i >= vocab) continue;
+    for (int k = 0; k < 4; ++k) {
       if constexpr (N == 8) {
-        const uint32_t x = __ldg(reinterpret_cast<const unsigned short*>(row) + i);
-        w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xffffu) | (x << 16) : (w[e >> 1] & 0xffff0000u) | x;
+        const int t = first + 2 * k;
+        const uint32_t lo = t >= 0 && t < vocab ? __ldg(reinterpret_cast<const unsigned short*>(p) + t) : 0xff80u;
+        const uint32_t hi = t + 1 >= 0 && t + 1 < vocab ? __ldg(reinterpret_cast<const unsigned short*>(p) + t + 1) : 0xff80u;
+        w[k] = lo | hi << 16;
       } else {
-        w[e] = __float_as_uint(__ldg(reinterpret_cast<const float*>(row) + i));
+        const int t = first + k;
+        w[k] = t >= 0 && t < vocab ? __float_as_uint(__ldg(reinterpret_cast<const float*>(p) + t)) : 0xff800000u;
       }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// The list of candidates of a CTA
-struct List {
-  uint64_t *keys, *best;  // [capacity], [BS_MAX_PICKS]
-  int* count;             // of those that were to go in: may be past the capacity
-  int capacity;
-  __device__ __forceinline__ void push(uint64_t key) const {
-    const int at = atomicAdd(count, 1);
-    if (at < capacity) keys[at] = key;
-  }
-  // All threads: the k best of the n keys stay, in order.  Every thread counts the keys before its own.  Returns how many there are.
-  __device__ __noinline__ int rank(int n, int k) const {
-    for (int i = threadIdx.x; i < n; i += BS_THREADS) {
-      const uint64_t mine = keys[i];
-      int before = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) before += keys[j] > mine ? 1 : 0;
-      if (before < k) best[before] = mine;
+  // a lane's vectors of a chunk, -inf in the places that are not the row's
+  __device__ __forceinline__ void load(int chunk, int lane, uint4 (&v)[BS_VECTORS]) const {
+    const int first = chunk * CHUNK - shift;
+    if (first >= 0 && first + CHUNK <= vocab) {
+      const uint4* q = reinterpret_cast<const uint4*>(p + first) + lane;
+#pragma unroll
+      for (int i = 0; i < BS_VECTORS; ++i) v[i] = __ldg(q + i * 32);
+    } else {
+#pragma unroll
+      for (int i = 0; i < BS_VECTORS; ++i) v[i] = edge(p, vocab, token(chunk, i, lane));
     }
-    __syncthreads();
-    const int left = min(n, k);
-    if (static_cast<int>(threadIdx.x) < left) keys[threadIdx.x] = best[threadIdx.x];
-    if (threadIdx.x == 0) *count = left;
-    __syncthreads();
-    return left;
   }
-  // All threads: those of the n keys stay, in no order, whose logits reach the bound.
-  __device__ __noinline__ int filter(int n, float bound) const {
-    const uint64_t least = static_cast<uint64_t>(ordered(bound)) << 32;
-    if (threadIdx.x == 0) *count = 0;
-    __syncthreads();
-    // in steps of the block: what a step writes lies before what later ones read
-    for (int i0 = 0; i0 < n; i0 += BS_THREADS) {
-      const uint64_t mine = i0 + static_cast<int>(threadIdx.x) < n ? keys[i0 + threadIdx.x] : 0;
-      __syncthreads();
-      if (mine >= least && mine != 0) keys[atomicAdd(count, 1)] = mine;
-      __syncthreads();
+  // sum of 2^(x log2(e) - ref) of a lane's logits, in 64 bits
+  __device__ __noinline__ double exact_sum(int chunk, int lane, double ref) const {
+    double sum = 0.0;
+    for (int i = 0; i < BS_VECTORS * N; ++i) {
+      const int t = token(chunk, i / N, lane) + i % N;
+      if (t >= 0 && t < vocab) sum += exp2(__dmul_rn(Logits<T>::one(p + t), LOG2E_64) - ref);
     }
-    const int left = *count;
-    __syncthreads();
-    return left;
+    return sum;
   }
 };
 
-// (Out of line: rare, or little beside the loop over the tiles, which has to fit the instruction cache.)
-// All threads: the candidates among tokens first .. last, for which there was no room (many equal logits, or a row that rises all along): 256 at a time.
-template <typename T>
-__device__ __noinline__ int overflow(const List list, const T* p, int vocab, int k, int count, int first, int last) {
-  if (threadIdx.x == 0) *list.count = count;
-  __syncthreads();
-  if (count >= k) count = list.rank(count, k);
-  for (; first < last; first += BS_THREADS) {
-    const int token = first + threadIdx.x;
-    const uint64_t least = count >= k ? list.keys[k - 1] : 0;
-    __syncthreads();
-    if (token >= 0 && token < vocab) {
-      const float f = Logits<T>::one(p + token);
-      if (f > -INFINITY && key_of(f, token) > least) list.push(key_of(f, token));
-    }
-    __syncthreads();
-    count = list.rank(*list.count, k);
-  }
-  return count;
-}
-// largest logit of a thread's part of a tile
-template <typename T>
-__device__ __noinline__ float tile_maximum(const T* p, int vocab, int token0) {
-  constexpr int N = Logits<T>::N;
-  float top = -INFINITY;
-  for (int i = 0; i < BS_VECTORS * N; ++i) {
-    const int token = token0 + i / N * (BS_THREADS * N) + i % N;
-    if (token >= 0 && token < vocab) top = fmaxf(top, Logits<T>::one(p + token));
-  }
-  return top;
-}
-// sum of 2^(x log2(e) - ref) over it, in 64 bits
-template <typename T>
-__device__ __noinline__ double exact_sum(const T* p, int vocab, int token0, double ref) {
-  constexpr int N = Logits<T>::N;
-  double sum = 0.0;
-  for (int i = 0; i < BS_VECTORS * N; ++i) {
-    const int token = token0 + i / N * (BS_THREADS * N) + i % N;
-    if (token >= 0 && token < vocab) sum += exp2(__dmul_rn(Logits<T>::one(p + token), LOG2E_64) - ref);
-  }
-  return sum;
-}
-// All threads: a number that the numbers of at least k of them reach, quickly: each warp's ceil(k / warps)-th largest, and the least of those.
-__device__ __noinline__ float reached_by(float x, int k, float* of_warps) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (k + BS_THREADS / 32 - 1) / (BS_THREADS / 32);
-  for (int i = 1; i < each; ++i) {  // the largest is taken out
-    const unsigned best = __reduce_max_sync(0xffffffffu, ordered(x));
-    const unsigned who = __ballot_sync(0xffffffffu, ordered(x) == best);
-    if (lane == __ffs(who) - 1) x = -INFINITY;
-  }
-  const unsigned best = __reduce_max_sync(0xffffffffu, ordered(x));
-  if (lane == 0) of_warps[warp] = number_of(best);
-  __syncthreads();
-  x = of_warps[0];
-#pragma unroll
-  for (int w = 1; w < BS_THREADS / 32; ++w) x = fminf(x, of_warps[w]);
-  __syncthreads();
-  return x;
-}
-// All threads: the k-th largest of one number each.  The warps sort theirs, and every thread finds its own's place in the others.
-__device__ __noinline__ float kth_of_threads(float x, int k, float* sorted, float* found) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-#pragma unroll
-  for (int n = 2; n <= 32; n <<= 1)
-#pragma unroll
-    for (int j = n >> 1; j > 0; j >>= 1) {
-      const float y = __shfl_xor_sync(0xffffffffu, x, j);
-      x = ((lane & j) == 0) == ((lane & n) == 0) ? fmaxf(x, y) : fminf(x, y);
-    }
-  sorted[tid] = x;
-  __syncthreads();
-  int rank = lane;
-  for (int w = 0; w < BS_THREADS / 32; ++w) {
-    if (w == warp) continue;
-    int lo = 0;  // how many of warp w come before
-#pragma unroll
-    for (int step = 16; step > 0; step >>= 1) {
-      const float y = sorted[w * 32 + lo + step - 1];
-      if (y > x || (y == x && w < warp)) lo += step;
-    }
-    const float y = sorted[w * 32 + lo];
-    if (y > x || (y == x && w < warp)) ++lo;
-    rank += lo;
-  }
-  if (rank == k - 1) *found = x;
-  __syncthreads();
-  return *found;
-}
-
-// Ranges of `total` tiles: CTA x of X
+// Ranges of `total` chunks: warp x of X
 struct ScanDeal {
   int base, rem;
   __device__ __forceinline__ ScanDeal(int total, int X) : base(total / X), rem(total % X) {}
   __device__ __forceinline__ int begin_of(int x) const { return x * base + min(x, rem); }
-  __device__ __forceinline__ int cta_of(int t) const {
+  __device__ __forceinline__ int owner_of(int t) const {
     const int big = rem * (base + 1);
     return t < big ? t / (base + 1) : rem + (t - big) / base;
   }
@@ -264,71 +158,44 @@ struct ScanDeal {
 
 template <typename T>
 __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(const ScanArgs a) {
-  constexpr int N = Logits<T>::N, TILE = BS_THREADS * BS_VECTORS * N;
-  extern __shared__ __align__(16) uint64_t s_keys[];
-  __shared__ uint64_t s_best[BS_MAX_PICKS];
-  __shared__ int s_count;
-  __shared__ float s_top[BS_THREADS], s_bound;
-  __shared__ double s_ref[BS_THREADS / 32], s_sum[BS_THREADS / 32];
-  List list{s_keys, s_best, &s_count, a.capacity};
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.picks;
-  const ScanDeal deal(a.rows * a.tiles, gridDim.x);
-  int u = deal.begin_of(blockIdx.x);
-  const int end = deal.begin_of(blockIdx.x + 1);
+  constexpr int N = Logits<T>::N;
+  const int lane = threadIdx.x & 31, x = blockIdx.x * BS_WARPS + b2::uniform(static_cast<int>(threadIdx.x >> 5));
   b2::pdl_launch_dependents();
   b2::pdl_wait();
+  if (x >= a.warps) return;
+  const ScanDeal deal(a.rows * a.chunks, a.warps);
+  int u = deal.begin_of(x);
+  const int end = deal.begin_of(x + 1);
   while (u < end) {
-    const int row = u / a.tiles, t0 = u - row * a.tiles, t1 = min(a.tiles, t0 + end - u);
-    u += t1 - t0;
+    const int row = u / a.chunks, c0 = u - row * a.chunks, c1 = min(a.chunks, c0 + end - u);
+    u += c1 - c0;
     if (!(a.scores[row] > -INFINITY) || (a.finished != nullptr && a.finished[row] != 0)) continue;  // (it has one continuation or none)
-    const int part = blockIdx.x - deal.cta_of(row * a.tiles);  // the CTA that holds the row's first tile is the first of its parts
-    const T* p = static_cast<const T*>(a.logits) + row * a.ld;
-    const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));  // tiles begin at the 16-byte boundary before the row
-    const int limit = max(K + 32, min(2 * K + 64, a.capacity / 2));  // candidates at which the list is cut
-    auto load = [&](int tile, uint4 (&v)[BS_VECTORS]) {
-      const int64_t first = static_cast<int64_t>(tile) * TILE - shift;
-      if (first >= 0 && first + TILE <= a.vocab) {
-        const uint4* q = reinterpret_cast<const uint4*>(p + first) + tid;
-#pragma unroll
-        for (int i = 0; i < BS_VECTORS; ++i) v[i] = __ldg(q + i * BS_THREADS);
-      } else {
-#pragma unroll
-        for (int i = 0; i < BS_VECTORS; ++i) v[i] = load_chunk(p, a.vocab, first + (i * BS_THREADS + tid) * N);
-      }
-    };
+    const Row<T> r(a, row);
     uint4 next[BS_VECTORS];
-    load(t0, next);
-    float bound = INFINITY;     // logits from here on are candidates; not known before the first tile has been read
-    float highest = -INFINITY;  // of the thread's logits
+    r.load(c0, lane, next);
     // The sum's reference is a power of two, so that raising it is exact, and x log2(e) - M is one rounding of an exact product.
     double ref = -INFINITY, sum = 0.0;
-    float ref_low = -INFINITY;  // ref as far as 32 bits go
+    float ref_low = -INFINITY, raise_at = -INFINITY;  // ref as far as 32 bits go; the logit above which it is raised
     auto raise = [&](double to) {
       if (to > ref) {
         sum *= power_of_two(ref - to);
         ref = to;
         ref_low = static_cast<float>(to);
+        raise_at = ref_low * (1.f / LOG2E) + BS_ABOVE;
       }
     };
-    if (tid == 0) s_count = 0;
-    int count = 0;
-    // The first tile, and then BS_GROUP at a time: what they hold is noted by vectors, and looked at when they are through.
-#pragma unroll 1
-    for (int tile = t0; tile < t1;) {
-      const int group = tile, last = tile == t0 ? t0 + 1 : min(t1, tile + BS_GROUP);
-      unsigned reach = 0, odd = 0;  // vectors whose largest reaches the bound; tiles with infinities, NaN or very large numbers
-      float best[BS_VECTORS];
-#pragma unroll 1
-      for (; tile < last; ++tile) {
-        uint4 now[BS_VECTORS];
+    for (int c = c0; c < c1; ++c) {
+      uint4 now[BS_VECTORS];
 #pragma unroll
-        for (int i = 0; i < BS_VECTORS; ++i) now[i] = next[i];
-        if (tile + 1 < t1) load(tile + 1, next);
-#pragma unroll
-        for (int i = 0; i < BS_VECTORS; ++i) best[i] = Logits<T>::largest(now[i]);
-        const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-        const float mine = rintf(top * LOG2E);
-        if (mine > ref_low && top < BS_PLAIN) raise(mine);
+      for (int i = 0; i < BS_VECTORS; ++i) now[i] = next[i];
+      if (c + 1 < c1) r.load(c + 1, lane, next);
+      // (the same in all lanes from here on, but for the sums)
+      const float top = Logits<T>::clean(number_of(__reduce_max_sync(0xffffffffu, ordered(Logits<T>::largest(now)))));
+      if (lane == 0) a.maxima[static_cast<int64_t>(row) * a.chunks + c] = top;
+      if (top == -INFINITY) continue;
+      bool odd = fabsf(top) >= BS_PLAIN;
+      if (!odd) {
+        if (top > raise_at) raise(rintf(top * LOG2E));
         uint64_t sums[2] = {};
         const uint64_t minus = b2::pair_of(-ref_low, -ref_low), scale = b2::pair_of(LOG2E, LOG2E);
 #pragma unroll
@@ -337,95 +204,30 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(c
           Logits<T>::unpack(now[i], f);
 #pragma unroll
           for (int e = 0; e < N; e += 2) {
-            float x, y;
-            b2::fma_pair(x, y, b2::pair_of(f[e], f[e + 1]), scale, minus);
-            sums[(e >> 1) & 1] = b2::add_pair(sums[(e >> 1) & 1], b2::pair_of(b2::ex2(x), b2::ex2(y)));
+            float y, z;
+            b2::fma_pair(y, z, b2::pair_of(f[e], f[e + 1]), scale, minus);
+            sums[(e >> 1) & 1] = b2::add_pair(sums[(e >> 1) & 1], b2::pair_of(b2::ex2(y), b2::ex2(z)));
           }
-          if (best[i] >= bound) reach |= 1u << ((tile - group) * BS_VECTORS + i);
         }
-        float x, y;
-        b2::halves_of(b2::add_pair(sums[0], sums[1]), x, y);
-        // (NaN among the logits makes the sum one; with nothing but -inf so far it is one as well, or has nothing to add)
-        if (fabsf(top) < BS_PLAIN && x + y < INFINITY) sum += x + y;
-        else if (top != -INFINITY) odd |= 1u << (tile - group);
-        highest = fmaxf(highest, top < INFINITY ? top : -INFINITY);
+        float y, z;
+        b2::halves_of(b2::add_pair(sums[0], sums[1]), y, z);
+        odd = __any_sync(0xffffffffu, !(y + z < INFINITY));  // (a NaN among the logits makes the sum one)
+        if (!odd) sum += y + z;
       }
-      // ---- once a group ----
-      for (; odd != 0; odd &= odd - 1) {
-        const int t = __ffs(odd) - 1, token0 = (group + t) * TILE - shift + tid * N;
-        const float top = tile_maximum<T>(p, a.vocab, token0);
-        if (top > -INFINITY) {
-          raise(rint(__dmul_rn(top, LOG2E_64)));
-          sum += exact_sum<T>(p, a.vocab, token0, ref);
-        }
-        highest = fmaxf(highest, top);
-      }
-      if (group == t0) {
-        bound = reached_by(highest, K, s_top);
-        if (bound == -INFINITY) bound = fmaxf(-FLT_MAX, kth_of_threads(highest, K, s_top, &s_bound));
-#pragma unroll
-        for (int i = 0; i < BS_VECTORS; ++i)
-          if (best[i] >= bound) reach |= 1u << i;
-      }
-      for (; reach != 0; reach &= reach - 1) {
-        const int v = __ffs(reach) - 1, token = (group + v / BS_VECTORS) * TILE - shift + (v % BS_VECTORS * BS_THREADS + tid) * N;
-        const uint4 w = load_chunk(p, a.vocab, token);  // (from L2, where it has just been)
-        float f[N];
-        Logits<T>::unpack(w, f);
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (f[e] >= bound) list.push(key_of(fminf(f[e], Logits<T>::most()), token + e));
-      }
-      __syncthreads();
-      const int seen = s_count, fresh = seen - count;
-      __syncthreads();  // (the next group's may go in)
-      if (seen <= a.capacity) {
-        count = seen;
-      } else {
-        count = overflow<T>(list, p, a.vocab, K, count, group * TILE - shift, last * TILE - shift);
-        if (count >= K) bound = fmaxf(bound, number_of(static_cast<uint32_t>(s_keys[K - 1] >> 32) + 1));
-      }
-      if (tile < t1 && fresh > K / 2) {
-        // Later tokens have to be above what K threads have seen: as high, they would come behind those.
-        const float higher = group == t0 && bound > -FLT_MAX ? bound : reached_by(highest, K, s_top);
-        if (higher >= bound) {
-          if (count > limit) count = list.filter(count, higher);
-          bound = number_of(ordered(higher) + 1);
-        }
+      if (odd) {  // infinities, NaN and very large numbers
+        raise(rint(__dmul_rn(top, LOG2E_64)));
+        sum += r.exact_sum(c, lane, ref);
       }
     }
-    // ---- the part: maximum and sum, and the K best in order ----
-    if (count > 2 * K + 32) {
-      const float higher = kth_of_threads(highest, K, s_top, &s_bound);
-      if (higher >= bound) count = list.filter(count, higher);
-    }
-    count = list.rank(count, K);
-    const int64_t at = static_cast<int64_t>(row) * a.parts + part;
-    if (tid < K) a.keys[at * K + tid] = tid < count ? s_keys[tid] : 0;
-    double top = ref;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) s_ref[warp] = top;
-    __syncthreads();
-    top = s_ref[0];
-#pragma unroll
-    for (int w = 1; w < BS_THREADS / 32; ++w) top = fmax(top, s_ref[w]);
-    double all = sum * power_of_two(ref - top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    if (lane == 0) s_sum[warp] = all;
-    __syncthreads();
-    if (tid == 0) {
-      all = 0.0;
-      for (int w = 0; w < BS_THREADS / 32; ++w) all += s_sum[w];
-      a.sums[at] = make_double2(top, all);
-    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    // the warp that holds the row's first chunk is the first of its parts
+    if (lane == 0) a.sums[static_cast<int64_t>(row) * a.parts + x - deal.owner_of(row * a.chunks)] = make_double2(ref, sum);
   }
 }
 
 struct PickArgs {
   ScanArgs scan;
-  int grid;  // of the scan
   int eos;   // -1: none
   float* scores;
   int32_t* parents;
@@ -444,93 +246,48 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 template <typename T>
 __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a) {
   const ScanArgs& s = a.scan;
-  constexpr int WARPS = BP_THREADS / 32;
-  __shared__ double s_total[BS_MAX_BEAMS], s_score[BS_MAX_BEAMS], s_sum[WARPS], s_ref[BS_MAX_BEAMS];
-  __shared__ int s_parts[BS_MAX_BEAMS + 1], s_kind[BS_MAX_BEAMS], s_again[BS_MAX_BEAMS], s_tally[32], s_count, s_any, s_reach, s_list[BP_LISTS];
+  constexpr int N = Logits<T>::N;
+  __shared__ double s_total[BS_MAX_BEAMS], s_score[BS_MAX_BEAMS], s_sum[BP_WARPS], s_ref[BS_MAX_BEAMS], s_power[64];
+  __shared__ int s_kind[BS_MAX_BEAMS], s_again[BS_MAX_BEAMS], s_tally[32], s_count, s_any, s_reach, s_list[BP_CHUNKS];
   __shared__ uint32_t s_low, s_high;
-  __shared__ Candidate s_got[BS_COLLECT], s_best[BS_MAX_PICKS + 1];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = s.beams, K = s.picks, row0 = blockIdx.x * B;
-  const ScanDeal deal(s.rows * s.tiles, a.grid);
+  __shared__ Candidate s_got[BP_COLLECT], s_best[BS_MAX_PICKS + 1];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = s.beams, K = s.picks, row0 = blockIdx.x * B, C = s.chunks;
+  const ScanDeal deal(s.rows * s.chunks, s.warps);
   b2::pdl_launch_dependents();
   b2::pdl_wait();
-  if (warp == 0) {
-    int parts = 0;
-    if (lane < B) {
-      const float score = s.scores[row0 + lane];
-      const bool there = score > -INFINITY, ended = s.finished != nullptr && s.finished[row0 + lane] != 0;
-      s_score[lane] = score;
-      s_kind[lane] = !there ? 0 : ended ? 1 : 2;
-      s_again[lane] = 0;
-      const int first = (row0 + lane) * s.tiles;
-      parts = !there ? 0 : ended ? 1 : deal.cta_of(first + s.tiles - 1) - deal.cta_of(first) + 1;
-    }
+  // ---- each row's sum; the chunks' maxima are on their way meanwhile ----
+  constexpr int MOST = 12;  // of a thread that it keeps
+  float highest[MOST];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, parts, o);
-      if (lane >= o) parts += up;
-    }
-    if (lane < B) s_parts[lane + 1] = parts;
-    if (lane == 0) {
-      s_parts[0] = s_count = s_any = s_reach = 0;
-      s_low = 0xffffffffu;
-      s_high = 0;
-    }
-  }
+  for (int i = 0; i < MOST; ++i) highest[i] = tid + i * BP_THREADS < B * C ? s.maxima[static_cast<int64_t>(row0) * C + tid + i * BP_THREADS] : -INFINITY;
   if (tid < 32) s_tally[tid] = 0;
-  __syncthreads();
-  const int lists = s_parts[B];
-  auto beam_of = [&](int list) {
-    int lo = 0, hi = B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_parts[mid] <= list) lo = mid;
-      else hi = mid - 1;
-    }
-    return lo;
-  };
-  // entry `depth` of a list of beam b: its key, 0 where there is none
-  auto key_at = [&](int b, int list, int depth) -> uint64_t {
-    if (s_kind[b] == 1) return depth == 0 ? 1 : 0;
-    return depth < K ? s.keys[(static_cast<int64_t>(row0 + b) * s.parts + list - s_parts[b]) * K + depth] : 0;
-  };
-  auto candidate = [&](int b, uint64_t key) {
-    if (s_kind[b] == 1) return Candidate{s_score[b], 0.f, b, -1};
-    const float x = number_of(static_cast<uint32_t>(key >> 32));
-    return Candidate{s_score[b] + (static_cast<double>(x) - s_total[b]), x, b, token_of(key)};
-  };
-  // ---- the lists' first entries, while the rows' sums are on their way ----
-  constexpr int MOST = 8;  // entries of a thread
-  const bool all_here = lists * K <= MOST * BP_THREADS;
-  const int deep = lists > 0 ? (all_here ? K : (K + lists) / lists) : 0, n = lists * deep;
-  uint64_t head[MOST];
-  int of[MOST];
-#pragma unroll
-  for (int i = 0; i < MOST; ++i) {
-    const int g = tid + i * BP_THREADS;
-    head[i] = 0;
-    of[i] = 0;
-    if (g < n) {
-      const int list = all_here ? g / K : g % lists;
-      of[i] = beam_of(list);
-      head[i] = key_at(of[i], list, all_here ? g - list * K : g / lists);
-    }
+  if (tid < B) s_again[tid] = 0;
+  if (tid == 0) {
+    s_count = s_any = s_reach = 0;
+    s_low = 0xffffffffu;
+    s_high = 0;
   }
-  for (int b = warp; b < B; b += WARPS) {
-    if (s_kind[b] != 2) continue;
-    const int parts = s_parts[b + 1] - s_parts[b];
-    const double2* sums = s.sums + static_cast<int64_t>(row0 + b) * s.parts;
+  for (int b = warp; b < B; b += BP_WARPS) {
+    const float score = s.scores[row0 + b];
+    const int kind = !(score > -INFINITY) ? 0 : s.finished != nullptr && s.finished[row0 + b] != 0 ? 1 : 2;  // no continuation, itself, all tokens
     double top = -INFINITY, all = 0.0;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-      const double2 mine = i0 + lane < parts ? sums[i0 + lane] : make_double2(-INFINITY, 0.0);
-      double higher = fmax(top, mine.x);
+    if (kind == 2) {
+      const int first = (row0 + b) * C, parts = deal.owner_of(first + C - 1) - deal.owner_of(first) + 1;
+      const double2* sums = s.sums + static_cast<int64_t>(row0 + b) * s.parts;
+      for (int i0 = 0; i0 < parts; i0 += 32) {
+        const double2 mine = i0 + lane < parts ? sums[i0 + lane] : make_double2(-INFINITY, 0.0);
+        double higher = fmax(top, mine.x);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) higher = fmax(higher, __shfl_xor_sync(0xffffffffu, higher, o));
-      all = all * power_of_two(top - higher) + mine.y * power_of_two(mine.x - higher);
-      top = higher;
+        for (int o = 16; o > 0; o >>= 1) higher = fmax(higher, __shfl_xor_sync(0xffffffffu, higher, o));
+        all = all * power_of_two(top - higher) + mine.y * power_of_two(mine.x - higher);
+        top = higher;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     if (lane == 0) {
+      s_score[b] = score;
+      s_kind[b] = kind;
       s_ref[b] = top;
       // log2(e) has 24 bits in the sum's exponents, which makes them this much too large; what carries the sum lies near M
       const double off = fabs(top) < 2 * BS_PLAIN ? top * (static_cast<double>(LOG2E) * LN2_64 - 1.0) : 0.0;
@@ -538,15 +295,71 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     }
   }
   __syncthreads();
-  // All threads: a number that `enough` of the entries reach, and not many more than `most`; 0 where there are not as many.  Entries are 0 where there are none.
-  auto reached = [&](const uint32_t (&mine)[MOST], int enough, int most) {
-    uint32_t low = 0xffffffffu, high = 0;
+  auto score_of = [&](int b, float x) { return s_score[b] + (static_cast<double>(x) - s_total[b]); };
+  // the best score in chunk g of the request, -inf where there is none; a finished beam has one, in its first chunk
+  auto chunk_score = [&](int g, float x) -> double {
+    const int b = g / C, kind = s_kind[b];
+    return kind == 2 ? (x > -INFINITY ? score_of(b, x) : -INFINITY) : kind == 1 && g == b * C ? s_score[b] : -INFINITY;
+  };
+  auto maximum = [&](int g) {
+    const int b = g / C;
+    return s_kind[b] == 2 ? s.maxima[static_cast<int64_t>(row0) * C + g] : -INFINITY;
+  };
+  // All lanes: the continuations in chunk g with a score from `bound` on (and perhaps some a little below) are handed to f.
+  auto each = [&](int g, double bound, auto f) {
+    const int b = g / C;
+    if (s_kind[b] == 1) {
+      if (lane == 0) f(Candidate{s_score[b], 0.f, b, -1});
+      return;
+    }
+    const Row<T> r(s, row0 + b);
+    uint4 v[BS_VECTORS];
+    r.load(g - b * C, lane, v);
+    const float x0 = fmaxf(-FLT_MAX, __double2float_rd(bound - s_score[b] + s_total[b]));  // (what is forbidden is no continuation)
 #pragma unroll
-    for (int i = 0; i < MOST; ++i)
+    for (int i = 0; i < BS_VECTORS; ++i) {
+      float x[N];
+      Logits<T>::unpack(v[i], x);
+      unsigned some = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) some |= x[e] >= x0 ? 1u << e : 0u;
+      for (; some != 0; some &= some - 1) {
+        const int e = __ffs(some) - 1;
+        float y = x[0];
+#pragma unroll
+        for (int k = 1; k < N; ++k) y = e == k ? x[k] : y;
+        y = Logits<T>::clean(y);
+        f(Candidate{score_of(b, y), y, b, r.token(g - b * C, i, lane) + e});
+      }
+    }
+    __syncwarp();
+  };
+
+  // ---- a bound that at least K + 1 chunks' maxima reach, and not many more ----
+  double least = -INFINITY;
+  {
+    uint32_t mine[MOST], low = 0xffffffffu, high = 0;
+    auto value = [&](int g, float x) {
+      const double score = chunk_score(g, x);
+      return score > -INFINITY ? ordered(static_cast<float>(score)) : 0u;
+    };
+    const int n = B * C;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      const int g = tid + i * BP_THREADS;
+      mine[i] = g < n ? value(g, highest[i]) : 0u;
       if (mine[i] != 0) {
         low = min(low, mine[i]);
         high = max(high, mine[i]);
       }
+    }
+    for (int g = tid + MOST * BP_THREADS; g < n; g += BP_THREADS) {  // (very large vocabularies)
+      const uint32_t o = value(g, maximum(g));
+      if (o != 0) {
+        low = min(low, o);
+        high = max(high, o);
+      }
+    }
     low = __reduce_min_sync(0xffffffffu, low);
     high = __reduce_max_sync(0xffffffffu, high);
     if (lane == 0 && high != 0) {
@@ -556,187 +369,168 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     __syncthreads();
     low = s_low;
     high = s_high;
-    if (high == 0) return 0u;
     // the bits that all of them have in common are the bound's
-    const int bits = low == high ? 0 : 32 - __clz(low ^ high);
-    uint32_t reach = bits == 32 ? 0u : low >> bits << bits;
+    const int bits = low >= high ? 0 : 32 - __clz(low ^ high);
+    uint32_t reach = bits == 32 || high == 0 ? 0u : low >> bits << bits;
     bool any = false;
     for (int bit = bits - 1; bit >= 0; --bit) {
       const uint32_t c = reach | (1u << bit);
       int count = 0;
 #pragma unroll
-      for (int i = 0; i < MOST; ++i) count += __popc(__ballot_sync(0xffffffffu, mine[i] >= c));
+      for (int i = 0; i < MOST; ++i) count += mine[i] >= c ? 1 : 0;
+      for (int g = tid + MOST * BP_THREADS; g < n; g += BP_THREADS) count += value(g, maximum(g)) >= c ? 1 : 0;
+      count = __reduce_add_sync(0xffffffffu, count);
       if (lane == 0 && count > 0) atomicAdd(s_tally + bit, count);
       __syncthreads();
       const int all = s_tally[bit];
-      if (all < enough) continue;
+      if (all < K + 1) continue;
       reach = c;
       any = true;
-      if (all <= most) break;
+      if (all <= K + 16) break;
     }
-    return any ? reach : 0u;
-  };
-  // ---- a bound that at least K + 1 of the entries reach ----
-  uint32_t t = 0;
-  {
-    uint32_t mine[MOST];
-#pragma unroll
-    for (int i = 0; i < MOST; ++i) mine[i] = head[i] != 0 ? ordered(static_cast<float>(candidate(of[i], head[i]).score)) : 0u;
-    t = reached(mine, K + 1, K + 16);
-  }
-  // (a little lower: what lies as near as the sums' error belongs to it)
-  auto below = [&](uint32_t reach) {
-    if (reach <= 0x00800000u) return static_cast<double>(-INFINITY);
-    const double x = number_of(reach);
-    return x - 2 * BS_NEAR - 2.4e-7 * fabs(x);
-  };
-  double least = below(t);
-  // ---- the entries that reach it ----
-  if (all_here) {
+    // (a little lower: what lies as near as the sums' error belongs to it)
+    if (any && reach > 0x00800000u) {
+      const double t = number_of(reach);
+      least = t - 2 * BS_NEAR - 2.4e-7 * fabs(t);
+    }
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
-      if (head[i] == 0) continue;
-      const Candidate c = candidate(of[i], head[i]);
-      if (c.score >= least) {
-        const int at = atomicAdd(&s_count, 1);
-        if (at < BS_COLLECT) s_got[at] = c;
-      }
-    }
-  } else {
-    // of the lists whose first entry does; a warp takes a list, 32 entries at a time
-#pragma unroll
-    for (int i = 0; i < MOST; ++i)
-      if (tid + i * BP_THREADS < lists && head[i] != 0 && candidate(of[i], head[i]).score >= least) {
+      const int g = tid + i * BP_THREADS;
+      if (mine[i] != 0 && chunk_score(g, highest[i]) >= least) {
         const int at = atomicAdd(&s_reach, 1);
-        if (at < BP_LISTS) s_list[at] = tid + i * BP_THREADS;
+        if (at < BP_CHUNKS) s_list[at] = g;
       }
-    __syncthreads();
-    const int reach = s_reach;
-    if (reach <= BP_LISTS) {
-      for (int l = warp; l < reach; l += WARPS) {
-        const int list = s_list[l], b = beam_of(list);
-        for (int d = 0; d < K; d += 32) {
-          const uint64_t key = key_at(b, list, d + lane);
-          Candidate c{};
-          bool reaches = key != 0;
-          if (reaches) {
-            c = candidate(b, key);
-            reaches = c.score >= least;
-          }
-          const unsigned all = __ballot_sync(0xffffffffu, reaches);
-          int at = 0;
-          if (lane == 0 && all != 0) at = atomicAdd(&s_count, __popc(all));
-          at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
-          if (reaches && at < BS_COLLECT) s_got[at] = c;
-          if (all != 0xffffffffu) break;
-        }
-      }
-    } else if (tid == 0) {
-      s_count = BS_COLLECT + 1;
     }
-    __syncthreads();
-    // most lists are short of it and some hold much: the bound again, of what they hold
-    const int held = s_count;
-    if (held > BP_RANKED && held <= BS_COLLECT) {
-      uint32_t mine[MOST];
-#pragma unroll
-      for (int i = 0; i < MOST; ++i) mine[i] = tid + i * BP_THREADS < held ? ordered(static_cast<float>(s_got[tid + i * BP_THREADS].score)) : 0u;
-      if (tid < 32) s_tally[tid] = 0;
-      if (tid == 0) {
-        s_low = 0xffffffffu;
-        s_high = s_count = 0;
+    for (int g = tid + MOST * BP_THREADS; g < n; g += BP_THREADS) {
+      const double score = chunk_score(g, maximum(g));
+      if (score > -INFINITY && score >= least) {
+        const int at = atomicAdd(&s_reach, 1);
+        if (at < BP_CHUNKS) s_list[at] = g;
       }
-      __syncthreads();
-      least = below(reached(mine, K + 1, K + 16));
-      constexpr int KEPT = BS_COLLECT / BP_THREADS;
-      Candidate kept[KEPT];
-#pragma unroll
-      for (int i = 0; i < KEPT; ++i)
-        if (tid + i * BP_THREADS < held) kept[i] = s_got[tid + i * BP_THREADS];
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < KEPT; ++i)
-        if (tid + i * BP_THREADS < held && kept[i].score >= least) s_got[atomicAdd(&s_count, 1)] = kept[i];
     }
   }
   __syncthreads();
-  const int got = s_count, best = min(got, K + 1);
-  auto rank_all = [&]() {
-    for (int i = tid; i < got; i += BP_THREADS) {
-      const Candidate mine = s_got[i];
-      int rank = 0;
+
+  // ---- a row's sum in 64 bits ----
+  // (a multiple of 1 / 64 in the exponent from the table, the rest of at most 1 / 128 by the series: the table-driven exponential of P. T. P. Tang)
+  auto sum_again = [&](int b) {
+    const T* p = static_cast<const T*>(s.logits) + (row0 + b) * s.ld;
+    const double ref = s_ref[b];
+    double all = 0.0;
 #pragma unroll 4
-      for (int k = 0; k < got; ++k) {
-        const double other = s_got[k].score;
-        rank += other > mine.score || (other == mine.score && before(s_got[k], mine)) ? 1 : 0;
+    for (int i = tid; i < s.vocab; i += BP_THREADS) {
+      const double t = __dmul_rn(Logits<T>::one(p + i), LOG2E_64) - ref, k = rint(t * 64.0), d = (t - k * (1.0 / 64.0)) * LN2_64;
+      if (t > -64.0) {
+        const int n = static_cast<int>(k);
+        all += s_power[n & 63] * __longlong_as_double(static_cast<long long>(1023 + (n >> 6)) << 52) * (1.0 + d * (1.0 + d * (0.5 + d * (1.0 / 6.0 + d * (1.0 / 24.0)))));
       }
-      if (rank < K + 1) s_best[rank] = mine;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) s_sum[warp] = all;
+    __syncthreads();
+    if (tid == 0) {
+      all = 0.0;
+      for (int w = 0; w < BP_WARPS; ++w) all += s_sum[w];
+      s_total[b] = ref * LN2_64 + log(all);
     }
     __syncthreads();
   };
-  // More than can be ranked at once (equal scores, or a few long lists): the K + 1 best one after the other.
-  auto one_by_one = [&]() {
-    Candidate last{INFINITY, 0.f, -1, -2};
-    for (int k = 0; k < best; ++k) {
-      Candidate mine{-INFINITY, 0.f, BS_MAX_BEAMS, 0x7fffffff};
-      for (int g = tid; g < lists * K; g += BP_THREADS) {
-        const int b = beam_of(g / K);
-        const uint64_t key = key_at(b, g / K, g % K);
-        if (key == 0) continue;
-        const Candidate c = candidate(b, key);
-        if (before(last, c) && before(c, mine)) mine = c;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const Candidate other{__shfl_xor_sync(0xffffffffu, mine.score, o), __shfl_xor_sync(0xffffffffu, mine.x, o), __shfl_xor_sync(0xffffffffu, mine.beam, o),
-                              __shfl_xor_sync(0xffffffffu, mine.token, o)};
-        if (before(other, mine)) mine = other;
-      }
-      if (lane == 0) s_got[warp] = mine;
-      __syncthreads();
-      last = s_got[0];
-      for (int w = 1; w < WARPS; ++w)
-        if (before(s_got[w], last)) last = s_got[w];
-      if (tid == 0) s_best[k] = last;
-      __syncthreads();
-    }
+  auto fill_powers = [&]() {
+    if (tid < 64) s_power[tid] = exp2(tid / 64.0);
+    __syncthreads();
   };
-  const bool many = got > BS_COLLECT;
-  if (many) one_by_one();
-  else rank_all();
+  // All threads: the first of what each has, in s_got[0]
+  auto first_of_all = [&](Candidate mine) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Candidate other{__shfl_xor_sync(0xffffffffu, mine.score, o), __shfl_xor_sync(0xffffffffu, mine.x, o), __shfl_xor_sync(0xffffffffu, mine.beam, o),
+                            __shfl_xor_sync(0xffffffffu, mine.token, o)};
+      if (before(other, mine)) mine = other;
+    }
+    __syncthreads();
+    if (lane == 0) s_got[warp] = mine;
+    __syncthreads();
+    mine = s_got[0];
+    for (int w = 1; w < BP_WARPS; ++w)
+      if (before(s_got[w], mine)) mine = s_got[w];
+    return mine;
+  };
+  const Candidate nothing{-INFINITY, 0.f, BS_MAX_BEAMS, 0x7fffffff};
+  int reach = s_reach;
+  bool exact = false;
+  if (reach > BP_CHUNKS) {
+    // Many chunks with the same maximum: all rows' sums in 64 bits, with which the first K + 1 chunks are sure, one after the other.
+    fill_powers();
+    for (int b = 0; b < B; ++b)
+      if (s_kind[b] == 2 && s_ref[b] > -INFINITY) sum_again(b);
+    exact = true;
+    least = -INFINITY;
+    Candidate last{INFINITY, 0.f, -1, -2};
+    for (reach = 0; reach < K + 1; ++reach) {
+      Candidate mine = nothing;
+      for (int g = tid; g < B * C; g += BP_THREADS) {
+        const Candidate c{chunk_score(g, maximum(g)), 0.f, g / C, g};
+        if (c.score > -INFINITY && before(last, c) && before(c, mine)) mine = c;
+      }
+      last = first_of_all(mine);
+      if (!(last.score > -INFINITY)) break;
+      if (tid == 0) s_list[reach] = last.token;
+    }
+    __syncthreads();
+  }
+  // ---- their continuations that reach the bound ----
+  for (int l = warp; l < reach; l += BP_WARPS)
+    each(s_list[l], least, [&](const Candidate& c) {
+      const int at = atomicAdd(&s_count, 1);
+      if (at < BP_COLLECT) s_got[at] = c;
+    });
+  __syncthreads();
+  const int got = s_count, best = min(got, K + 1);
+  const bool many = got > BP_COLLECT;
+  auto rank_all = [&]() {
+    if (!many) {
+      for (int i = tid; i < got; i += BP_THREADS) {
+        const Candidate mine = s_got[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int k = 0; k < got; ++k) {
+          const double other = s_got[k].score;
+          rank += other > mine.score || (other == mine.score && before(s_got[k], mine)) ? 1 : 0;
+        }
+        if (rank < K + 1) s_best[rank] = mine;
+      }
+    } else {
+      // more than can be ranked at once (equal logits, or chunks that hold many of the best): the K + 1 best one after the other
+      Candidate last{INFINITY, 0.f, -1, -2};
+      for (int k = 0; k < best; ++k) {
+        Candidate mine = nothing;
+        for (int l = warp; l < reach; l += BP_WARPS)
+          each(s_list[l], -INFINITY, [&](const Candidate& c) {
+            if (before(last, c) && before(c, mine)) mine = c;
+          });
+        last = first_of_all(mine);
+        if (tid == 0) s_best[k] = last;
+      }
+    }
+    __syncthreads();
+  };
+  rank_all();
   // ---- continuations of different beams that are too near each other: those beams' sums in 64 bits ----
-  if (tid + 1 < best) {
+  if (!exact && tid + 1 < best) {
     const Candidate &c = s_best[tid], &d = s_best[tid + 1];
     if (c.beam != d.beam && c.score - d.score <= BS_NEAR && (s_kind[c.beam] == 2 || s_kind[d.beam] == 2)) s_again[c.beam] = s_again[d.beam] = s_any = 1;
   }
   __syncthreads();
   if (s_any) {
-    for (int b = 0; b < B; ++b) {
-      if (!s_again[b] || s_kind[b] != 2) continue;
-      const T* p = static_cast<const T*>(s.logits) + (row0 + b) * s.ld;
-      const double top = s_ref[b] * LN2_64;
-      double all = 0.0;
-#pragma unroll 4
-      for (int i = tid; i < s.vocab; i += BP_THREADS) all += exp(static_cast<double>(Logits<T>::one(p + i)) - top);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-      if (lane == 0) s_sum[warp] = all;
-      __syncthreads();
-      if (tid == 0) {
-        all = 0.0;
-        for (int w = 0; w < WARPS; ++w) all += s_sum[w];
-        s_total[b] = top + log(all);
-      }
-      __syncthreads();
-    }
-    if (many) {
-      one_by_one();
-    } else {
+    fill_powers();
+    for (int b = 0; b < B; ++b)
+      if (s_again[b] && s_kind[b] == 2) sum_again(b);
+    if (!many)
       for (int i = tid; i < got; i += BP_THREADS)
-        if (s_kind[s_got[i].beam] == 2) s_got[i].score = s_score[s_got[i].beam] + (static_cast<double>(s_got[i].x) - s_total[s_got[i].beam]);
-      __syncthreads();
-      rank_all();
-    }
+        if (s_kind[s_got[i].beam] == 2) s_got[i].score = score_of(s_got[i].beam, s_got[i].x);
+    __syncthreads();
+    rank_all();
   }
   if (tid < K) {
     const bool there = tid < best && s_best[tid].score > -INFINITY;
@@ -1020,21 +814,20 @@ int configure_once() {
 }
 
 struct SelectPlan {
-  int tiles, grid, parts, capacity;
-  int64_t keys_bytes, bytes;
+  int chunks, warps, parts;
+  int64_t maxima_bytes, bytes;
 };
-SelectPlan plan_select(int num_sms, int rows, int vocab, int picks, bool fp32) {
+SelectPlan plan_select(int num_sms, int rows, int vocab, bool fp32) {
   SelectPlan p;
   // (a row may begin anywhere between two 16-byte boundaries)
-  const int64_t size = fp32 ? 4 : 2, chunks = (vocab * size + 16 - size + 15) / 16;
-  p.tiles = static_cast<int>(std::max<int64_t>(1, (chunks * 16 + BS_TILE_BYTES - 1) / BS_TILE_BYTES));
-  const int64_t total = static_cast<int64_t>(rows) * p.tiles;
-  p.grid = static_cast<int>(std::min<int64_t>(total, static_cast<int64_t>(num_sms) * BS_CTAS_PER_SM));
-  const int64_t least = total / std::max(1, p.grid);  // tiles of the shortest range
-  p.parts = static_cast<int>(std::min<int64_t>(p.tiles, (p.tiles + least - 1) / std::max<int64_t>(1, least) + 1));
-  p.capacity = picks * (fp32 ? 4 : 8) * BS_VECTORS + 256;  // (K threads' logits reach the bound of a first tile, or more where they are equal)
-  p.keys_bytes = (static_cast<int64_t>(rows) * p.parts * picks * 8 + 15) / 16 * 16;
-  p.bytes = p.keys_bytes + static_cast<int64_t>(rows) * p.parts * static_cast<int64_t>(sizeof(double2));
+  const int64_t size = fp32 ? 4 : 2;
+  p.chunks = static_cast<int>((vocab * size + 16 - size + BS_CHUNK_BYTES - 1) / BS_CHUNK_BYTES);
+  const int64_t total = static_cast<int64_t>(rows) * p.chunks;
+  p.warps = static_cast<int>(std::min<int64_t>(total, static_cast<int64_t>(num_sms) * BS_CTAS_PER_SM * BS_WARPS));
+  const int64_t least = std::max<int64_t>(1, total / std::max(1, p.warps));  // chunks of the shortest range
+  p.parts = static_cast<int>(std::min<int64_t>(p.chunks, (p.chunks + least - 1) / least + 1));
+  p.maxima_bytes = (total * 4 + 15) / 16 * 16;
+  p.bytes = p.maxima_bytes + static_cast<int64_t>(rows) * p.parts * static_cast<int64_t>(sizeof(double2));
   return p;
 }
 
@@ -1043,8 +836,10 @@ SelectPlan plan_select(int num_sms, int rows, int vocab, int picks, bool fp32) {
 extern "C" {
 
 int64_t b2_beam_select_workspace(b2_ctx* ctx, int n, int beams, int vocab, int picks, int fp32) {
-  if (ctx == nullptr || n < 0 || beams < 1 || beams > BS_MAX_BEAMS || picks < 1 || picks > BS_MAX_PICKS || vocab < 1 || static_cast<int64_t>(n) * beams > 1 << 24) return -1;
-  return n == 0 ? 0 : plan_select(ctx->num_sms, n * beams, vocab, picks, fp32 != 0).bytes;
+  if (ctx == nullptr || n < 0 || beams < 1 || beams > BS_MAX_BEAMS || picks < 1 || picks > BS_MAX_PICKS || vocab < 1 || vocab > 1 << 30 || static_cast<int64_t>(n) * beams > 1 << 24) return -1;
+  const int64_t chunks = static_cast<int64_t>(vocab) * (fp32 ? 4 : 2) / BS_CHUNK_BYTES + 2;
+  if (chunks * n * beams >= 1ll << 31) return -1;  // (they are counted in 32 bits)
+  return n == 0 ? 0 : plan_select(ctx->num_sms, n * beams, vocab, fp32 != 0).bytes;
 }
 
 int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n, int beams, int vocab, const float* scores, const uint8_t* finished, int picks, int eos_token,
@@ -1053,19 +848,14 @@ int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n,
   if (n == 0) return B2_OK;
   const int64_t need = b2_beam_select_workspace(ctx, n, beams, vocab, picks, fp32);
   if (need < 0) return b2::set_error(B2_ERR_SHAPE, "%d requests of %d beams, %d picks of %d: at most %d beams and %d picks", n, beams, picks, vocab, BS_MAX_BEAMS, BS_MAX_PICKS);
-  const int64_t row_tiles = (static_cast<int64_t>(vocab) * (fp32 ? 4 : 2) + 30) / BS_TILE_BYTES + 1;
-  if (row_tiles * n * beams >= 1ll << 31 || static_cast<int64_t>(vocab) + BS_TILE_BYTES >= 1ll << 31)
-    return b2::set_error(B2_ERR_SHAPE, "%d rows of %d tokens", n * beams, vocab);
   if (!logits || !scores || !scores_out || !parents_out || !tokens_out || !finished_out || ld < vocab) return B2_ERR_ARG;
   if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)) return B2_ERR_ARG;
-  const SelectPlan p = plan_select(ctx->num_sms, n * beams, vocab, picks, fp32 != 0);
+  const SelectPlan p = plan_select(ctx->num_sms, n * beams, vocab, fp32 != 0);
   char* ws = static_cast<char*>(workspace);
-  const ScanArgs s{logits, ld, n * beams, beams, vocab, picks, p.tiles, p.parts, p.capacity, scores, finished, reinterpret_cast<uint64_t*>(ws),
-                   reinterpret_cast<double2*>(ws + p.keys_bytes)};
-  const PickArgs k{s, p.grid, eos_token, scores_out, parents_out, tokens_out, finished_out};
+  const ScanArgs s{logits, ld, n * beams, beams, vocab, picks, p.chunks, p.parts, p.warps, scores, finished, reinterpret_cast<float*>(ws), reinterpret_cast<double2*>(ws + p.maxima_bytes)};
+  const PickArgs k{s, eos_token, scores_out, parents_out, tokens_out, finished_out};
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
-  const size_t smem = static_cast<size_t>(p.capacity) * 8;
-  B2_CUDA(b2_launch(fp32 ? beam_scan_kernel<float> : beam_scan_kernel<__nv_bfloat16>, dim3(p.grid), dim3(BS_THREADS), smem, on, s));
+  B2_CUDA(b2_launch(fp32 ? beam_scan_kernel<float> : beam_scan_kernel<__nv_bfloat16>, dim3((p.warps + BS_WARPS - 1) / BS_WARPS), dim3(BS_THREADS), 0, on, s));
   B2_CUDA(b2_launch(fp32 ? beam_pick_kernel<float> : beam_pick_kernel<__nv_bfloat16>, dim3(n), dim3(BP_THREADS), 0, on, k));
   return B2_OK;
 }
