@@ -511,7 +511,7 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
  * The sums are kept unnormalised with weights of up to 2^8: 256 * the keys seen * the largest |value| has to stay below the type's maximum (3.4e38).
  * Lengths and tables are read after earlier kernels have completed.  Calls that may run at the same time need a workspace each (16-byte aligned, contents irrelevant).
  * b2_prefix_attention_supported says (1 / 0) whether the shape is served: head_dim 64 or 128, up to 128 query heads per KV head, blocks of
- * a multiple of 16 tokens.  b2_prefix_attention_workspace: bytes, or -1 where the shape is not served; at most 1024 sequences and groups, tables of less than 2^27 tokens. */
+ * a multiple of 16 tokens.  b2_prefix_attention_workspace: bytes, or -1 where the shape is not served; at most 1024 sequences and 512 groups, tables of less than 2^27 tokens. */
 int b2_prefix_attention_supported(int nq, int nkv, int head_dim, int block_size);
 int64_t b2_prefix_attention_workspace(b2_ctx* ctx, int n_seqs, int n_groups, int nq, int nkv, int head_dim, int block_size, int bt_width);
 int b2_prefix_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int num_blocks, int block_size,

@@ -718,8 +718,8 @@ PyObject* shared_prefix_attention(Args a) {
   if (!row_layout(q, nq, hd)) raise(PyExc_AssertionError, "q: heads must lie side by side, in rows on 16-byte boundaries");
   if (!kc.is_contiguous() || !vc.is_contiguous() || !on_16_bytes(kc) || !on_16_bytes(vc)) raise(PyExc_AssertionError, "k_cache and v_cache must be contiguous, on 16-byte boundaries");
   constexpr int64_t limit = (int64_t(1) << 31) - 1;
-  if (kc.size(0) < 1 || kc.size(0) > limit / bs || tables.dim() != 2 || tables.size(1) > ((1 << 27) - 1) / bs || n > 1024 || groups > 1024)
-    raise(PyExc_ValueError, "shared_prefix_attention: %lld blocks, %lld sequences in %lld groups: at most 1024 of both, tables of less than 2^27 tokens", (long long)kc.size(0), (long long)n, (long long)groups);
+  if (kc.size(0) < 1 || kc.size(0) > limit / bs || tables.dim() != 2 || tables.size(1) > ((1 << 27) - 1) / bs || n > 1024 || groups > 512)
+    raise(PyExc_ValueError, "shared_prefix_attention: %lld blocks, %lld sequences in %lld groups: at most 1024 in 512, tables of less than 2^27 tokens", (long long)kc.size(0), (long long)n, (long long)groups);
   vector_of(prefix, at::kInt, groups, "prefix_lens");
   vector_of(cu, at::kInt, groups + 1, "cu_groups");
   vector_of(lens, at::kInt, n, "context_lens");
