@@ -43,7 +43,7 @@ struct Prefix {
   __host__ __device__ static constexpr uint32_t own_q(int h) { return h * 1024 * HALVES; }  // 8 h rows
   __host__ __device__ static constexpr int meet_dims(int h) { return h == 1 ? HD : 32; }    // dimensions that meet at a time
   __host__ __device__ static constexpr uint32_t meet(int h) { return OWN_Q + OWN_STAGES * own_q(h); }
-  __host__ __device__ static constexpr uint32_t plan(int h) { return meet(h) + PO_WARPS * 8 * h * (meet_dims(h) + 8) * 4; }
+  __host__ __device__ static constexpr uint32_t plan(int h) { return meet(h) + PO_WARPS * 8 * h * (meet_dims(h) + 4) * 4; }
   static constexpr size_t smem(int h, int n_seqs, int n_groups) { return 1024 + plan(h) + (2 * n_groups + n_seqs + 2) * sizeof(int) + n_seqs * sizeof(uint16_t); }
 };
 static_assert(Prefix<128>::smem(2, PX_MAX_SEQS, PX_MAX_GROUPS) + 1024 <= 227 * 1024 && Prefix<64>::smem(2, PX_MAX_SEQS, PX_MAX_GROUPS) + 1024 <= 227 * 1024, "a CTA's shared memory (1 KB: static)");
@@ -178,24 +178,27 @@ struct Segment {
 template <bool OWN>
 struct PrefixWalk {
   const Plan plan;
-  int pos, end, at;  // at: group or sequence
-  __device__ __forceinline__ PrefixWalk(const PrefixArgs& a, const Plan& p, int begin, int stop) : plan(p), pos(begin), end(stop) {
+  int pos, end, at, known;  // at: group or sequence; known: the one that the segment is of
+  __device__ __forceinline__ PrefixWalk(const PrefixArgs& a, const Plan& p, int begin, int stop) : plan(p), pos(begin), end(stop), known(-1) {
     at = last_at(OWN ? plan.own_units : plan.common_units, OWN ? a.n_seqs : a.n_groups, pos);
   }
   __device__ __forceinline__ bool next(const PrefixArgs& a, Segment& x) {
     if (pos >= end) return false;
     const int* first = OWN ? plan.own_units : plan.common_units;
     while (first[at + 1] <= pos) ++at;
-    if (OWN) {
-      x.len = length(a, at);
-      x.start = plan.common_tiles(plan.group_of[at]) * PX_KEYS;
-      x.tiles = tiles_of(x.len - x.start);
-      x.table = x.seq = at;
-    } else {
-      x.start = 0;
-      x.tiles = plan.common_tiles(at);
-      x.len = x.tiles * PX_KEYS;
-      x.table = plan.leader(at);
+    if (at != known) {  // (the items of a sequence, or of a group, lie one after the other)
+      known = at;
+      if (OWN) {
+        x.len = length(a, at);
+        x.start = plan.common_tiles(plan.group_of[at]) * PX_KEYS;
+        x.tiles = tiles_of(x.len - x.start);
+        x.table = x.seq = at;
+      } else {
+        x.start = 0;
+        x.tiles = plan.common_tiles(at);
+        x.len = x.tiles * PX_KEYS;
+        x.table = plan.leader(at);
+      }
     }
     const int units = x.tiles + PX_ITEM_UNITS, in = pos - first[at], item = in / units, u0 = in - item * units;
     if (OWN) {
@@ -214,6 +217,10 @@ struct PrefixWalk {
     pos += u1 - u0;
     x.t0 = max(0, u0 - PX_ITEM_UNITS);
     x.t1 = u1 - PX_ITEM_UNITS;
+    // (Coordinates of TMA loads.  In registers of each thread, all of them with the same value, one of two loads of Q took another for its first coordinate: zeros.)
+    x.seq = b2::uniform(x.seq);
+    x.head = b2::uniform(x.head);
+    x.row = b2::uniform(x.row);
     return true;
   }
 };
@@ -477,24 +484,29 @@ __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtens
 }
 
 // ---- the other keys: up to 16 heads of one sequence -----------------------------------------------------------------------------------------
-// Every K and V row is used by the heads of one group only, which would fill a fraction of the tensor core's 128 rows: mma.sync with 8 or 16 rows does as much work as there
-// is.  Bound: HBM.
+// Every K and V row is used by the heads of one group only, which would fill a fraction of the tensor core's 128 rows: mma.sync with the keys (of the scores, S^T = K Q^T) and
+// the dimensions (of the result, O^T = V^T P^T) on its 16 rows and 8 heads on its columns does as much work as there is.  Bound: HBM; a warp's chain of products and exponentials
+// is 0.6 of a tile's time on it.
 //   warps 0..3   16 keys of each tile of 64, each warp with its own maxima, sums and results, which meet at the segment's end
-//   warp 4       TMA: K and V tiles
-__device__ __forceinline__ void mma_rows16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+//   warp 4       TMA: K and V tiles, Q with the first
+__device__ __forceinline__ void mma_16x8(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_rows(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma_rows16(c, a, b0, b1); }
-__device__ __forceinline__ void mma_rows(float (&c)[2], const uint32_t (&a)[2], uint32_t b0, uint32_t b1) { b2::mma_rows8(c[0], c[1], a[0], a[1], b0, b1); }
+// a warp's 8 x 8 matrix of 16-bit numbers, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
-// H: halves of 8 rows; warp: of these
+// H: times 8 heads; warp: of these
 template <int HD, int H>
 __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const PrefixArgs& a, const Plan& plan, unsigned char* smem, uint32_t bars, float (*s_m)[16],
                                          float (*s_l)[16], int warp, volatile int* abort_flag) {
   using T = Prefix<HD>;
-  constexpr int HALVES = T::HALVES, STAGES = T::OWN_STAGES, STEPS = HD / 16, DIMS = T::meet_dims(H), PAD = DIMS + 8;
+  constexpr int HALVES = T::HALVES, STAGES = T::OWN_STAGES, STEPS = HD / 16, DIMS = T::meet_dims(H), PAD = DIMS + 4;
   const uint32_t base = b2::smem_u32(smem), ring = base + T::OWN_RING, s_q = base + T::OWN_Q;
   float* const meet = reinterpret_cast<float*>(smem + T::meet(H));  // [PO_WARPS][8 H][PAD]
   const uint32_t full = bars, empty = full + STAGES * 8, met = empty + STAGES * 8;
@@ -537,10 +549,12 @@ __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorM
         ok = all_wait(empty + st * 8, ((c / STAGES) & 1) ^ 1, B2_WAIT_SMEM_EMPTY);
         if (!ok) break;
         const uint32_t bar = full + st * 8, dst = ring + st * 2 * T::TILE;
-        if (b2::elect_one()) {
-          b2::mbar_arrive_expect_tx(bar, 2 * boxes * a.box * 128 * HALVES + (j == 0 ? 128 * HALVES * min(a.group, 8 * H) : 0));
-          if (j == 0)
+        if (b2::elect_one()) b2::mbar_arrive_expect_tx(bar, 2 * boxes * a.box * 128 * HALVES + (j == 0 ? 128 * HALVES * min(a.group, 8 * H) : 0));
+        __syncwarp();
+        if (j == 0) {
+          if (b2::elect_one())
             for (int h = 0; h < HALVES; ++h) b2::tma_load_3d(s_q + st * T::own_q(H) + h * 1024 * H, &tmQ, bar, h * 64, seg.head * a.group + seg.row, seg.seq, b2::kEvictNormal);
+          __syncwarp();
         }
         for (int i = 0; i < boxes; ++i) {
           const int r = rows.row(j * per_tile + i);
@@ -555,7 +569,7 @@ __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorM
     }
   } else {
     const int g = lane >> 2, t = lane & 3, key0 = warp * 16, swizzle = lane & 7;
-    const uint32_t k_lane = (key0 + (lane & 7) + (lane >> 4) * 8) * 128, v_lane = (key0 + (lane & 15)) * 128;
+    const uint32_t k_lane = (key0 + (lane & 15)) * 128, v_lane = (key0 + (lane & 7) + (lane >> 4) * 8) * 128;
     const int64_t all_rows = static_cast<int64_t>(a.n_seqs) * a.nq;
     uint32_t meetings = 0;
     auto all_here = [&]() {  // the four warps, like a barrier, but bounded
@@ -567,70 +581,79 @@ __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorM
     };
     while (ok && walk.next(a, seg)) {
       if (seg.t0 >= seg.t1) continue;
-      uint32_t qa[STEPS][2 * H];  // (rows behind the last one hold anything, which stays in those rows)
-      float m[H], l[H], o[HD / 8][2 * H];
+      uint32_t qb[STEPS][2 * H];  // (heads behind the last one hold anything, which stays with those heads)
+      float m[2 * H], l[2 * H], o[STEPS][H][4];  // heads 2 t and 2 t + 1 of each 8; dimensions g and g + 8 of each 16
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
+      for (int h = 0; h < 2 * H; ++h) {
         m[h] = -INFINITY;
         l[h] = 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i)
+      for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-        for (int e = 0; e < 2 * H; ++e) o[i][e] = 0.f;
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][h][e] = 0.f;
       const int n = seg.t1 - seg.t0;
       for (int j = 0; j < n; ++j, ++c) {
         const int st = c % STAGES, there = seg.len - seg.start - (seg.t0 + j) * PX_KEYS - key0;  // keys of this warp
         ok = all_wait(full + st * 8, (c / STAGES) & 1, B2_WAIT_SMEM_FULL);
         if (!ok) break;
+        __syncwarp();
         if (j == 0) {
           const uint32_t q_at = s_q + st * T::own_q(H) + (lane & (8 * H - 1)) * 128;
 #pragma unroll
           for (int k = 0; k < STEPS; k += 2 / H) {
-            // 16 rows: a step of 16 dimensions; 8 rows: two steps
+            // 16 heads: a step of 16 dimensions (heads 0 to 7, 8 to 15, the second 8 dimensions of both); 8 heads: two steps
             uint32_t r[4];
             const int chunk = (k & 3) * 2 + (H == 2 ? lane >> 4 : lane >> 3);
             b2::ldmatrix_x4(r, q_at + (k >> 2) * 1024 * H + ((chunk ^ swizzle) << 4));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) qa[H == 2 ? k : k + (e >> 1)][H == 2 ? e : e & 1] = r[e];
+            for (int e = 0; e < 4; ++e) qb[H == 2 ? k : k + (e >> 1)][H == 2 ? e : e & 1] = r[e];
           }
         }
         if (there > 0) {
           const uint32_t k_at = ring + st * 2 * T::TILE + k_lane, v_at = ring + st * 2 * T::TILE + T::TILE + v_lane;
-          float s[2][2 * H] = {};
+          float s[H][4] = {}, s2[H][4] = {};  // (two sums of each, so that a product waits for every other one)
 #pragma unroll
           for (int k = 0; k < STEPS; ++k) {
-            uint32_t b[4];
-            b2::ldmatrix_x4(b, k_at + (k >> 2) * T::HALF + (((((k & 3) * 2) + ((lane >> 3) & 1)) ^ swizzle) << 4));
-            mma_rows(s[0], qa[k], b[0], b[1]);
-            mma_rows(s[1], qa[k], b[2], b[3]);
+            uint32_t ka[4];
+            b2::ldmatrix_x4(ka, k_at + (k >> 2) * T::HALF + (((((k & 3) * 2) + (lane >> 4)) ^ swizzle) << 4));
+#pragma unroll
+            for (int h = 0; h < H; ++h) mma_16x8(k & 1 ? s2[h] : s[h], ka, qb[k][h], qb[k][H + h]);
           }
-          uint32_t p[2 * H];
-          float f[H];
+          uint32_t p[H][2];
+          float f[2 * H];
           bool grown = false;
 #pragma unroll
           for (int h = 0; h < H; ++h) {
-            float v[4] = {s[0][2 * h], s[0][2 * h + 1], s[1][2 * h], s[1][2 * h + 1]};
+            float v[4];  // key g: two heads; key g + 8
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (e >> 1) * 8 + 2 * t + (e & 1) < there ? v[e] * a.signed_log2 : -INFINITY;
-            float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float higher = fmaxf(m[h], top), ref = higher == -INFINITY ? 0.f : higher;
-            f[h] = b2::ex2(m[h] - ref);
-            grown = grown || higher > m[h];
-            m[h] = higher;
+            for (int e = 0; e < 4; ++e) v[e] = (e >> 1) * 8 + g < there ? (s[h][e] + s2[h][e]) * a.signed_log2 : -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = b2::ex2(v[e] - ref);
-            l[h] = l[h] * f[h] + ((v[0] + v[1]) + (v[2] + v[3]));
-            p[H == 2 ? h : 0] = b2::pack_bf16(v[0], v[1]);
-            p[H == 2 ? 2 + h : 1] = b2::pack_bf16(v[2], v[3]);
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(v[e], v[2 + e]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              float &mx = m[2 * h + e], higher = fmaxf(mx, top);
+              const float ref = higher == -INFINITY ? 0.f : higher;
+              f[2 * h + e] = b2::ex2(mx - ref);
+              grown = grown || higher > mx;
+              mx = higher;
+              v[e] = b2::ex2(v[e] - ref);
+              v[2 + e] = b2::ex2(v[2 + e] - ref);
+              l[2 * h + e] = l[2 * h + e] * f[2 * h + e] + (v[e] + v[2 + e]);
+            }
+            p[h][0] = transposed(b2::pack_bf16(v[0], v[1]));
+            p[h][1] = transposed(b2::pack_bf16(v[2], v[3]));
           }
           if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-            for (int i = 0; i < HD / 8; ++i)
+            for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-              for (int e = 0; e < 2 * H; ++e) o[i][e] *= f[e >> 1];
+              for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][h][e] *= f[2 * h + (e & 1)];
           }
           if (there < 16) {
             // rows of V past the context's end may hold anything, and zero times infinity or NaN is NaN: they count as zero
@@ -643,10 +666,10 @@ __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorM
           }
 #pragma unroll
           for (int i = 0; i < STEPS; ++i) {
-            uint32_t b[4];
-            b2::ldmatrix_x4_trans(b, v_at + (i >> 2) * T::HALF + (((((i & 3) * 2) + (lane >> 4)) ^ swizzle) << 4));
-            mma_rows(o[2 * i], p, b[0], b[1]);
-            mma_rows(o[2 * i + 1], p, b[2], b[3]);
+            uint32_t va[4];
+            b2::ldmatrix_x4_trans(va, v_at + (i >> 2) * T::HALF + (((((i & 3) * 2) + ((lane >> 3) & 1)) ^ swizzle) << 4));
+#pragma unroll
+            for (int h = 0; h < H; ++h) mma_16x8(o[i][h], va, p[h][0], p[h][1]);
           }
         }
         __syncwarp();
@@ -655,12 +678,12 @@ __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorM
       if (!ok) break;
       // ---- the warps' results together ----
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if (t == 0) {
-          s_m[warp][h * 8 + g] = m[h];
-          s_l[warp][h * 8 + g] = l[h];
+      for (int h = 0; h < 2 * H; ++h) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
+        if (g == 0) {
+          s_m[warp][(h >> 1) * 8 + 2 * t + (h & 1)] = m[h];
+          s_l[warp][(h >> 1) * 8 + 2 * t + (h & 1)] = l[h];
         }
       }
       ok = all_here();
@@ -671,11 +694,11 @@ __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorM
 #pragma unroll
         for (int w = 0; w < PO_WARPS; ++w) sum += s_l[w][r] * (s_m[w][r] == top ? 1.f : b2::ex2(s_m[w][r] - top));
       };
-      float f[H];
+      float f[2 * H];
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        float top, sum;
-        together(h * 8 + g, top, sum);
+      for (int h = 0; h < 2 * H; ++h) {
+        const int r = (h >> 1) * 8 + 2 * t + (h & 1);
+        const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
         f[h] = m[h] == top ? 1.f : b2::ex2(m[h] - top);
       }
       constexpr int EACH = 8 * H * DIMS / (PO_WARPS * 32);  // dimensions that a thread puts together
@@ -692,41 +715,46 @@ __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorM
           if (!ok) break;
         }
 #pragma unroll
-        for (int i = 0; i < DIMS / 8; ++i)
+        for (int i = 0; i < DIMS / 16; ++i)
 #pragma unroll
           for (int h = 0; h < H; ++h)
-            *reinterpret_cast<float2*>(meet + (warp * 8 * H + h * 8 + g) * PAD + i * 8 + 2 * t) = make_float2(o[d0 / 8 + i][2 * h] * f[h], o[d0 / 8 + i][2 * h + 1] * f[h]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              meet[(warp * 8 * H + h * 8 + 2 * t + (e & 1)) * PAD + i * 16 + (e >> 1) * 8 + g] = o[d0 / 16 + i][h][e] * f[2 * h + (e & 1)];
         ok = all_here();
         if (!ok) break;
-        if (!exists) continue;
-        float v[EACH] = {};
+        if (exists) {
+          float v[EACH] = {};
 #pragma unroll
-        for (int w = 0; w < PO_WARPS; ++w)
+          for (int w = 0; w < PO_WARPS; ++w)
 #pragma unroll
-          for (int e = 0; e < EACH; e += 4) {
-            const float4 y = *reinterpret_cast<const float4*>(meet + (w * 8 * H + r) * PAD + dim + e);
-            v[e] += y.x; v[e + 1] += y.y; v[e + 2] += y.z; v[e + 3] += y.w;
-          }
-        if (direct) {
-          const float inv = sum != 0.f ? 1.f / sum : 0.f;
-          uint16_t* const to = a.out + (static_cast<int64_t>(seg.seq) * a.nq + seg.head * a.group + seg.row + r) * HD + d0 + dim;
+            for (int e = 0; e < EACH; e += 4) {
+              const float4 y = *reinterpret_cast<const float4*>(meet + (w * 8 * H + r) * PAD + dim + e);
+              v[e] += y.x; v[e + 1] += y.y; v[e + 2] += y.z; v[e + 3] += y.w;
+            }
+          if (direct) {
+            const float inv = sum != 0.f ? 1.f / sum : 0.f;
+            uint16_t* const to = a.out + (static_cast<int64_t>(seg.seq) * a.nq + seg.head * a.group + seg.row + r) * HD + d0 + dim;
 #pragma unroll
-          for (int e = 0; e < EACH; e += 4)
-            *reinterpret_cast<uint2*>(to + e) = make_uint2(b2::pack_bf16(v[e] * inv, v[e + 1] * inv), b2::pack_bf16(v[e + 2] * inv, v[e + 3] * inv));
-        } else {
+            for (int e = 0; e < EACH; e += 4)
+              *reinterpret_cast<uint2*>(to + e) = make_uint2(b2::pack_bf16(v[e] * inv, v[e + 1] * inv), b2::pack_bf16(v[e + 2] * inv, v[e + 3] * inv));
+          } else {
 #pragma unroll
-          for (int e = 0; e < EACH; e += 4) {
-            const int quad = (d0 + dim + e) / 4;
-            float* const to = begins ? a.rows_o + (all_rows * HD + (quad * all_rows + at) * 4) : slot + (quad * T::OWN_ROWS + r) * 4;
-            *reinterpret_cast<float4*>(to) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < EACH; e += 4) {
+              const int quad = (d0 + dim + e) / 4;
+              float* const to = begins ? a.rows_o + (all_rows * HD + (quad * all_rows + at) * 4) : slot + (quad * T::OWN_ROWS + r) * 4;
+              *reinterpret_cast<float4*>(to) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            }
           }
         }
+        __syncwarp();
       }
       if (!ok) break;
       if (exists && !direct && dim == 0) {
         (begins ? a.rows_m + all_rows + at : slot + HD * T::OWN_ROWS + r)[0] = top;
         (begins ? a.rows_l + all_rows + at : slot + (HD + 1) * T::OWN_ROWS + r)[0] = sum;
       }
+      __syncwarp();  // (threads that had nothing to store would go on by themselves, and what follows is for whole warps)
     }
   }
 }
