@@ -549,16 +549,17 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
 // block, which the next tokens go to, stays with the first row that has it, and the others get a copy in a block from the stack.  A block that no
 // row has any more goes onto the stack.
 //
-// beam_tables_kernel: a CTA per request; a thread per column of its tables (a row's neighbours are the next thread's, so that the loads are whole
-// lines).  Rows with children hold their blocks; only the blocks of rows without have to be looked for among those (mostly the first looked
-// at has it: a prompt's block).  It leaves the request's copies and given-back blocks in lists, since their places on the stack depend on the requests before.  Further
-// CTAs bring the histories.
-// beam_move_kernel: every CTA forms the prefix sums over the requests' lists, and then does its share of the copies (pieces of 4 KB, a warp
-// each), of the new entries and of the stack.
+// beam_tables_kernel: a CTA per request, 64 to 256 columns of its tables at a time through shared memory; a warp takes a column, a lane a row, and finds the rows
+// that have the same block by a match over the warp.  (A thread per column that compared its rows one after the other: 39 us instead of 11 for seven requests of 29 rows over 400 columns; the other way round with two
+// rows, 12 us instead of 15 for two requests of two rows over 10000 columns, where the walk over the columns is most of it.)  It
+// leaves the request's copies and given-back blocks in lists, since their places on the stack depend on the requests before.  Further CTAs bring the histories.
+// beam_move_kernel: every CTA forms the prefix sums over the requests' lists and looks up what is copied where, and then does its share of the copies (pieces of 4 KB, a
+// warp each), of the new entries and of the stack.
 //
 // Bound: latency for one request; HBM for the copies (every copied token read and written once in all planes) and the histories.
 // ---------------------------------------------------------------------------
-constexpr int BR_THREADS = 256, BR_MAX_ROWS = 8192, BR_PIECE = 4096, BR_HISTORY = 1024;
+constexpr int BR_THREADS = 256, BR_WARPS = BR_THREADS / 32, BR_MAX_ROWS = 8192, BR_PIECE = 4096, BR_HISTORY = 1024, BR_COPIES = 1024;
+constexpr int BT_THREADS = 512, BT_WARPS = BT_THREADS / 32, BT_COLUMNS = 256, BT_ENTRIES = 32 * (64 + 1);  // (8 rows of 257 and 16 of 129 are fewer)
 
 struct ReorderArgs {
   const int32_t* parents;
@@ -586,10 +587,11 @@ struct ReorderArgs {
   int32_t* given;  // [n][beams * bt_width] by column and row
 };
 
-__global__ void __launch_bounds__(BR_THREADS) beam_tables_kernel(const ReorderArgs a) {
+__global__ void __launch_bounds__(BT_THREADS) beam_tables_kernel(const ReorderArgs a) {
   __shared__ int s_p[32], s_len[32], s_have[32], s_need[32], s_first[32], s_open[32];
-  __shared__ int s_x[32][BR_THREADS];
-  __shared__ int s_warp[BR_THREADS / 32];
+  __shared__ int s_x[BT_ENTRIES], s_new[BT_ENTRIES];  // [rows][columns + 1] (a column's rows in as many banks)
+  __shared__ unsigned s_gone[BT_COLUMNS];  // rows whose block no row has any more
+  __shared__ int s_at[BT_COLUMNS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.beams, W = a.bt_width, bs = a.block_size;
   b2::pdl_launch_dependents();
   b2::pdl_wait();
@@ -608,8 +610,8 @@ __global__ void __launch_bounds__(BR_THREADS) beam_tables_kernel(const ReorderAr
       int64_t* out = a.history_out + static_cast<int64_t>(row) * a.history_width;
       const int j1 = min(a.history_width, j0 + BR_HISTORY);
 #pragma unroll
-      for (int e = 0; e < BR_HISTORY / BR_THREADS; ++e) {
-        const int j = j0 + e * BR_THREADS + tid;
+      for (int e = 0; e < BR_HISTORY / BT_THREADS; ++e) {
+        const int j = j0 + e * BT_THREADS + tid;
         if (j < j1) out[j] = j < said ? __ldg(reinterpret_cast<const long long*>(in) + j) : j == said ? token : -1;
       }
       if (j0 == 0 && tid == 0) a.history_lens_out[row] = said + (token >= 0 && said < a.history_width ? 1 : 0);
@@ -630,15 +632,19 @@ __global__ void __launch_bounds__(BR_THREADS) beam_tables_kernel(const ReorderAr
     s_first[tid] = min(a.first != nullptr ? max(0, __ldg(a.first + r)) : 0, s_len[tid] / bs);
   }
   __syncthreads();
+  // ---- open blocks: what each row's parent has in the columns in which the rows' lengths end ----
+  for (int i = tid; i < B * B; i += BT_THREADS) {
+    const int b = i / B, c = i - b * B, p = s_p[b], of = s_p[c], column = of >= 0 ? s_len[of] / bs : 0;
+    s_x[i] = p >= 0 && of >= 0 && s_len[of] % bs > 0 && column < s_have[p] ? old(p, column) : -1;
+  }
+  __syncthreads();
   if (warp == 0) {
-    // ---- open blocks ----
     const int p = lane < B ? s_p[lane] : -1, len = p >= 0 ? s_len[p] : 0, column = len / bs;
-    const int mine = len % bs > 0 ? old(p, column) : -1;
+    const int mine = lane < B ? s_x[lane * B + lane] : -1;
     bool copied = false;
-    for (int b = 0; b < B; ++b) {
-      const int q = s_p[b];
-      if (mine >= 0 && b < lane && q >= 0 && column < s_have[q] && (q == p || old(q, column) == mine)) copied = true;
-    }
+    for (int b = 0; b < B; ++b)
+      if (b < lane && lane < B && mine >= 0 && s_x[b * B + lane] == mine) copied = true;
+    __syncwarp();
     const unsigned copies = __ballot_sync(0xffffffffu, copied);
     if (lane < B) {
       s_need[lane] = p >= 0 ? s_have[p] : 0;
@@ -649,46 +655,58 @@ __global__ void __launch_bounds__(BR_THREADS) beam_tables_kernel(const ReorderAr
     if (lane == 0) a.counts[r].x = __popc(copies);
   }
   __syncthreads();
-  // ---- the tables, column by column ----
+  // ---- the tables ----
+  const int p = lane < B ? s_p[lane] : -1, have = lane < B ? s_have[lane] : 0, need = lane < B ? s_need[lane] : 0, own_first = lane < B ? s_first[lane] : 0,
+            open = lane < B ? s_open[lane] : -1;
+  const int shift = B <= 8 ? 8 : B <= 16 ? 7 : 6, most = 1 << shift, line = most + 1;  // columns at a time
   int before = 0;
-  for (int j0 = 0; j0 < W; j0 += BR_THREADS) {
-    const int j = j0 + tid;
-    unsigned gone = 0;
-    if (j < W) {
+  for (int j0 = 0; j0 < W; j0 += most) {
+    const int columns = min(most, W - j0);
 #pragma unroll 4
-      for (int q = 0; q < B; ++q) s_x[q][tid] = j < s_have[q] ? old(q, j) : -1;
-      unsigned held = 0;  // rows whose block some child has
-      for (int b = 0; b < B; ++b) {
-        const int p = s_p[b];
-        const bool has = j < s_need[b] && j != s_open[b];
-        if (has) held |= 1u << p;
-        a.tables_out[static_cast<int64_t>(row0 + b) * W + j] = has ? s_x[p][tid] : -1;
-      }
-      for (int q = 0; q < B; ++q) {
-        const int x = s_x[q][tid];
-        if (x < 0 || j < s_first[q] || ((held >> q) & 1)) continue;
-        bool kept = false;
-        for (unsigned m = held; m != 0 && !kept; m &= m - 1) kept = s_x[__ffs(m) - 1][tid] == x;
-        for (unsigned m = gone; m != 0 && !kept; m &= m - 1) kept = s_x[__ffs(m) - 1][tid] == x;
-        if (!kept) gone |= 1u << q;
-      }
+    for (int i = tid; i < B << shift; i += BT_THREADS) {
+      const int q = i >> shift, c = i & (most - 1);
+      s_x[q * line + c] = j0 + c < s_have[q] ? old(q, j0 + c) : -1;
     }
-    const int mine = __popc(gone);
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
-    int at = before + incl - mine;
-    for (int w = 0; w < BR_THREADS / 32; ++w) {
-      if (w < warp) at += s_warp[w];
-      before += s_warp[w];
+    for (int c = warp; c < columns; c += BT_WARPS) {
+      const int j = j0 + c, x = lane < B && j < have ? s_x[lane * line + c] : -1;
+      const bool has = j < need && j != open;
+      const int mine = __shfl_sync(0xffffffffu, x, max(p, 0));
+      const unsigned held = __reduce_or_sync(0xffffffffu, has ? 1u << p : 0u);  // rows whose block some child has
+      // (mostly a prompt's block, which all rows have: a match costs several times as much)
+      const int first_x = __shfl_sync(0xffffffffu, x, 0);
+      const bool alike = __all_sync(0xffffffffu, lane >= B || x == first_x) != 0;
+      const unsigned same = alike ? (lane < B ? 0xffffffffu >> (32 - B) : 0u) : __match_any_sync(0xffffffffu, x), given = __ballot_sync(0xffffffffu, x >= 0 && j >= own_first);
+      // (each block once, by the first of the rows that give it)
+      const bool gone = ((given >> lane) & 1) != 0 && (same & held) == 0 && __ffs(same & given) - 1 == lane;
+      const unsigned all = __ballot_sync(0xffffffffu, gone);
+      if (lane < B) s_new[lane * line + c] = has ? mine : -1;
+      if (lane == 0) s_gone[c] = all;
     }
-    int32_t* out = a.given + static_cast<int64_t>(row0) * W + at;
-    for (unsigned m = gone; m != 0; m &= m - 1) *out++ = s_x[__ffs(m) - 1][tid];
+    __syncthreads();
+    for (int i = tid; i < B << shift; i += BT_THREADS) {
+      const int b = i >> shift, c = i & (most - 1);
+      if (c < columns) a.tables_out[static_cast<int64_t>(row0 + b) * W + j0 + c] = s_new[b * line + c];
+    }
+    // what is given back, by column and row
+    if (warp == 0) {
+      for (int c0 = 0; c0 < columns; c0 += 32) {
+        const int n = c0 + lane < columns ? __popc(s_gone[c0 + lane]) : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += up;
+        }
+        s_at[c0 + lane] = before + incl - n;
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    __syncthreads();
+    for (int c = warp; c < columns; c += BT_WARPS) {
+      const unsigned all = s_gone[c];
+      if ((all >> lane) & 1) a.given[static_cast<int64_t>(row0) * W + s_at[c] + __popc(all & ((1u << lane) - 1))] = s_x[lane * line + c];
+    }
     __syncthreads();
   }
   if (tid == 0) a.counts[r].y = before;
@@ -775,28 +793,38 @@ __global__ void __launch_bounds__(BR_THREADS) beam_move_kernel(const ReorderArgs
   for (int i = height + first; i < left; i += step) a.free_blocks[i] = returned(i - height);
   if (first == 0) *a.num_free_out = left;
   // ---- the cache ----
+  __shared__ int s_src[BR_COPIES], s_dst[BR_COPIES], s_tokens[BR_COPIES];
   const int64_t block_bytes = bs * a.token_bytes;
   const int pieces = static_cast<int>((block_bytes + BR_PIECE - 1) / BR_PIECE);
-  const int64_t per_copy = static_cast<int64_t>(a.planes) * pieces, units = take * per_copy;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * (BR_THREADS / 32);
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * (BR_THREADS / 32) + warp; u < units; u += warps) {
-    const int c = static_cast<int>(u / per_copy), rest = static_cast<int>(u - c * per_copy), plane = rest / pieces, piece = rest - plane * pieces;
-    const int r = request_of(s_take, c);
-    const int4 copy = a.copies[static_cast<int64_t>(r) * a.beams + c - s_take[r]];
-    const int64_t bytes = copy.w * a.token_bytes, from = static_cast<int64_t>(piece) * BR_PIECE;
-    if (from >= bytes) continue;
-    const int block = block_for(c);
-    if (block < 0) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(a.cache + plane * a.plane_bytes + copy.y * block_bytes + from);
-    uint4* dst = reinterpret_cast<uint4*>(a.cache + plane * a.plane_bytes + block * block_bytes + from);
-    const int vectors = static_cast<int>(min(static_cast<int64_t>(BR_PIECE), bytes - from) / 16);
-    uint4 v[BR_PIECE / 512];
+  const int64_t per_copy = static_cast<int64_t>(a.planes) * pieces;
+  for (int c0 = 0; c0 < take; c0 += BR_COPIES) {
+    const int copies = min(BR_COPIES, take - c0);
+    __syncthreads();  // (those before have been made)
+    for (int c = tid; c < copies; c += BR_THREADS) {
+      const int r = request_of(s_take, c0 + c);
+      const int4 copy = a.copies[static_cast<int64_t>(r) * a.beams + c0 + c - s_take[r]];
+      const int block = block_for(c0 + c);
+      s_src[c] = copy.y;
+      s_dst[c] = block;
+      s_tokens[c] = block < 0 ? 0 : copy.w;
+    }
+    __syncthreads();
+    const int64_t units = copies * per_copy, warps = static_cast<int64_t>(gridDim.x) * BR_WARPS;
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * BR_WARPS + warp; u < units; u += warps) {
+      const int c = static_cast<int>(u / per_copy), rest = static_cast<int>(u - c * per_copy), plane = rest / pieces, piece = rest - plane * pieces;
+      const int64_t bytes = s_tokens[c] * a.token_bytes, from = static_cast<int64_t>(piece) * BR_PIECE;
+      if (from >= bytes) continue;
+      const uint4* src = reinterpret_cast<const uint4*>(a.cache + plane * a.plane_bytes + s_src[c] * block_bytes + from);
+      uint4* dst = reinterpret_cast<uint4*>(a.cache + plane * a.plane_bytes + s_dst[c] * block_bytes + from);
+      const int vectors = static_cast<int>(min(static_cast<int64_t>(BR_PIECE), bytes - from) / 16);
+      uint4 v[BR_PIECE / 512];
 #pragma unroll
-    for (int e = 0; e < BR_PIECE / 512; ++e)
-      if (e * 32 + lane < vectors) v[e] = src[e * 32 + lane];
+      for (int e = 0; e < BR_PIECE / 512; ++e)
+        if (e * 32 + lane < vectors) v[e] = src[e * 32 + lane];
 #pragma unroll
-    for (int e = 0; e < BR_PIECE / 512; ++e)
-      if (e * 32 + lane < vectors) dst[e * 32 + lane] = v[e];
+      for (int e = 0; e < BR_PIECE / 512; ++e)
+        if (e * 32 + lane < vectors) dst[e * 32 + lane] = v[e];
+    }
   }
   b2::pdl_release_results();  // later kernels may read the lengths and tables ahead of their dependency wait
 }
@@ -896,7 +924,7 @@ int b2_reorder_beams(b2_ctx* ctx, const int32_t* parents, int n, int beams, cons
   // histories: a CTA for each piece of a row, four per SM at most
   const int64_t pieces = history != nullptr ? rows * std::max(1, (history_width + BR_HISTORY - 1) / BR_HISTORY) : 0;
   const int more = static_cast<int>(std::min<int64_t>(pieces, 4 * ctx->num_sms));
-  if (n + more > 0) B2_CUDA(b2_launch(beam_tables_kernel, dim3(n + more), dim3(BR_THREADS), 0, on, a));
+  if (n + more > 0) B2_CUDA(b2_launch(beam_tables_kernel, dim3(n + more), dim3(BT_THREADS), 0, on, a));
   const int64_t most = rows * planes * ((block_size * token_bytes + BR_PIECE - 1) / BR_PIECE) / (BR_THREADS / 32);
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4 * ctx->num_sms, most)));
   B2_CUDA(b2_launch(beam_move_kernel, dim3(grid), dim3(BR_THREADS), 2 * (n + 1) * sizeof(int), on, a));
