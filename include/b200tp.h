@@ -384,7 +384,8 @@ int b2_advance_decode(const int64_t* tokens, int64_t* input_ids, int64_t* positi
  * A row is not served when more than max_tokens are asked for by it and those before it - it then has no tokens - or when it needs
  * blocks and more than there are are asked for by it and those before it - its tokens then keep their places with slot -1 -; its
  * length and blocks stay.  (Attention over such a row's tokens with its context_lens takes its last cached tokens for the new ones; what it gives means nothing.)  A token whose table entry is negative or whose slot would be >= num_slots gets slot -1.  A row with a length
- * that is negative or more than bt_width * block_size counts as a row without tokens.  A block may belong to one row only.
+ * that is negative or more than bt_width * block_size counts as a row without tokens.  A block may belong to one row only; rows that only grow may share their
+ * full blocks (beams, whose blocks b2_reorder_beams gives back).
  * n <= 8192 and n * bt_width * block_size < 2^31 (B2_ERR_SHAPE otherwise). */
 int b2_batch_inputs(int32_t* block_tables, int64_t bt_stride, int bt_width, const int32_t* cached_lens, const int32_t* seq_lens, int n,
                     int32_t* free_blocks, int free_capacity, const int32_t* num_free, int block_size, int64_t num_slots, int max_tokens,
@@ -507,7 +508,7 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
  * prefix_lens[g] tokens are in the same blocks: their tables agree there (which of them is read is not said).  A sequence without a group sees nothing.
  *   out = softmax(scale q K^T) V over the sequence's first context_lens tokens, [n_seqs, nq, head_dim] contiguous, fp32 scores and sums
  * What lies behind a context may hold anything; a sequence without tokens (0: a padded one) comes back as zeros and may have any table.  A context that is shorter than the
- * prefix shortens it for its group.  max_group: the most sequences of a group; the work is dealt by it, and any number gives the same result within rounding.  scale: of either sign, or zero.
+ * prefix shortens it for its group.  max_group: the most sequences of a group, for the argument checks: the work is dealt by cu_groups, and a larger group is served too.  scale: of either sign, or zero.
  * The sums are kept unnormalised with weights of up to 2^8: 256 * the keys seen * the largest |value| has to stay below the type's maximum (3.4e38).
  * Lengths and tables are read after earlier kernels have completed.  Calls that may run at the same time need a workspace each (16-byte aligned, contents irrelevant).
  * b2_prefix_attention_supported says (1 / 0) whether the shape is served: head_dim 64 or 128, up to 128 query heads per KV head, blocks of
@@ -574,10 +575,11 @@ int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n,
  *   tables_out [n * beams, bt_width]: the parent's blocks, -1 behind them.  A block with room left (the last of a length that is no multiple
  *     of block_size) stays with the first row that has it; the others get a block from the stack free_blocks[num_free] and a copy of its tokens.
  *   free_blocks is updated in place: blocks of columns from first_blocks[r] (but at most the row's full blocks) on that no row has any more are put on the
- *     stack, ordered by request, column and row, and then the copies take theirs from the top, ordered by request and row; num_free_out: the new height.
+ *     stack, ordered by request, column and row, and then the copies take theirs from the top, ordered by request and row; num_free_out: the new height
+ *     (what is then above free_capacity is lost).
  *   lens_out: the parent's length.  A row for which there is no block has -1 in its place and loses the tokens in it (its length ends with its full blocks).
  *   cache: planes (layers, keys and values) of [num_blocks, block_size] tokens of token_bytes bytes, plane_bytes apart; 16-byte aligned, a multiple of 16 bytes each.
- *   history (NULL: none) [n * beams, history_width] int64 with row stride history_stride, of which history_lens count: history_out is the parent's, then the row's
+ *   history [n * beams, history_width] int64 with row stride history_stride, of which history_lens (NULL: there are no histories) count: history_out is the parent's, then the row's
  *     token of tokens [n * beams] (NULL: none; negative: none) where there is room, then -1.
  * Lengths that are negative or more than bt_width * block_size count as 0, block numbers outside the cache as none.  No output may overlap an input but free_blocks.  The
  * inputs but free_blocks and the cache are not changed, and places of the stack below num_free neither, so that the same call again gives the same results.

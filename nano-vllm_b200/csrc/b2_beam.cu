@@ -247,8 +247,8 @@ template <typename T>
 __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a) {
   const ScanArgs& s = a.scan;
   constexpr int N = Logits<T>::N;
-  __shared__ double s_total[BS_MAX_BEAMS], s_score[BS_MAX_BEAMS], s_sum[BP_WARPS], s_ref[BS_MAX_BEAMS], s_power[64];
-  __shared__ int s_kind[BS_MAX_BEAMS], s_again[BS_MAX_BEAMS], s_tally[32], s_count, s_any, s_reach, s_list[BP_CHUNKS];
+  __shared__ double s_top[BS_MAX_BEAMS], s_log[BS_MAX_BEAMS], s_score[BS_MAX_BEAMS], s_sum[BP_WARPS], s_power[64];  // log sum exp x: a row's largest logit, and the log of the rest
+  __shared__ int s_kind[BS_MAX_BEAMS], s_again[BS_MAX_BEAMS], s_tally[32], s_count, s_any, s_far, s_reach, s_list[BP_CHUNKS];
   __shared__ uint32_t s_low, s_high;
   __shared__ Candidate s_got[BP_COLLECT], s_best[BS_MAX_PICKS + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = s.beams, K = s.picks, row0 = blockIdx.x * B, C = s.chunks;
@@ -263,15 +263,19 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
   if (tid < 32) s_tally[tid] = 0;
   if (tid < B) s_again[tid] = 0;
   if (tid == 0) {
-    s_count = s_any = s_reach = 0;
+    s_count = s_any = s_far = s_reach = 0;
     s_low = 0xffffffffu;
     s_high = 0;
   }
+  __syncthreads();
   for (int b = warp; b < B; b += BP_WARPS) {
     const float score = s.scores[row0 + b];
     const int kind = !(score > -INFINITY) ? 0 : s.finished != nullptr && s.finished[row0 + b] != 0 ? 1 : 2;  // no continuation, itself, all tokens
     double top = -INFINITY, all = 0.0;
+    float largest = -INFINITY;
     if (kind == 2) {
+      for (int g = lane; g < C; g += 32) largest = fmaxf(largest, s.maxima[static_cast<int64_t>(row0 + b) * C + g]);
+      largest = number_of(__reduce_max_sync(0xffffffffu, ordered(largest)));
       const int first = (row0 + b) * C, parts = deal.owner_of(first + C - 1) - deal.owner_of(first) + 1;
       const double2* sums = s.sums + static_cast<int64_t>(row0 + b) * s.parts;
       for (int i0 = 0; i0 < parts; i0 += 32) {
@@ -288,14 +292,48 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     if (lane == 0) {
       s_score[b] = score;
       s_kind[b] = kind;
-      s_ref[b] = top;
+      s_top[b] = largest;
       // log2(e) has 24 bits in the sum's exponents, which makes them this much too large; what carries the sum lies near M
-      const double off = fabs(top) < 2 * BS_PLAIN ? top * (static_cast<double>(LOG2E) * LN2_64 - 1.0) : 0.0;
-      s_total[b] = (top - off) * LN2_64 + log(all);
+      s_log[b] = (top - top * (static_cast<double>(LOG2E) * LN2_64 - 1.0)) * LN2_64 - largest + log(all);
+      if (kind == 2 && fabsf(largest) >= BS_PLAIN && largest > -INFINITY) s_again[b] = s_far = 1;  // (M has not the bits)
     }
   }
   __syncthreads();
-  auto score_of = [&](int b, float x) { return s_score[b] + (static_cast<double>(x) - s_total[b]); };
+  // ---- a row's sum in 64 bits ----
+  // (a multiple of 1 / 64 in the exponent from the table, the rest of at most 1 / 128 by the series: the table-driven exponential of P. T. P. Tang)
+  auto sum_again = [&](int b) {
+    const T* p = static_cast<const T*>(s.logits) + (row0 + b) * s.ld;
+    const double top = s_top[b];  // (not the scan's M: rows that are alike have the same sum, whatever their place)
+    double all = 0.0;
+#pragma unroll 4
+    for (int i = tid; i < s.vocab; i += BP_THREADS) {
+      const double t = __dmul_rn(Logits<T>::one(p + i) - top, LOG2E_64), k = rint(t * 64.0), d = (t - k * (1.0 / 64.0)) * LN2_64;
+      if (t > -64.0) {
+        const int n = static_cast<int>(k);
+        all += s_power[n & 63] * __longlong_as_double(static_cast<long long>(1023 + (n >> 6)) << 52) * (1.0 + d * (1.0 + d * (0.5 + d * (1.0 / 6.0 + d * (1.0 / 24.0)))));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) s_sum[warp] = all;
+    __syncthreads();
+    if (tid == 0) {
+      all = 0.0;
+      for (int w = 0; w < BP_WARPS; ++w) all += s_sum[w];
+      s_log[b] = log(all);
+    }
+    __syncthreads();
+  };
+  auto fill_powers = [&]() {
+    if (tid < 64) s_power[tid] = exp2(tid / 64.0);
+    __syncthreads();
+  };
+  if (s_far) {
+    fill_powers();
+    for (int b = 0; b < B; ++b)
+      if (s_again[b]) sum_again(b);
+  }
+  auto score_of = [&](int b, float x) { return s_score[b] + (static_cast<double>(x) - s_top[b] - s_log[b]); };
   // the best score in chunk g of the request, -inf where there is none; a finished beam has one, in its first chunk
   auto chunk_score = [&](int g, float x) -> double {
     const int b = g / C, kind = s_kind[b];
@@ -315,7 +353,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     const Row<T> r(s, row0 + b);
     uint4 v[BS_VECTORS];
     r.load(g - b * C, lane, v);
-    const float x0 = fmaxf(-FLT_MAX, __double2float_rd(bound - s_score[b] + s_total[b]));  // (what is forbidden is no continuation)
+    const float x0 = fmaxf(-FLT_MAX, __double2float_rd(bound - s_score[b] + s_log[b] + s_top[b]));  // (what is forbidden is no continuation)
 #pragma unroll
     for (int i = 0; i < BS_VECTORS; ++i) {
       float x[N];
@@ -411,35 +449,6 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
   }
   __syncthreads();
 
-  // ---- a row's sum in 64 bits ----
-  // (a multiple of 1 / 64 in the exponent from the table, the rest of at most 1 / 128 by the series: the table-driven exponential of P. T. P. Tang)
-  auto sum_again = [&](int b) {
-    const T* p = static_cast<const T*>(s.logits) + (row0 + b) * s.ld;
-    const double ref = s_ref[b];
-    double all = 0.0;
-#pragma unroll 4
-    for (int i = tid; i < s.vocab; i += BP_THREADS) {
-      const double t = __dmul_rn(Logits<T>::one(p + i), LOG2E_64) - ref, k = rint(t * 64.0), d = (t - k * (1.0 / 64.0)) * LN2_64;
-      if (t > -64.0) {
-        const int n = static_cast<int>(k);
-        all += s_power[n & 63] * __longlong_as_double(static_cast<long long>(1023 + (n >> 6)) << 52) * (1.0 + d * (1.0 + d * (0.5 + d * (1.0 / 6.0 + d * (1.0 / 24.0)))));
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    if (lane == 0) s_sum[warp] = all;
-    __syncthreads();
-    if (tid == 0) {
-      all = 0.0;
-      for (int w = 0; w < BP_WARPS; ++w) all += s_sum[w];
-      s_total[b] = ref * LN2_64 + log(all);
-    }
-    __syncthreads();
-  };
-  auto fill_powers = [&]() {
-    if (tid < 64) s_power[tid] = exp2(tid / 64.0);
-    __syncthreads();
-  };
   // All threads: the first of what each has, in s_got[0]
   auto first_of_all = [&](Candidate mine) {
 #pragma unroll
@@ -463,7 +472,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     // Many chunks with the same maximum: all rows' sums in 64 bits, with which the first K + 1 chunks are sure, one after the other.
     fill_powers();
     for (int b = 0; b < B; ++b)
-      if (s_kind[b] == 2 && s_ref[b] > -INFINITY) sum_again(b);
+      if (s_kind[b] == 2 && s_top[b] > -INFINITY) sum_again(b);
     exact = true;
     least = -INFINITY;
     Candidate last{INFINITY, 0.f, -1, -2};
@@ -517,15 +526,28 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
   };
   rank_all();
   // ---- continuations of different beams that are too near each other: those beams' sums in 64 bits ----
-  if (!exact && tid + 1 < best) {
-    const Candidate &c = s_best[tid], &d = s_best[tid + 1];
-    if (c.beam != d.beam && c.score - d.score <= BS_NEAR && (s_kind[c.beam] == 2 || s_kind[d.beam] == 2)) s_again[c.beam] = s_again[d.beam] = s_any = 1;
+  // Those that may belong to the K best are the ones from BS_NEAR below the K-th on: mostly K or K + 1, neighbours in s_best.
+  if (!exact && best > 1) {
+    if (many) {
+      if (tid < B) s_again[tid] = 1;
+      if (tid == 0) s_any = 1;
+    } else {
+      const double last = s_best[min(best, K) - 1].score - BS_NEAR;
+      auto near = [&](const Candidate& c, const Candidate& d) { return c.beam != d.beam && fabs(c.score - d.score) <= BS_NEAR && d.score >= last && (s_kind[c.beam] == 2 || s_kind[d.beam] == 2); };
+      if (tid + 1 < best && near(s_best[tid], s_best[tid + 1])) s_again[s_best[tid].beam] = s_again[s_best[tid + 1].beam] = s_any = 1;
+      for (int i = tid; i < got; i += BP_THREADS) {
+        const Candidate mine = s_got[i];
+        if (best <= K || mine.score < last || !before(s_best[K], mine)) continue;
+        for (int k = 0; k < got; ++k)
+          if (near(mine, s_got[k])) s_again[mine.beam] = s_again[s_got[k].beam] = s_any = 1;
+      }
+    }
   }
   __syncthreads();
   if (s_any) {
     fill_powers();
     for (int b = 0; b < B; ++b)
-      if (s_again[b] && s_kind[b] == 2) sum_again(b);
+      if (s_again[b] && s_kind[b] == 2 && s_top[b] > -INFINITY) sum_again(b);
     if (!many)
       for (int i = tid; i < got; i += BP_THREADS)
         if (s_kind[s_got[i].beam] == 2) s_got[i].score = score_of(s_got[i].beam, s_got[i].x);
@@ -904,7 +926,8 @@ int b2_reorder_beams(b2_ctx* ctx, const int32_t* parents, int n, int beams, cons
   if (need < 0) return b2::set_error(B2_ERR_SHAPE, "%d requests of %d beams: at most 32 beams and %d rows", n, beams, BR_MAX_ROWS);
   if (n > 0 && (bt_width <= 0 || bt_stride < bt_width || !parents || !block_tables || !context_lens || !tables_out || !lens_out)) return B2_ERR_ARG;
   if (!num_free || !num_free_out || (free_capacity > 0 && !free_blocks) || (planes > 0 && !cache)) return B2_ERR_ARG;
-  if (history != nullptr && (!history_lens || !history_out || !history_lens_out || history_stride < history_width)) return B2_ERR_ARG;
+  const bool texts = history_lens != nullptr;  // (histories without places have no address)
+  if (texts ? !history_lens_out || (history_width > 0 && (!history || !history_out)) || history_stride < history_width : history || history_out || history_lens_out || tokens) return B2_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(cache) | token_bytes | (planes > 1 ? plane_bytes : 0)) & 15) return B2_ERR_ARG;
   constexpr int64_t limit = (1ll << 31) - 1;
   if (static_cast<int64_t>(n) * beams * bt_width > limit / block_size || static_cast<int64_t>(n) * beams * bt_width + free_capacity > limit || num_blocks > limit / block_size ||
@@ -917,12 +940,12 @@ int b2_reorder_beams(b2_ctx* ctx, const int32_t* parents, int n, int beams, cons
   char* ws = static_cast<char*>(workspace);
   const int64_t counts_bytes = (n * static_cast<int64_t>(sizeof(int2)) + 15) / 16 * 16;
   const ReorderArgs a{parents, n, beams, block_tables, bt_stride, bt_width, block_size, num_blocks, context_lens, first_blocks, free_blocks, free_capacity, num_free,
-                      static_cast<unsigned char*>(cache), planes, plane_bytes, token_bytes, history, history_stride, history != nullptr ? history_width : 0, history_lens, tokens,
+                      static_cast<unsigned char*>(cache), planes, plane_bytes, token_bytes, history, history_stride, texts ? history_width : 0, history_lens, tokens,
                       tables_out, lens_out, num_free_out, history_out, history_lens_out, reinterpret_cast<int2*>(ws + rows * sizeof(int4)), reinterpret_cast<int4*>(ws),
                       reinterpret_cast<int32_t*>(ws + rows * sizeof(int4) + counts_bytes)};
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
   // histories: a CTA for each piece of a row, four per SM at most
-  const int64_t pieces = history != nullptr ? rows * std::max(1, (history_width + BR_HISTORY - 1) / BR_HISTORY) : 0;
+  const int64_t pieces = texts ? rows * std::max(1, (history_width + BR_HISTORY - 1) / BR_HISTORY) : 0;
   const int more = static_cast<int>(std::min<int64_t>(pieces, 4 * ctx->num_sms));
   if (n + more > 0) B2_CUDA(b2_launch(beam_tables_kernel, dim3(n + more), dim3(BT_THREADS), 0, on, a));
   const int64_t most = rows * planes * ((block_size * token_bytes + BR_PIECE - 1) / BR_PIECE) / (BR_THREADS / 32);
