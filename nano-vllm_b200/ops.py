@@ -292,8 +292,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """Decode attention, one query token per sequence, q [n, nq, head_dim], over the paged cache, for sequences that share the beginning of their contexts (the beams of a
     request, requests behind one prompt): group g has the sequences cu_groups[g] .. cu_groups[g + 1] (int32 [groups + 1]), whose block tables agree in the first
     prefix_lens[g] tokens.  Those are read once for the group.  The result is that of paged_attention within rounding; sequences without tokens and
-    those of no group come back as zeros.  max_group: the most sequences of a group.  Shapes that the kernel does not serve (head_dim other than 64 and 128, blocks that are no
-    multiple of 16 tokens, more than 1024 sequences) raise.  The rules in full are at b2_prefix_attention.  Forward only."""
+    those of no group come back as zeros.  max_group: the most sequences of a group (a larger one is served too).  Shapes that the kernel does not serve (head_dim other than 64 and 128, blocks that are no
+    multiple of 16 tokens, more than 1024 sequences or 512 groups) raise.  The rules in full are at b2_prefix_attention.  Forward only."""
     return _native.shared_prefix_attention(get_runtime().handle, q, k_cache, v_cache, cu_groups, prefix_lens, context_lens, block_tables, max_group, scale)
 
 
