@@ -388,6 +388,99 @@ class ModelRunner:
         ends = np.cumsum(counts)
         return [flat[e - c:e] for e, c in zip(ends, counts)]
 
+    @torch.inference_mode()
+    def beam_search(self, seqs: list[Seq], beams: int, max_new_tokens: int, free_blocks: list[int], *, eos_token: int | None = None,
+                    rules: dict[str, torch.Tensor] | None = None) -> list[list[tuple[list[int], float]]]:
+        """The `beams` continuations of each sequence with the largest sums of log-probabilities that a beam search finds, best first, as (tokens, sum), on every rank; fewer
+        where there are no more.  A continuation has max_new_tokens, or fewer and ends in eos_token.  The prompts' block tables have room for their tokens, of which
+        num_cached_tokens are in the cache and the others are computed first, in one pass.  free_blocks: what the search may use; for each sequence `beams` times the blocks that
+        max_new_tokens fill behind the prompt's full blocks.  Afterwards these blocks, and those of the prompts that are not full, hold nothing of use.  rules: arguments of ops.adjust_logits
+        other than the histories (which are the prompts and the beams' tokens), a row for each sequence; looked at on rank 0 only, whose error makes every rank raise."""
+        bs, n, rows = self.block_size, len(seqs), len(seqs) * beams
+        if not 1 <= beams <= 32 or max_new_tokens < 1:
+            raise ValueError(f"{beams} beams, {max_new_tokens} new tokens: 1 to 32 beams, at least one token")
+        if not seqs:
+            return []
+        if rows > min(self.max_num_seqs, 1024) or n > 512:
+            raise ValueError(f"{n} sequences of {beams} beams: at most max_num_seqs ({self.max_num_seqs}) rows, 1024, of 512 sequences")
+        lens, news = [len(s) for s in seqs], [len(s) - s.num_cached_tokens for s in seqs]
+        if min(news) < 1 or sum(news) > self.max_num_batched_tokens:
+            raise ValueError(f"{sum(news)} prompt tokens to compute: at least one of each sequence, at most max_num_batched_tokens ({self.max_num_batched_tokens})")
+        if max(lens) + max_new_tokens > self.max_model_len:
+            raise ValueError(f"{max(lens)} + {max_new_tokens} tokens: at most max_model_len ({self.max_model_len})")
+        if any(l > len(s.block_table) * bs for l, s in zip(lens, seqs)):
+            raise ValueError("the block tables have no room for the prompts")
+        full = [l // bs for l in lens]  # blocks of the prompts that stay as they are: all beams share them
+        needed = sum(beams * (-(-(l + max_new_tokens) // bs) - f) for l, f in zip(lens, full))
+        if len(free_blocks) < needed:
+            raise ValueError(f"{len(free_blocks)} free blocks: the search may need {needed}")
+        # The rows before the first selection: the prompt in the first of each sequence, the others empty.
+        width, most = -(-(max(lens) + max_new_tokens) // bs), max(lens)
+        tables, row_lens = np.full((n, beams, width), -1, dtype=np.int32), np.zeros((n, beams), dtype=np.int32)
+        past, said = np.zeros((n, beams, most + max_new_tokens), dtype=np.int64), np.zeros((n, beams), dtype=np.int32)
+        for i, (s, l) in enumerate(zip(seqs, lens)):
+            tables[i, 0, :-(-l // bs)] = s.block_table[:-(-l // bs)]
+            row_lens[i, 0] = said[i] = l
+            past[i, :, :l] = s.token_ids
+        stack = np.zeros(len(free_blocks) + n, dtype=np.int32)  # (the prompts' open blocks may come to it)
+        stack[:len(free_blocks)] = free_blocks
+        tables_t, lens_t, past_t, said_t, prompt_t, stack_t, height_t, first_t, prefix_t, cu_t = self._to_device(
+            tables.reshape(rows, width), row_lens.reshape(rows), past.reshape(rows, -1), said.reshape(rows), np.repeat(np.array(lens, dtype=np.int32), beams), stack,
+            np.array([len(free_blocks)], dtype=np.int32), np.array(full, dtype=np.int32), np.array(full, dtype=np.int32) * bs, np.arange(0, rows + 1, beams, dtype=np.int32))
+        live, ended = torch.zeros(n, 1, device=self.device), None
+        try:
+            ids, pos = self.prepare_prefill(seqs)
+            logits = self.model.compute_logits(self.model(ids, pos))
+            for step in range(max_new_tokens):
+                picks = self._select_beams(logits, live, beams, ended, eos_token, rules, past_t, said_t, prompt_t)
+                live, ended = picks.scores, picks.finished
+                state = ops.reorder_beams(picks.parents, tables_t, lens_t, stack_t, height_t, self.kv_cache, first_blocks=first_t, history=past_t, history_lens=said_t, tokens=picks.tokens)
+                tables_t, past_t, said_t = state.block_tables, state.history, state.history_lens
+                if step + 1 == max_new_tokens or bool((ended | (picks.parents < 0)).all()):
+                    break
+                # Every row takes a token, so that the rows stay where they are; those that have ended, or are empty, see nothing.
+                inputs = ops.batch_inputs(tables_t, state.context_lens, state.context_lens + 1, stack_t, state.num_free, bs, self.num_kvcache_blocks * bs, rows)
+                lens_t, height_t = inputs.context_lens, inputs.num_free
+                seen = torch.where(ended.view(rows) | (state.context_lens == 0), 0, lens_t)
+                set_context(False, slot_mapping=inputs.slot_mapping, context_lens=seen, block_tables=tables_t, cu_groups=cu_t, prefix_lens=prefix_t, max_group=beams)
+                logits = self.model.compute_logits(self.model(picks.tokens.view(rows).clamp(min=0), inputs.positions))
+            if self.world > 1:  # (rank 0's, as bits)
+                bits = live.reshape(rows).view(torch.int32).to(torch.int64)
+                ops.broadcast_tokens(bits)
+                live = bits.to(torch.int32).view(torch.float32).view(n, beams)
+            scores, said_h, past_h = live.tolist(), said_t.view(n, beams).tolist(), past_t.view(n, beams, -1).tolist()
+        finally:
+            reset_context()
+        self.runtime.check_status()
+        return [[(past_h[i][b][l:said_h[i][b]], scores[i][b]) for b in range(beams) if scores[i][b] > float("-inf")] for i, l in enumerate(lens)]
+
+    def _select_beams(self, logits, scores, picks, ended, eos_token, rules, past, said, prompt_lens) -> ops.BeamPicks:
+        """ops.beam_select on rank 0, and its picks on every rank (the scores on rank 0 only).  The logits are of as many rows a sequence as there are scores."""
+        n = scores.shape[0]
+        failed, out = None, None
+        if self.rank == 0:
+            try:
+                if rules:
+                    each, rows = scores.shape[1], slice(None, None, picks // scores.shape[1])  # (before the first selection all rows of a sequence have the prompt)
+                    logits = ops.adjust_logits(logits, **{name: x.repeat_interleave(each, 0) for name, x in rules.items()}, history=past[rows], history_lens=said[rows].contiguous(),
+                                               prompt_lens=prompt_lens[rows].contiguous(), out=logits)
+                out = ops.beam_select(logits, scores, picks, finished=ended, eos_token=eos_token)
+            except Exception as error:  # (the other ranks are on their way to the broadcast: they get a beam that there is not)
+                failed = error
+        if self.world > 1:
+            packed = torch.full((n * picks,), -1, dtype=torch.int64, device=self.device)
+            if out is not None:
+                packed = ((out.tokens + 1 << 8) | (out.parents + 1 << 1) | out.finished).view(-1)
+            ops.broadcast_tokens(packed)
+            if self.rank != 0:
+                if int(packed[0]) < 0:
+                    raise RuntimeError("rank 0 could not apply the step's rules or select its beams; its own error says why")
+                packed = packed.view(n, picks)
+                out = ops.BeamPicks(torch.zeros(n, picks, device=self.device), (packed >> 1 & 127).to(torch.int32) - 1, (packed >> 8) - 1, (packed & 1).bool())
+        if failed is not None:
+            raise failed
+        return out
+
     # ---- CUDA graphs (reference :222-257) -----------------------------------------
     @torch.inference_mode()
     def _capture_graphs(self):

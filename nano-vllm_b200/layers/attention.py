@@ -98,12 +98,15 @@ class Attention(nn.Module):
 
     def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Attention over K/V that are already in the paged cache (decode,
-        prefill with a cached prefix, or trees of drafted tokens) or passed in (plain prefill)."""
+        prefill with a cached prefix, trees of drafted tokens, or sequences that share a beginning) or passed in (plain prefill)."""
         ctx = get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
         tree_mask = getattr(ctx, "tree_mask", None)  # (a context of the reference's fields has none)
         if tree_mask is not None:  # trees of drafted tokens: own kernel whatever the backend, there is no library call
             return ops.tree_attention(q, k_cache, v_cache, ctx.cu_seqlens_q, ctx.context_lens, ctx.block_tables, tree_mask, ctx.max_seqlen_q, self.scale)
+        prefix_lens = getattr(ctx, "prefix_lens", None)
+        if prefix_lens is not None:  # as for the trees
+            return ops.shared_prefix_attention(q, k_cache, v_cache, ctx.cu_groups, prefix_lens, ctx.context_lens, ctx.block_tables, ctx.max_group, self.scale)
         if Attention.backend == "sdpa":
             if ctx.is_prefill:
                 cu_q, cu_k = ctx.cu_seqlens_q.tolist(), ctx.cu_seqlens_k.tolist()

@@ -141,7 +141,7 @@ class Qwen3Model(nn.Module):
         """All layers of a decode step through ops.decode_stack; None where that does not apply: the layers then run one by one.
         It computes what the stock layers compute, so every layer must be one, without hooks of its own."""
         ctx = get_context()
-        if ctx.is_prefill or getattr(ctx, "tree_mask", None) is not None or ctx.context_lens is None or ctx.slot_mapping is None or ctx.block_tables is None or Attention.backend != "flash_attn":
+        if ctx.is_prefill or getattr(ctx, "tree_mask", None) is not None or getattr(ctx, "prefix_lens", None) is not None or ctx.context_lens is None or ctx.slot_mapping is None or ctx.block_tables is None or Attention.backend != "flash_attn":
             return None
         first = self.layers[0]
         if not _stock_classes() or not _is_stock(first) or embedded.dim() != 2 or first.self_attn.attn.k_cache.dim() != 4:
