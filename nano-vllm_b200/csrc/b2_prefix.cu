@@ -20,8 +20,8 @@ namespace {
 // batch.  A piece that begins an item is left in a row of its own, one for common and one for other keys, a piece that goes on with one that an earlier range
 // began in the range's slot; prefix_join_kernel joins them.  Sequences without common keys whose context is one piece are stored at once.
 // ---------------------------------------------------------------------------
-constexpr int PX_ROWS = 128, PX_KEYS = 64, PX_COLUMNS = 256;
-constexpr int PX_WARPS = 6, PO_WARPS = 4, PX_THREADS = (PX_WARPS + PO_WARPS + 1) * 32;  // of common keys, of others and their TMA warp
+constexpr int PX_ROWS = 128, PX_KEYS = 64, PX_COLUMNS = 512;
+constexpr int PX_WARPS = 10, PO_WARPS = 4, PX_THREADS = (PX_WARPS + PO_WARPS + 1) * 32;  // of common keys, of others and their TMA warp
 constexpr int PX_MAX_SEQS = 1024, PX_MAX_GROUPS = 512;
 constexpr int PX_ITEM_UNITS = 2;  // what an item costs beside its tiles, in tiles
 constexpr int PX_WHOLE_TILES = 8;
@@ -41,12 +41,15 @@ struct Prefix {
   static constexpr int OWN_STAGES = 6 / HALVES, OWN_ROWS = 16, OWN_SLOT = OWN_ROWS * (HD + 2);
   static constexpr uint32_t OWN_RING = Q + 2 * STAGES * TILE, OWN_Q = OWN_RING + OWN_STAGES * 2 * TILE;
   __host__ __device__ static constexpr uint32_t own_q(int h) { return h * 1024 * HALVES; }  // 8 h rows
-  __host__ __device__ static constexpr int meet_dims(int h) { return h == 1 ? HD : 32; }    // dimensions that meet at a time
+  __host__ __device__ static constexpr int meet_dims(int h) { return h == 1 ? 64 : 32; }    // dimensions that meet at a time
   __host__ __device__ static constexpr uint32_t meet(int h) { return OWN_Q + OWN_STAGES * own_q(h); }
   __host__ __device__ static constexpr uint32_t plan(int h) { return meet(h) + PO_WARPS * 8 * h * (meet_dims(h) + 4) * 4; }
   static constexpr size_t smem(int h, int n_seqs, int n_groups) { return 1024 + plan(h) + (2 * n_groups + n_seqs + 2) * sizeof(int) + n_seqs * sizeof(uint16_t); }
 };
-static_assert(Prefix<128>::smem(2, PX_MAX_SEQS, PX_MAX_GROUPS) + 1024 <= 227 * 1024 && Prefix<64>::smem(2, PX_MAX_SEQS, PX_MAX_GROUPS) + 1024 <= 227 * 1024, "a CTA's shared memory (1 KB: static)");
+constexpr size_t PX_STATIC = 2944, PX_SMEM = 227 * 1024;
+static_assert(Prefix<128>::smem(1, PX_MAX_SEQS, PX_MAX_GROUPS) + PX_STATIC <= PX_SMEM && Prefix<128>::smem(2, PX_MAX_SEQS, PX_MAX_GROUPS) + PX_STATIC <= PX_SMEM &&
+                  Prefix<64>::smem(1, PX_MAX_SEQS, PX_MAX_GROUPS) + PX_STATIC <= PX_SMEM && Prefix<64>::smem(2, PX_MAX_SEQS, PX_MAX_GROUPS) + PX_STATIC <= PX_SMEM,
+              "a CTA's shared memory");
 
 struct PrefixArgs {
   const int32_t* tables;
@@ -242,30 +245,31 @@ struct BoxRows {
     if (box >= last) return 0;
     return min(max(0, __ldg(table + blk)), a.num_blocks - 1) * a.block_size + p - blk * a.block_size;  // inside the cache whatever the table holds
   }
-  // box i of the segment's, in order
-  __device__ __forceinline__ int row(int i) {
+  // boxes i .. i + 3 of the segment's, in order; those of a tile, so that they do not go past a multiple of 32 (what is behind the tile's means nothing)
+  __device__ __forceinline__ void four(int i, int (&r)[4]) {
     if (i >> 5 != group) {
       rows = next;
       group = i >> 5;
       next = of(group + 1);
     }
-    return __shfl_sync(0xffffffffu, rows, i & 31);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = __shfl_sync(0xffffffffu, rows, (i + k) & 31);
   }
 };
 
 // ---- the common keys: 128 rows of the tensor core -----------------------------------------------------------------------------------------
-//   warps 0..3   one thread per row: running maximum and sum, P = exp2(...) rounded to bf16 over the scores in tensor memory (the
-//                product's operand has 16 bits), and the sum O rescaled where the maximum has grown
-//   warp 4       TMA: Q of the segment, then K and V tiles
-//   warp 5       tcgen05.mma: S = Q K^T (128 x 64, two buffers), O += P V with P read from tensor memory
+//   warps 0..7   two threads per row, one for the even and one for the odd tiles, each with its own running maximum, sum and O: P = exp2(...) rounded to bf16 over the scores
+//                in tensor memory (the product's operand has 16 bits), and O rescaled where the maximum has grown.  They meet at the segment's end.
+//   warp 8       TMA: Q of the segment, then K and V tiles
+//   warp 9       tcgen05.mma: S = Q K^T (128 x 64, four buffers), O += P V with P read from tensor memory
 template <int HD>
 __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const PrefixArgs& a, const Plan& plan, uint32_t s_q, uint32_t bars, uint32_t tmem,
-                                            int warp, volatile int* abort_flag) {
+                                            float (*s_m)[PX_ROWS], float (*s_l)[PX_ROWS], int warp, volatile int* abort_flag) {
   using T = Prefix<HD>;
   constexpr int HALVES = T::HALVES, STAGES = T::STAGES;
   const uint32_t s_k = s_q + T::Q, s_v = s_k + STAGES * T::TILE;
   const uint32_t q_full = bars, q_empty = q_full + 8, k_full = q_empty + 8, k_empty = k_full + STAGES * 8, v_full = k_empty + STAGES * 8, v_empty = v_full + STAGES * 8,
-                 s_full = v_empty + STAGES * 8, p_full = s_full + 2 * 8, o_done = p_full + 2 * 8;
+                 s_full = v_empty + STAGES * 8, p_full = s_full + 4 * 8, o_done = p_full + 4 * 8, met = o_done + 4 * 8;
   const int lane = threadIdx.x & 31, x = blockIdx.x;
   const Deal deal(plan.common_units[a.n_groups], gridDim.x);
   const int begin = deal.begin_of(x), end = deal.end_of(x);
@@ -277,7 +281,7 @@ __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtens
   int c = 0, segs = 0;  // tiles and segments so far
 
   if (begin >= end) {
-  } else if (warp == 4) {
+  } else if (warp == 8) {
     // ---------------- TMA (the whole warp walks and one thread issues, here and in the next warp) ----------------
     bool ok = true;
     while (ok && walk.next(a, seg)) {
@@ -296,29 +300,31 @@ __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtens
         const int st = no % STAGES;
         if (!all_wait(empty + st * 8, ((no / STAGES) & 1) ^ 1, B2_WAIT_SMEM_EMPTY)) return false;
         const uint32_t bar = full + st * 8;
-        if (b2::elect_one()) b2::mbar_arrive_expect_tx(bar, T::TILE);
-        for (int i = 0; i < per_tile; ++i) {
-          const int r = rows.row(j * per_tile + i);
-          if (b2::elect_one())
-            for (int h = 0; h < HALVES; ++h) b2::tma_load_2d(dst + st * T::TILE + h * T::HALF + i * a.box * 128, map, bar, seg.head * HD + h * 64, r, b2::kEvictNormal);
+        int r[4];
+        rows.four(j * per_tile, r);
+        if (b2::elect_one()) {  // (one after the other by one thread: an election for each box took 0.1 us more)
+          b2::mbar_arrive_expect_tx(bar, T::TILE);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < per_tile)
+              for (int h = 0; h < HALVES; ++h) b2::tma_load_2d(dst + st * T::TILE + h * T::HALF + i * a.box * 128, map, bar, seg.head * HD + h * 64, r[i], b2::kEvictNormal);
         }
         __syncwarp();
         return true;
       };
       auto load_k = [&](int j) { return load(j, c + j, &tmK, k_full, k_empty, s_k, k_rows); };
       auto load_v = [&](int j) { return load(j, c + j, &tmV, v_full, v_empty, s_v, v_rows); };
-      // in the order of use: K of two tiles, then V of a tile and K of the one after the next
+      // in the order of use: K of three tiles, then V of a tile and K of the third after it
       const int n = seg.t1 - seg.t0;
-      ok = load_k(0);
-      if (n > 1) ok = ok && load_k(1);
+      for (int j = 0; ok && j < min(n, 3); ++j) ok = load_k(j);
       for (int j = 0; ok && j < n; ++j) {
         ok = load_v(j);
-        if (j + 2 < n) ok = ok && load_k(j + 2);
+        if (j + 3 < n) ok = ok && load_k(j + 3);
       }
       c += n;
       ++segs;
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ---------------- tensor core ----------------
     const uint32_t idesc_s = b2::umma_idesc_bf16(PX_KEYS) | a.negate;
     constexpr uint32_t idesc_o = b2::umma_idesc_bf16(HD) | (1u << 16);  // second operand MN-major
@@ -328,18 +334,17 @@ __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtens
       b2::tc_fence_after();
       return ok;
     };
-    // scores of tile i, into the columns that P of tile i - 2 was read from, once it has been (a barrier for each of the two buffers: where a
-    // segment ends, both products may be complete before this wait begins, and with one barrier it would take the later phase for one that is to come)
+    // scores of tile i, into the columns that P of tile i - 4 was read from, once it has been
     auto scores = [&](int i, bool last) {
-      const int st = i % STAGES;
-      bool ok = i < 2 || wait(o_done + (i & 1) * 8, ((i >> 1) & 1) ^ 1, B2_WAIT_TMEM_FULL);
+      const int st = i % STAGES, buf = i & 3;
+      bool ok = i < 4 || wait(o_done + buf * 8, ((i >> 2) & 1) ^ 1, B2_WAIT_TMEM_FULL);
       ok = ok && wait(k_full + st * 8, (i / STAGES) & 1, B2_WAIT_SMEM_FULL);
       if (ok && b2::elect_one()) {
         const uint64_t dk = desc_k + st * (T::TILE >> 4);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          b2::umma_bf16(tmem + (i & 1) * PX_KEYS, desc_q + (k >> 2) * (T::Q_HALF >> 4) + 2 * (k & 3), dk + (k >> 2) * (T::HALF >> 4) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
-        b2::umma_commit(s_full + (i & 1) * 8);
+          b2::umma_bf16(tmem + buf * PX_KEYS, desc_q + (k >> 2) * (T::Q_HALF >> 4) + 2 * (k & 3), dk + (k >> 2) * (T::HALF >> 4) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
+        b2::umma_commit(s_full + buf * 8);
         b2::umma_commit(k_empty + st * 8);
         if (last) b2::umma_commit(q_empty);
       }
@@ -350,30 +355,40 @@ __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtens
     while (ok && walk.next(a, seg)) {
       if (seg.t0 >= seg.t1) continue;
       const int n = seg.t1 - seg.t0;
-      ok = wait(q_full, segs & 1, B2_WAIT_SMEM_FULL) && scores(c, n == 1);
-      if (n > 1) ok = ok && scores(c + 1, n == 2);
+      ok = wait(q_full, segs & 1, B2_WAIT_SMEM_FULL);
+      for (int j = 0; ok && j < min(n, 3); ++j) ok = scores(c + j, j + 1 == n);
       for (int j = 0; ok && j < n; ++j) {
-        const int i = c + j, st = i % STAGES;
-        ok = wait(v_full + st * 8, (i / STAGES) & 1, B2_WAIT_SMEM_FULL) && wait(p_full + (i & 1) * 8, (i >> 1) & 1, B2_WAIT_TMEM_EMPTY);
+        const int i = c + j, st = i % STAGES, buf = i & 3;
+        ok = wait(v_full + st * 8, (i / STAGES) & 1, B2_WAIT_SMEM_FULL) && wait(p_full + buf * 8, (i >> 2) & 1, B2_WAIT_TMEM_EMPTY);
         if (!ok) break;
         if (b2::elect_one()) {
           const uint64_t dv = desc_v + st * (T::TILE >> 4);
 #pragma unroll
           for (int k = 0; k < PX_KEYS / 16; ++k)  // 16 tokens: 8 columns of P, 2048 bytes of V
-            b2::umma_bf16_ts(tmem + 2 * PX_KEYS, tmem + (i & 1) * PX_KEYS + k * 8, dv + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-          b2::umma_commit(o_done + (i & 1) * 8);
+            b2::umma_bf16_ts(tmem + 4 * PX_KEYS + (i & 1) * HD, tmem + buf * PX_KEYS + k * 8, dv + k * (2048 >> 4), idesc_o, (j > 1 || k > 0) ? 1u : 0u);
+          b2::umma_commit(o_done + buf * 8);
           b2::umma_commit(v_empty + st * 8);
         }
         __syncwarp();
-        if (j + 2 < n) ok = scores(i + 2, j + 3 == n);
+        if (j + 3 < n) ok = scores(i + 3, j + 4 == n);
       }
       c += n;
       ++segs;
     }
   } else {
-    // ---------------- a thread per row ----------------
-    const int row = threadIdx.x;
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, t_o = tmem + 2 * PX_KEYS + lanes;
+    // ---------------- two threads per row ----------------
+    const int row = threadIdx.x & (PX_ROWS - 1), odd = warp >> 2;  // odd: which tiles
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, t_o = tmem + 4 * PX_KEYS + odd * HD + lanes;
+    int meetings = 0;
+    auto all_here = [&]() {  // the eight warps, like a barrier, but bounded
+      b2::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) b2::mbar_arrive(met);
+      const bool here = all_wait(met, meetings & 1, B2_WAIT_TMEM_FULL);
+      ++meetings;
+      b2::tc_fence_after();
+      return here;
+    };
     const uint64_t scale2 = b2::pair_of(a.scale_log2, a.scale_log2);
     const int64_t all_rows = static_cast<int64_t>(a.n_seqs) * a.nq;
     bool ok = true;
@@ -382,10 +397,10 @@ __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtens
       const int n = seg.t1 - seg.t0;
       float m = -INFINITY;  // the row's maximum, in units of scores
       uint64_t l[2] = {};   // its sum, in two pairs
-      const bool idle = warp * 32 >= seg.rows;  // none of the warp's rows exists
-      for (int j = 0; j < n; ++j) {
-        const int i = c + j, buf = i & 1;
-        ok = all_wait(s_full + buf * 8, (i >> 1) & 1, B2_WAIT_TMEM_FULL);
+      const bool idle = (warp & 3) * 32 >= seg.rows;  // none of the warp's rows exists
+      for (int j = (c ^ odd) & 1; j < n; j += 2) {
+        const int i = c + j, buf = i & 3;
+        ok = all_wait(s_full + buf * 8, (i >> 2) & 1, B2_WAIT_TMEM_FULL);
         if (!ok) break;
         b2::tc_fence_after();
         if (!idle) {
@@ -427,8 +442,8 @@ __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtens
             }
             b2::tmem_st_32x16(t_s + h * 16, p);  // (this row has read its columns)
           }
-          if (j > 0 && any_grown) {
-            ok = all_wait(o_done + ((i - 1) & 1) * 8, ((i - 1) >> 1) & 1, B2_WAIT_TMEM_FULL);
+          if (j > 1 && any_grown) {
+            ok = all_wait(o_done + ((i - 2) & 3) * 8, ((i - 2) >> 2) & 1, B2_WAIT_TMEM_FULL);
             if (!ok) break;
             b2::tc_fence_after();
 #pragma unroll
@@ -449,34 +464,53 @@ __device__ __forceinline__ void common_keys(const CUtensorMap& tmQ, const CUtens
         if (lane == 0) b2::mbar_arrive(p_full + buf * 8);
       }
       if (!ok) break;
-      c += n;
-      ok = all_wait(o_done + ((c - 1) & 1) * 8, ((c - 1) >> 1) & 1, B2_WAIT_TMEM_FULL);
+      // ---- both threads' results together ----
+      const int first = (c ^ odd) & 1, last = c + n - 1 - ((n - 1 - first) & 1);  // of this thread's tiles, if it has any
+      if (first < n) ok = all_wait(o_done + (last & 3) * 8, (last >> 2) & 1, B2_WAIT_TMEM_FULL);
       if (!ok) break;
-      b2::tc_fence_after();
       if (!idle) {
         float sums[2];
         b2::halves_of(b2::add_pair(l[0], l[1]), sums[0], sums[1]);
+        s_m[odd][row] = m;
+        s_l[odd][row] = sums[0] + sums[1];
+      }
+      ok = all_here();
+      if (!ok) break;
+      if (!idle) {
         const bool exists = row < seg.rows, begins = seg.t0 == 0;
+        const float m0 = s_m[0][row], m1 = s_m[1][row], top = fmaxf(m0, m1);
+        // (one tile: the other O holds anything)
+        const float f0 = m0 == top ? 1.f : b2::ex2((m0 - top) * a.scale_log2), f1 = m1 == top ? 1.f : b2::ex2((m1 - top) * a.scale_log2);
+        const bool has0 = n > 1 || (c & 1) == 0, has1 = n > 1 || (c & 1) == 1;
         const int64_t at = (static_cast<int64_t>(seg.head) * a.n_seqs + seg.seq) * a.group + row;  // (sequences of 128 rows lie one after the other)
         float* const slot = a.slots + static_cast<int64_t>(x) * T::SLOT;
         float* const o = begins ? a.rows_o + at * 4 : slot + row * 4;
         const int64_t step = begins ? all_rows * 4 : PX_ROWS * 4;
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
+        for (int d0 = 0; d0 < HD / 2; d0 += 32) {  // each of the two brings half of the dimensions
+          const int d = odd * (HD / 2) + d0;
           uint32_t r[2][32];
-          b2::tmem_ld_32x32(t_o + h * 64, r[0]);
-          b2::tmem_ld_32x32(t_o + h * 64 + 32, r[1]);
+          b2::tmem_ld_32x32(tmem + 4 * PX_KEYS + lanes + d, r[0]);
+          b2::tmem_ld_32x32(tmem + 4 * PX_KEYS + HD + lanes + d, r[1]);
           b2::tc_wait_ld(r);
-          if (!exists) continue;
+          if (exists) {
 #pragma unroll
-          for (int g = 0; g < 16; ++g)
-            *reinterpret_cast<uint4*>(o + (h * 16 + g) * step) = make_uint4(r[g >> 3][(g & 7) * 4], r[g >> 3][(g & 7) * 4 + 1], r[g >> 3][(g & 7) * 4 + 2], r[g >> 3][(g & 7) * 4 + 3]);
+            for (int e = 0; e < 32; e += 4) {
+              float v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] = (has0 ? __uint_as_float(r[0][e + k]) * f0 : 0.f) + (has1 ? __uint_as_float(r[1][e + k]) * f1 : 0.f);
+              *reinterpret_cast<float4*>(o + (d + e) / 4 * step) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+          }
+          __syncwarp();
         }
-        if (exists) {
-          (begins ? a.rows_m + at : slot + HD * PX_ROWS + row)[0] = m * a.scale_log2;
-          (begins ? a.rows_l + at : slot + (HD + 1) * PX_ROWS + row)[0] = sums[0] + sums[1];
+        if (exists && odd == 0) {
+          (begins ? a.rows_m + at : slot + HD * PX_ROWS + row)[0] = top * a.scale_log2;
+          (begins ? a.rows_l + at : slot + (HD + 1) * PX_ROWS + row)[0] = (has0 ? s_l[0][row] * f0 : 0.f) + (has1 ? s_l[1][row] * f1 : 0.f);
         }
       }
+      ok = all_here();  // (the next segment's products write over O)
+      c += n;
       ++segs;
     }
   }
@@ -556,13 +590,16 @@ __device__ __forceinline__ void own_keys(const CUtensorMap& tmQ, const CUtensorM
             for (int h = 0; h < HALVES; ++h) b2::tma_load_3d(s_q + st * T::own_q(H) + h * 1024 * H, &tmQ, bar, h * 64, seg.head * a.group + seg.row, seg.seq, b2::kEvictNormal);
           __syncwarp();
         }
-        for (int i = 0; i < boxes; ++i) {
-          const int r = rows.row(j * per_tile + i);
-          if (b2::elect_one())
-            for (int h = 0; h < HALVES; ++h) {
-              b2::tma_load_2d(dst + h * T::HALF + i * a.box * 128, &tmK, bar, seg.head * HD + h * 64, r, a.row_blocks > 1 ? b2::kEvictNormal : b2::kEvictFirst);
-              b2::tma_load_2d(dst + T::TILE + h * T::HALF + i * a.box * 128, &tmV, bar, seg.head * HD + h * 64, r, a.row_blocks > 1 ? b2::kEvictNormal : b2::kEvictFirst);
-            }
+        int r[4];
+        rows.four(j * per_tile, r);
+        if (b2::elect_one()) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < boxes)
+              for (int h = 0; h < HALVES; ++h) {
+                b2::tma_load_2d(dst + h * T::HALF + i * a.box * 128, &tmK, bar, seg.head * HD + h * 64, r[i], a.row_blocks > 1 ? b2::kEvictNormal : b2::kEvictFirst);
+                b2::tma_load_2d(dst + T::TILE + h * T::HALF + i * a.box * 128, &tmV, bar, seg.head * HD + h * 64, r[i], a.row_blocks > 1 ? b2::kEvictNormal : b2::kEvictFirst);
+              }
         }
         __syncwarp();
       }
@@ -766,9 +803,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attention_kernel(const _
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const Plan plan = plan_of(reinterpret_cast<int*>(smem + T::plan(H)), a.n_groups, a.n_seqs);
-  constexpr int COMMON_BARS = 2 + 4 * T::STAGES + 6, BARS = COMMON_BARS + 2 * T::OWN_STAGES + 1, P_FULL = 2 + 4 * T::STAGES + 2;
+  constexpr int COMMON_BARS = 2 + 4 * T::STAGES + 13, BARS = COMMON_BARS + 2 * T::OWN_STAGES + 1, P_FULL = 2 + 4 * T::STAGES + 4;
   __shared__ __align__(8) uint64_t s_bars[BARS];
-  __shared__ float s_m[PO_WARPS][16], s_l[PO_WARPS][16];
+  __shared__ float s_m[PO_WARPS][16], s_l[PO_WARPS][16], s_common_m[2][PX_ROWS], s_common_l[2][PX_ROWS];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const uint32_t bars = b2::smem_u32(s_bars);
@@ -778,12 +815,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attention_kernel(const _
     b2::tma_prefetch_desc(&tmQ1);
     b2::tma_prefetch_desc(&tmK);
     b2::tma_prefetch_desc(&tmV);
-    // (P by the four warps of the rows; the other keys' stages are left, and results brought together, by four warps)
-    for (int i = 0; i < BARS; ++i) b2::mbar_init(bars + i * 8, i == P_FULL || i == P_FULL + 1 || i >= COMMON_BARS + T::OWN_STAGES ? 4 : 1);
+    // (P by the four warps of the rows; the other keys' stages are left, and results brought together, by four warps, the common keys' results by eight)
+    for (int i = 0; i < BARS; ++i) b2::mbar_init(bars + i * 8, i == COMMON_BARS - 1 ? 8 : (i >= P_FULL && i < P_FULL + 4) || i >= COMMON_BARS + T::OWN_STAGES ? 4 : 1);
     s_abort = 0;
     b2::mbar_fence_init();
   }
-  if (warp == 5) {
+  if (warp == 9) {
     b2::tmem_alloc(b2::smem_u32(&s_tmem), PX_COLUMNS);
     b2::tmem_relinquish();
   }
@@ -795,7 +832,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attention_kernel(const _
   const uint32_t tmem = b2::uniform(s_tmem);
   // (Only now: a kernel that waits for this one with columns of tensor memory in hand must not get the ones that this CTA has yet to allocate.)
   b2::pdl_launch_dependents();
-  if (warp < PX_WARPS) common_keys<HD>(tmQ, tmK, tmV, a, plan, b2::smem_u32(smem), bars, tmem, warp, &s_abort);
+  if (warp < PX_WARPS) common_keys<HD>(tmQ, tmK, tmV, a, plan, b2::smem_u32(smem), bars, tmem, s_common_m, s_common_l, warp, &s_abort);
   else own_keys<HD, H>(tmQ1, tmK, tmV, a, plan, smem, bars + COMMON_BARS * 8, s_m, s_l, warp - PX_WARPS, &s_abort);
   __syncwarp();
   b2::tc_fence_before();
@@ -806,7 +843,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attention_kernel(const _
     for (int i = 0; i < 100; ++i) __nanosleep(2000);  // copies in flight land before the CTA leaves
     if (threadIdx.x == 0) b2::report_timeout(a.status, aborted);
   }
-  if (warp == 5) b2::tmem_dealloc(tmem, PX_COLUMNS);
+  if (warp == 9) b2::tmem_dealloc(tmem, PX_COLUMNS);
 }
 
 // Joins the pieces of each row, in the order of their keys.  A block takes 32 rows and 64 dimensions, a thread a row and two times four dimensions.
