@@ -505,7 +505,8 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
 /* ---- decode attention for sequences that share the beginning of their contexts: beams of a request, requests behind one prompt (no
  *      counterpart in the reference, which walks every context for itself, nanovllm/layers/attention.py:70-74) --
  * q [n_seqs, nq, head_dim] bf16 (row stride q_stride), one query token per sequence; group g has the sequences cu_groups[g] .. cu_groups[g+1], whose first
- * prefix_lens[g] tokens are in the same blocks: their tables agree there (which of them is read is not said).  A sequence without a group sees nothing.
+ * prefix_lens[g] tokens are in the same blocks: their tables agree there (which of them is read is not said).  A sequence without a group sees nothing,
+ * and none has one where cu_groups falls.
  *   out = softmax(scale q K^T) V over the sequence's first context_lens tokens, [n_seqs, nq, head_dim] contiguous, fp32 scores and sums
  * What lies behind a context may hold anything; a sequence without tokens (0: a padded one) comes back as zeros and may have any table.  A context that is shorter than the
  * prefix shortens it for its group.  max_group: the most sequences of a group, for the argument checks: the work is dealt by cu_groups, and a larger group is served too.  scale: of either sign, or zero.

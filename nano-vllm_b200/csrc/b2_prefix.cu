@@ -101,17 +101,20 @@ __device__ __forceinline__ int last_at(const int* first, int n, int unit) {  // 
 // All threads of a block fill the plan; scratch: [n_groups] ints of shared memory that the async proxy writes later.
 __device__ __forceinline__ void make_plan(const PrefixArgs& a, const Plan& plan, int* first_live) {
   const int n_seqs = a.n_seqs, n_groups = a.n_groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bool falls = false;  // bounds that fall: groups would overlap, and their rows' pieces too
   for (int g = threadIdx.x; g < n_groups; g += PX_THREADS) {
     first_live[g] = PX_MAX_SEQS;
     plan.common[g] = max(0, __ldg(a.prefix + g));
-    plan.common_units[g + 1] = bound(a, g + 1);  // (for the search below)
-    if (g == 0) plan.common_units[0] = bound(a, 0);
+    const int from = bound(a, g), to = bound(a, g + 1);
+    falls = falls || to < from;
+    plan.common_units[g + 1] = to;  // (for the search below)
+    if (g == 0) plan.common_units[0] = from;
   }
-  __syncthreads();
+  falls = __syncthreads_or(falls) != 0;
   for (int s = threadIdx.x; s < n_seqs; s += PX_THREADS) {
     const int len = length(a, s);
     int g = last_at(plan.common_units, n_groups, s);
-    if (n_groups == 0 || s < plan.common_units[g] || s >= plan.common_units[g + 1]) g = 0xffff;
+    if (n_groups == 0 || falls || s < plan.common_units[g] || s >= plan.common_units[g + 1]) g = 0xffff;
     plan.group_of[s] = static_cast<uint16_t>(g);
     if (g != 0xffff && len > 0) {  // (a sequence without tokens shortens nothing, and its table may be anything)
       atomicMin(plan.common + g, len);

@@ -111,6 +111,13 @@ def test_refusals(runner):
     for args in ((seqs, 0, 5, free), (seqs, 33, 5, free), (seqs, 4, 0, free), (seqs * 20, 4, 5, free), (seqs, 4, 2000, free), (seqs, 4, 30, free[:3]), (sequences([20, 0], 1), 4, 5, free)):
         with pytest.raises(ValueError):
             runner.beam_search(*args)
+    for blocks in ([100] * 50, list(range(50)), list(range(380, 430)), [-1] + free):
+        with pytest.raises(ValueError, match="blocks"):
+            runner.beam_search(seqs, 4, 5, blocks)
+    shared = sequences([20, 20], seed=13)
+    shared[1].block_table = list(shared[0].block_table)
+    with pytest.raises(ValueError, match="share"):
+        runner.beam_search(shared, 4, 5, free)
     seqs[0].block_table = [0]
     with pytest.raises(ValueError, match="room"):
         runner.beam_search(seqs, 4, 5, free)

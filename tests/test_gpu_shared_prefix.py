@@ -210,6 +210,14 @@ def test_lengths_that_tables_do_not_hold(ops):
     case.check(got)
 
 
+def test_bounds_that_fall(ops):
+    """Groups that would overlap are none: every sequence sees nothing, and what is behind the result stays as it was."""
+    case = Case([(128, [128, 200, 140]), (64, [64, 100])], 4, 2, 128, 16, seed=16)
+    for cu in ([0, 5, 0], [3, 0, 5], [5, 5, 0], [0, 5, 2]):
+        assert not ops.shared_prefix_attention(**case.args(cu_groups=torch.tensor(cu, dtype=torch.int32, device=DEV))).any()
+    case.check(ops.shared_prefix_attention(**case.args()))
+
+
 def test_no_sequences_and_no_groups(ops):
     case = Case([(64, [64, 100])], 4, 2, 128, 16, seed=10)
     none = case.args(cu_groups=torch.zeros(1, dtype=torch.int32, device=DEV), prefix_lens=torch.zeros(0, dtype=torch.int32, device=DEV), max_group=0)
