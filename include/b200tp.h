@@ -343,7 +343,9 @@ int b2_philox4x32_10(const uint32_t counter[4], const uint32_t key[2], uint32_t 
  *      rank 0 to the other ranks inside its pickled "run" message
  *      (nanovllm/engine/model_runner.py:76-89: the next step's last_token of
  *      every sequence) ---------------------------------------------------------
- * buf: int64 [n] on every rank, n <= max_seqs, values >= 0.  Rank 0's values
+ * buf: int64 [n] on every rank, n <= max_seqs, values >= 0 (a negative one
+ * counts as not there yet: the other ranks wait out timeout_ms for it, take 0
+ * and report B2_WAIT_TOKENS).  Rank 0's values
  * are written into every other rank's buf by the end of the call's kernel.
  * No-op when world == 1. */
 int b2_broadcast_tokens(b2_ctx* ctx, int64_t* buf, int n, void* stream);

@@ -449,10 +449,10 @@ class ModelRunner:
                 seen = torch.where(ended.view(rows) | (state.context_lens == 0), 0, lens_t)
                 set_context(False, slot_mapping=inputs.slot_mapping, context_lens=seen, block_tables=tables_t, cu_groups=cu_t, prefix_lens=prefix_t, max_group=beams)
                 logits = self.model.compute_logits(self.model(picks.tokens.view(rows).clamp(min=0), inputs.positions))
-            if self.world > 1:  # (rank 0's, as bits)
-                bits = live.reshape(rows).view(torch.int32).to(torch.int64)
+            if self.world > 1:  # (rank 0's, as bits; the broadcast takes no negative values)
+                bits = live.reshape(rows).view(torch.int32).to(torch.int64) + (1 << 31)
                 ops.broadcast_tokens(bits)
-                live = bits.to(torch.int32).view(torch.float32).view(n, beams)
+                live = (bits - (1 << 31)).to(torch.int32).view(torch.float32).view(n, beams)
             scores, said_h, past_h = live.tolist(), said_t.view(n, beams).tolist(), past_t.view(n, beams, -1).tolist()
         finally:
             reset_context()

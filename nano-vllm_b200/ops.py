@@ -236,7 +236,8 @@ def argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tenso
 
 
 def broadcast_tokens(buf: torch.Tensor) -> torch.Tensor:
-    """Rank 0's int64 token ids into `buf` on every rank (in place)."""
+    """Rank 0's int64 token ids into `buf` on every rank (in place), at most max_seqs of them.  None of them may be negative: the other ranks take a negative value for one that has not
+    come yet, wait until the time is up, and have 0 for it."""
     assert buf.dtype == torch.int64 and buf.is_cuda and buf.is_contiguous()
     _abi.check(_lib.b2_broadcast_tokens(get_runtime().ctx, buf.data_ptr(), buf.numel(), _stream()), "b2_broadcast_tokens")
     return buf
