@@ -473,15 +473,16 @@ class ModelRunner:
             except Exception as error:  # (the other ranks are on their way to the broadcast: they get a beam that there is not)
                 failed = error
         if self.world > 1:
-            packed = torch.full((n * picks,), -1, dtype=torch.int64, device=self.device)
+            # (not negative, which the broadcast does not take: token and parent from 0 on; a parent is one of 32, which leaves bit 7 to say that there are no picks)
+            packed = torch.full((n * picks,), 1 << 7, dtype=torch.int64, device=self.device)
             if out is not None:
                 packed = ((out.tokens + 1 << 8) | (out.parents + 1 << 1) | out.finished).view(-1)
             ops.broadcast_tokens(packed)
             if self.rank != 0:
-                if int(packed[0]) < 0:
+                if int(packed[0]) == 1 << 7:
                     raise RuntimeError("rank 0 could not apply the step's rules or select its beams; its own error says why")
                 packed = packed.view(n, picks)
-                out = ops.BeamPicks(torch.zeros(n, picks, device=self.device), (packed >> 1 & 127).to(torch.int32) - 1, (packed >> 8) - 1, (packed & 1).bool())
+                out = ops.BeamPicks(torch.zeros(n, picks, device=self.device), (packed >> 1 & 63).to(torch.int32) - 1, (packed >> 8) - 1, (packed & 1).bool())
         if failed is not None:
             raise failed
         return out
