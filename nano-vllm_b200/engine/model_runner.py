@@ -10,6 +10,7 @@ in token lists and block tables (every rank must be given the same batch).
 """
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -414,10 +415,10 @@ class ModelRunner:
         needed = sum(beams * (-(-(l + max_new_tokens) // bs) - f) for l, f in zip(lens, full))
         if len(free_blocks) < needed:
             raise ValueError(f"{len(free_blocks)} free blocks: the search may need {needed}")
-        used = {b for s, l in zip(seqs, lens) for b in s.block_table[:-(-l // bs)]}
-        if len(set(free_blocks)) < len(free_blocks) or not used.isdisjoint(free_blocks) or not all(0 <= b < self.num_kvcache_blocks for b in (*free_blocks, *used)):
+        used = Counter(b for s, l in zip(seqs, lens) for b in s.block_table[:-(-l // bs)])
+        if len(set(free_blocks)) < len(free_blocks) or any(b in used for b in free_blocks) or not all(0 <= b < self.num_kvcache_blocks for b in (*free_blocks, *used)):
             raise ValueError("the free blocks must be blocks of the cache, each once, and none of the prompts'")
-        if len({s.block_table[f] for s, l, f in zip(seqs, lens, full) if l % bs}) < sum(l % bs > 0 for l in lens):
+        if any(l % bs and used[s.block_table[f]] > 1 for s, l, f in zip(seqs, lens, full)):  # (the first beams write to it, and give it back)
             raise ValueError("prompts may share full blocks only")
         # The rows before the first selection: the prompt in the first of each sequence, the others empty.
         width, most = -(-(max(lens) + max_new_tokens) // bs), max(lens)
