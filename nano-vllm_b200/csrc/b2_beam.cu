@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(BT_THREADS) beam_tables_kernel(const ReorderAr
       const bool alive = p >= 0 && p < B;
       const int from = row / B * B + (alive ? p : 0);
       const int said = alive ? min(max(0, __ldg(a.history_lens + from)), a.history_width) : 0;
-      const int64_t token = a.tokens != nullptr && alive ? __ldg(reinterpret_cast<const long long*>(a.tokens) + row) : -1;
+      const int64_t token = a.tokens != nullptr && alive ? max(-1ll, __ldg(reinterpret_cast<const long long*>(a.tokens) + row)) : -1;  // (negative: none)
       const int64_t *in = a.history + from * a.history_stride;
       int64_t* out = a.history_out + static_cast<int64_t>(row) * a.history_width;
       const int j1 = min(a.history_width, j0 + BR_HISTORY);
