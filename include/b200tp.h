@@ -576,7 +576,8 @@ int b2_beam_select(b2_ctx* ctx, const void* logits, int64_t ld, int fp32, int n,
  * context_lens tokens in the cache, in the blocks of block_tables [n * beams, bt_width] (row stride bt_stride).  Rows of a request may have a block in common, in
  * the same column; two requests may not, but for the first first_blocks[r] columns (NULL: none), which are not given back.
  *   tables_out [n * beams, bt_width]: the parent's blocks, -1 behind them.  A block with room left (the last of a length that is no multiple
- *     of block_size) stays with the first row that has it; the others get a block from the stack free_blocks[num_free] and a copy of its tokens.
+ *     of block_size) stays with the first row that has it; the others get a block from the stack free_blocks[num_free] and a copy of its tokens.  A row before that has
+ *     the block as a full one counts as the first; where one behind has it so, it stays with that one.
  *   free_blocks is updated in place: blocks of columns from first_blocks[r] (but at most the row's full blocks) on that no row has any more are put on the
  *     stack, ordered by request, column and row, and then the copies take theirs from the top, ordered by request and row; num_free_out: the new height
  *     (what is then above free_capacity is lost).

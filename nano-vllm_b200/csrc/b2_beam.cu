@@ -569,8 +569,8 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
 // beam_tables_kernel, beam_move_kernel
 //
 // Row b of a request becomes a child of its row p = parents[b].  Its table is the parent's; a block that is full is shared.  The open
-// block, which the next tokens go to, stays with the first row that has it, and the others get a copy in a block from the stack.  A block that no
-// row has any more goes onto the stack.
+// block, which the next tokens go to, stays with the first row that has it, and the others get a copy in a block from the stack; where it is full in another row, which
+// would read what the next tokens write over, all of them get a copy.  A block that no row has any more goes onto the stack.
 //
 // beam_tables_kernel: a CTA per request, 64 to 256 columns of its tables at a time through shared memory; a warp takes a column, a lane a row, and finds the rows
 // that have the same block by a match over the warp.  (A thread per column that compared its rows one after the other: 39 us instead of 11 for seven requests of 29 rows over 400 columns; the other way round with two
@@ -665,9 +665,10 @@ __global__ void __launch_bounds__(BT_THREADS) beam_tables_kernel(const ReorderAr
   if (warp == 0) {
     const int p = lane < B ? s_p[lane] : -1, len = p >= 0 ? s_len[p] : 0, column = len / bs;
     const int mine = lane < B ? s_x[lane * B + lane] : -1;
-    bool copied = false;
-    for (int b = 0; b < B; ++b)
-      if (b < lane && lane < B && mine >= 0 && s_x[b * B + lane] == mine) copied = true;
+    bool copied = false;  // a row before has the block as well, or any row as a full one
+    if (lane < B && mine >= 0)
+      for (int b = 0; b < B; ++b)
+        if (s_x[b * B + lane] == mine && (b < lane || s_len[s_p[b]] / bs > column)) copied = true;
     __syncwarp();
     const unsigned copies = __ballot_sync(0xffffffffu, copied);
     if (lane < B) {

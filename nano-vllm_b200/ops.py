@@ -348,7 +348,7 @@ def reorder_beams(parents: torch.Tensor, block_tables: torch.Tensor, context_len
                   tokens: torch.Tensor | None = None) -> BeamState:
     """Rows of n requests of some beams each become children of the rows that parents int32 [n, beams] names (-1: an empty row): block_tables [n * beams, width]
     with context_lens tokens in the cache, and the token histories [n * beams, width] with history_lens tokens, to which tokens int64 [n, beams] (beam_select's; negative:
-    none) is appended.  Full blocks are shared by all children.  A block with room left stays with its first child; the others get a copy, in
+    none) is appended.  Full blocks are shared by all children.  A block with room left stays with its first child, or with those for which it is full; the others get a copy, in
     kv_cache [..., blocks, block_size, KV heads, head_dim] (all layers' keys and values), in a block from the stack free_blocks[:num_free].  Blocks that no row has any more go
     onto the stack; the first first_blocks[r] columns of request r's tables (a prompt's full blocks, whose owner is the caller) do not.  free_blocks and kv_cache are updated
     in place, the rest comes back new.  Rows of a request may share blocks in the same column, different requests only the first_blocks.  A row for which there is no block
