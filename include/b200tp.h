@@ -560,7 +560,7 @@ int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, 
  * Request r's beam b has row r * beams + b of logits [n * beams, vocab] (bf16, or fp32 where fp32 is 1; row stride ld) and the score
  * scores[r, b].  Continuing it with token v gives scores[r, b] + logits[v] - log sum_u exp(logits[u]); outputs [n, picks]: the best of the beams * vocab
  * continuations, best first, of equal ones the lowest beam, then the lowest token.  The scores are formed in 64 bits where two continuations are near each other and rounded once.
- * A beam whose score is -inf or NaN has no continuation.  A beam with finished (NULL: none) set has one: itself, with its score and token -1.  A logit of -inf or NaN is no continuation;
+ * A beam whose score is -inf or NaN has no continuation; those of one whose score is +inf have +inf, all of them.  A beam with finished (NULL: none) set has one: itself, with its score and token -1.  A logit of -inf or NaN is no continuation;
  * +inf counts as the type's largest number.  Places for which there are no continuations: score -inf, parent -1, token -1, not finished.
  * finished_out: the parent is finished or the token is eos_token (-1: none).
  * beams <= 32, picks <= 64, n * beams <= 2^24, logits of less than 2^42 bytes.  b2_beam_select_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant;

@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     }
     // (a little lower: what lies as near as the sums' error belongs to it)
     if (any && reach > 0x00800000u) {
-      const double t = number_of(reach);
+      const double t = fminf(number_of(reach), FLT_MAX);  // (all continuations of a score of +inf are above that)
       least = t - 2 * BS_NEAR - 2.4e-7 * fabs(t);
     }
 #pragma unroll
