@@ -19,8 +19,8 @@ namespace {
 // nothing to do with each other.  Exponentials of the hardware, sums of a thread's 32 or 16 logits of a chunk in 32 bits, and of those in 64.
 //
 // beam_pick_kernel: a CTA per request.  Scores are formed in 64 bits.  The sums' error could turn the order of continuations of two beams that lie
-// closer than BS_NEAR.  Each is off by 2^-22 (2.4e-7) of an exponential, 2^-20 log(2) (6.6e-7) of an exponent's rounding where it is below 32 (what lies further down weighs less than 2^-14 even
-// over 2^18 tokens), 3e-7 of log2(e) in 24 bits there, and ten additions in 32 bits (6e-7): 1.8e-6, 3.6e-6 for the two.  Where two of those that may be among the K best are that near, their beams'
+// closer than BS_NEAR.  Each is off by 2^-22 (2.4e-7) of an exponential, 2^-20 log(2) (6.6e-7) of an exponent's rounding, which is below 32 (BS_ABOVE; what lies further down than that weighs less than 2^-14
+// even over 2^18 tokens), 3e-7 of log2(e) in 24 bits there, and ten additions in 32 bits (6e-7): 1.8e-6, 3.6e-6 for the two.  Where two of those that may be among the K best are that near, their beams'
 // sums are formed again in 64 bits from the logits, in an order and with a reference that depend on nothing but the row.
 //
 // Bound: the pass by HBM and the exponentials' unit, 31 us for 64 requests of 8 beams over 151936 tokens (60 % and 69 %); what follows by its chain of steps, 11 us there.
@@ -34,7 +34,7 @@ constexpr double BS_NEAR = 4e-6;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LOG2E_64 = 1.4426950408889634, LN2_64 = 0.6931471805599453;
 constexpr float BS_PLAIN = 65536.f;  // below this size x log2(e) is formed in 32 bits
-constexpr float BS_ABOVE = 24.f;     // the sum's reference is raised when a logit is this far above it: e^24 a term is far from too much
+constexpr float BS_ABOVE = 22.f;     // the sum's reference is raised when a logit is this far above it: exponents stay below 32, whose last bit is 2^-19
 
 struct ScanArgs {
   const void* logits;
