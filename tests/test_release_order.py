@@ -58,3 +58,11 @@ def test_columns_are_allocated_before_the_next_kernel_is_let_in():
             if "pdl_launch_dependents" in after:  # (or in a function that runs at the end)
                 assert "__syncthreads();" in after[:after.index("pdl_launch_dependents")], kernel
     assert {"tree_attention_kernel", "prefill_attention_kernel", "gemm_kernel", "gemm_tile_kernel", "gemm_pair_kernel"} <= set(found), found
+
+
+def test_reordered_tables_are_released_at_the_end():
+    """Decode attention may follow beam_move_kernel, the last of the two that write tables and lengths; the first lets nothing but the second in, which waits for all of it."""
+    text = body(code("b2_beam.cu"), "beam_move_kernel")
+    assert "pdl_launch_dependents" not in text and "return;" not in text
+    assert text.rstrip().endswith("b2::pdl_release_results();")
+    assert text.index("b2::pdl_wait();") < text.index("a.counts")
