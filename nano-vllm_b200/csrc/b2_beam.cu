@@ -344,6 +344,27 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     const int b = g / C;
     return s_kind[b] == 2 ? s.maxima[static_cast<int64_t>(row0) * C + g] : -INFINITY;
   };
+  // a bound in ordered bits, a little lower: what lies as near as the sums' error belongs to it
+  auto below = [](uint32_t bits) {
+    const double t = fminf(number_of(bits), FLT_MAX);  // (all continuations of a score of +inf are above that)
+    return t - 2 * BS_NEAR - 2.4e-7 * fabs(t);
+  };
+  // All lanes: how many of the lane's continuations in chunk g have a score from `bound` on
+  auto count_from = [&](int g, double bound) {
+    const int b = g / C;
+    if (s_kind[b] == 1) return lane == 0 && s_score[b] >= bound ? 1 : 0;
+    uint4 v[BS_VECTORS];
+    Row<T>(s, row0 + b).load(g - b * C, lane, v);
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < BS_VECTORS; ++i) {
+      float x[N];
+      Logits<T>::unpack(v[i], x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) count += score_of(b, Logits<T>::clean(x[e])) >= bound ? 1 : 0;  // (no logit in its place: next to the largest numbers a score is lost)
+    }
+    return count;
+  };
   // All lanes: the continuations in chunk g with a score from `bound` on (and perhaps some a little below) are handed to f.
   auto each = [&](int g, double bound, auto f) {
     const int b = g / C;
@@ -427,11 +448,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
       any = true;
       if (all <= K + 16) break;
     }
-    // (a little lower: what lies as near as the sums' error belongs to it)
-    if (any && reach > 0x00800000u) {
-      const double t = fminf(number_of(reach), FLT_MAX);  // (all continuations of a score of +inf are above that)
-      least = t - 2 * BS_NEAR - 2.4e-7 * fabs(t);
-    }
+    if (any && reach > 0x00800000u) least = below(reach);
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
       const int g = tid + i * BP_THREADS;
@@ -490,12 +507,43 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
     __syncthreads();
   }
   // ---- their continuations that reach the bound ----
-  for (int l = warp; l < reach; l += BP_WARPS)
-    each(s_list[l], least, [&](const Candidate& c) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < BP_COLLECT) s_got[at] = c;
-    });
-  __syncthreads();
+  auto collect = [&]() {
+    for (int l = warp; l < reach; l += BP_WARPS)
+      each(s_list[l], least, [&](const Candidate& c) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < BP_COLLECT) s_got[at] = c;
+      });
+    __syncthreads();
+  };
+  collect();
+  if (s_count > BP_COLLECT) {
+    // Fewer chunks than picks, which give no bound, or chunks that hold many of the best: a bound that at least K + 1 of the continuations reach, bit by bit from their number.
+    // (One after the other, as below, 64 picks of 50257 tokens of one beam took 3.3 ms.)
+    if (tid < 32) s_tally[tid] = 0;
+    __syncthreads();
+    uint32_t bound = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t c = bound | (1u << bit);
+      if (c > s_high + 1) continue;  // (no chunk's largest reaches it)
+      if (c < 0x00800000u) break;    // (-inf)
+      const double t = fminf(number_of(c), FLT_MAX);
+      int count = 0;
+      for (int l = warp; l < reach; l += BP_WARPS) count += count_from(s_list[l], t);
+      count = __reduce_add_sync(0xffffffffu, count);
+      if (lane == 0 && count > 0) atomicAdd(s_tally + bit, count);
+      __syncthreads();
+      const int all = s_tally[bit];
+      if (all < K + 1) continue;
+      bound = c;
+      if (all <= BP_COLLECT / 4) break;
+    }
+    if (bound != 0) {
+      least = below(bound);
+      if (tid == 0) s_count = 0;
+      __syncthreads();
+      collect();
+    }
+  }
   const int got = s_count, best = min(got, K + 1);
   const bool many = got > BP_COLLECT;
   auto rank_all = [&]() {
