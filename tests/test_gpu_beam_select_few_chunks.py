@@ -101,3 +101,17 @@ def test_time(ops):
     ordinary = microseconds(151936, 64)
     for vocab, picks in ((50257, 64), (32000, 32), (50257, 50)):
         assert microseconds(vocab, picks) <= 10 * ordinary
+
+
+@pytest.mark.parametrize("n, beams, picks, vocab, dtype", [(2, 32, 64, 151936, torch.float32), (1, 16, 5, 400003, torch.bfloat16), (1, 3, 64, 3000001, torch.bfloat16)])
+def test_more_chunks_than_a_cta_keeps(ops, n, beams, picks, vocab, dtype):
+    """Chunks whose largest logits a CTA reads again each time, since it has no registers for them; equal ones too, of which there are more than it lists."""
+    logits, scores = draw(n, beams, vocab, dtype, seed=beams)
+    check(ops, logits, scores, picks, eos=3)
+    finished = torch.zeros(n, beams, dtype=torch.bool, device=DEV)
+    finished[:, ::5] = True
+    scores[0, 1] = -INF
+    check(ops, logits, scores, picks, finished)
+    logits.fill_(-1.5)
+    logits[:, vocab - 1] = 4.0
+    check(ops, logits, torch.full_like(scores, -2.0), picks)
