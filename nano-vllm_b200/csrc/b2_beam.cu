@@ -714,9 +714,12 @@ __global__ void __launch_bounds__(BT_THREADS) beam_tables_kernel(const ReorderAr
     const int p = lane < B ? s_p[lane] : -1, len = p >= 0 ? s_len[p] : 0, column = len / bs;
     const int mine = lane < B ? s_x[lane * B + lane] : -1;
     bool copied = false;  // a row before has the block as well, or any row as a full one
-    if (lane < B && mine >= 0)
-      for (int b = 0; b < B; ++b)
-        if (s_x[b * B + lane] == mine && (b < lane || s_len[s_p[b]] / bs > column)) copied = true;
+    const int64_t end = (column + 1ll) * bs;
+#pragma unroll 4
+    for (int b = 0; b < B; ++b) {
+      const int other = __shfl_sync(0xffffffffu, len, b);
+      copied = copied || (lane < B && mine >= 0 && s_x[b * B + lane] == mine && (b < lane || other >= end));
+    }
     __syncwarp();
     const unsigned copies = __ballot_sync(0xffffffffu, copied);
     if (lane < B) {
