@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
   collect();
   if (s_count > BP_COLLECT) {
     // Fewer chunks than picks, which give no bound, or chunks that hold many of the best: a bound that at least K + 1 of the continuations reach, bit by bit from their number.
-    // (One after the other, as below, 64 picks of 50257 tokens of one beam took 3.3 ms.)
+    // (64 picks of 50257 tokens of one beam: 97 us, a round 4 to 5; one after the other, as below, 3.3 ms.)
     if (tid < 32) s_tally[tid] = 0;
     __syncthreads();
     uint32_t bound = 0;
@@ -559,7 +559,8 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
         if (rank < K + 1) s_best[rank] = mine;
       }
     } else {
-      // more than can be ranked at once (equal logits, or chunks that hold many of the best): the K + 1 best one after the other
+      // more than can be ranked at once and no bound between them (equal logits by the thousand): the K + 1 best one after the other (rows of one number, 151936 tokens: 4 picks of 4 beams 258 us, 64 of
+      // 32 beams 4 ms)
       Candidate last{INFINITY, 0.f, -1, -2};
       for (int k = 0; k < best; ++k) {
         Candidate mine = nothing;

@@ -394,7 +394,7 @@ class ModelRunner:
                     rules: dict[str, torch.Tensor] | None = None) -> list[list[tuple[list[int], float]]]:
         """The `beams` continuations of each sequence with the largest sums of log-probabilities that a beam search finds, best first, as (tokens, sum), on every rank; fewer
         where there are no more.  A continuation has max_new_tokens, or fewer and ends in eos_token.  The prompts' block tables have room for their tokens, of which
-        num_cached_tokens are in the cache and the others are computed first, in one pass.  free_blocks: what the search may use; for each sequence `beams` times the blocks that
+        num_cached_tokens are in the cache and the others are computed first, in one pass; they may share full blocks, and no others.  free_blocks: what the search may use; for each sequence `beams` times the blocks that
         max_new_tokens fill behind the prompt's full blocks.  Afterwards these blocks, and those of the prompts that are not full, hold nothing of use.  rules: arguments of ops.adjust_logits
         other than the histories (which are the prompts and the beams' tokens), a row for each sequence; looked at on rank 0 only, whose error makes every rank raise."""
         bs, n, rows = self.block_size, len(seqs), len(seqs) * beams
