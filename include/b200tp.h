@@ -513,7 +513,7 @@ int b2_tree_attention(b2_ctx* ctx, const void* q, int64_t q_stride, const void* 
  * What lies behind a context may hold anything; a sequence without tokens (0: a padded one) comes back as zeros and may have any table.  A context that is shorter than the
  * prefix shortens it for its group.  max_group: the most sequences of a group, for the argument checks: the work is dealt by cu_groups, and a larger group is served too.  scale: of either sign, or zero.
  * The sums are kept unnormalised with weights of up to 2^8: 256 * the keys seen * the largest |value| has to stay below the type's maximum (3.4e38).
- * Lengths and tables are read after earlier kernels have completed.  Calls that may run at the same time need a workspace each (16-byte aligned, contents irrelevant).
+ * Lengths and tables are read after earlier kernels have completed.  out may not overlap an input.  Calls that may run at the same time need a workspace each (16-byte aligned, contents irrelevant).
  * b2_prefix_attention_supported says (1 / 0) whether the shape is served: head_dim 64 or 128, up to 128 query heads per KV head, blocks of
  * a multiple of 16 tokens.  b2_prefix_attention_workspace: bytes, or -1 where the shape is not served; at most 1024 sequences and 512 groups, tables of less than 2^27 tokens. */
 int b2_prefix_attention_supported(int nq, int nkv, int head_dim, int block_size);
@@ -563,6 +563,7 @@ int b2_adjust_logits(const void* logits, int64_t ld, void* out, int64_t ld_out, 
  * A beam whose score is -inf or NaN has no continuation; those of one whose score is +inf have +inf, all of them.  A beam with finished (NULL: none) set has one: itself, with its score and token -1.  A logit of -inf or NaN is no continuation;
  * +inf counts as the type's largest number.  Places for which there are no continuations: score -inf, parent -1, token -1, not finished.
  * finished_out: the parent is finished or the token is eos_token (-1: none).
+ * (A score below the least number of 32 bits is -inf too, with its beam and token.)  No output may overlap an input.
  * beams <= 32, picks <= 64, n * beams <= 2^24, logits of less than 2^42 bytes.  b2_beam_select_workspace: bytes of device memory a call needs (16-byte aligned, contents irrelevant;
  * calls that may run at the same time need one each), or -1 where the shape is not served. */
 int64_t b2_beam_select_workspace(b2_ctx* ctx, int n, int beams, int vocab, int picks, int fp32);
