@@ -135,12 +135,12 @@ struct Row {
       for (int i = 0; i < BS_VECTORS; ++i) v[i] = edge(p, vocab, token(chunk, i, lane));
     }
   }
-  // sum of 2^(x log2(e) - ref) of a lane's logits, in 64 bits
+  // sum of 2^(x log2(e) - ref) of a lane's logits, in 64 bits; log2(e) is the 24-bit one of the other chunks, which a row's log is put right for as a whole
   __device__ __noinline__ double exact_sum(int chunk, int lane, double ref) const {
     double sum = 0.0;
     for (int i = 0; i < BS_VECTORS * N; ++i) {
       const int t = token(chunk, i / N, lane) + i % N;
-      if (t >= 0 && t < vocab) sum += exp2(__dmul_rn(Logits<T>::one(p + t), LOG2E_64) - ref);
+      if (t >= 0 && t < vocab) sum += exp2(__dmul_rn(Logits<T>::one(p + t), LOG2E) - ref);
     }
     return sum;
   }
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS_PER_SM) beam_scan_kernel(c
         if (!odd) sum += y + z;
       }
       if (odd) {  // infinities, NaN and very large numbers
-        raise(rint(__dmul_rn(top, LOG2E_64)));
+        raise(rint(__dmul_rn(top, LOG2E)));
         sum += r.exact_sum(c, lane, ref);
       }
     }
