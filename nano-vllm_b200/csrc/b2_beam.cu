@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const PickArgs a)
   collect();
   if (s_count > BP_COLLECT) {
     // Fewer chunks than picks, which give no bound, or chunks that hold many of the best: a bound that at least K + 1 of the continuations reach, bit by bit from their number.
-    // (64 picks of 50257 tokens of one beam: 97 us, a round 4 to 5; one after the other, as below, 3.3 ms.)
+    // (64 picks of 50257 tokens of one beam: 97 us; one after the other, as below, 3.3 ms.)
     if (tid < 32) s_tally[tid] = 0;
     __syncthreads();
     uint32_t bound = 0;
